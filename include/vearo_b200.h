@@ -227,6 +227,24 @@ int vb_layernorm_backward_accum(const vb_tensor* x, const vb_tensor* w, const vb
  * grad_out, copies them as gb instead of summing the columns again.  The sums are dropped as soon as the tensor is written to
  * through this library or released.  VB200_COLSUM_REUSE=0 in the environment switches this off. */
 
+/* ---- decoder training on packed texts (no counterpart in the reference) ---------------------
+ * Three operators that a decoder with rotary positions, grouped heads and packed texts trains with, beside vb_layernorm,
+ * vb_fused_attention and vb_cross_entropy.  Tokens are rows: queries [T, Hq, dk], keys and values [T, Hkv, dk] (strided views are
+ * read in place while the components of a head are contiguous, else copied), outputs fresh and contiguous.  The calls run
+ * on the library's device whatever device is current, and are refused (VB_ERR_UNSUPPORTED) while the compute stream is being captured.
+ *
+ * RMS norm of every head and the rotary position turn, one pass for queries and keys (k, wk, k_out all NULL: queries alone):
+ *   y = w * x / sqrt(mean(x^2) + eps);   pair j of a head turned by positions[t] * theta^(-2j / rot_dim).
+ * Pairs are components (j, j + rot_dim/2), or (2j, 2j + 1) when interleaved; components from rot_dim on are normed only
+ * (rot_dim = 0: no turn).  positions is an f32 tensor [T] and is used as it is: negative or fractional positions turn accordingly.
+ * dk <= 512. */
+int vb_qk_norm_rope(const vb_tensor* q, const vb_tensor* k_or_null, const vb_tensor* wq, const vb_tensor* wk_or_null, const vb_tensor* positions,
+                    float theta, int rot_dim, int interleaved, float eps, vb_tensor* q_out, vb_tensor* k_out);
+/* grad_q, grad_k: gradients of q_out and k_out.  gwq, gwk: sums over all tokens and heads, added in a fixed order. */
+int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k_or_null, const vb_tensor* wq, const vb_tensor* wk_or_null,
+                             const vb_tensor* positions, float theta, int rot_dim, int interleaved, float eps, const vb_tensor* grad_q,
+                             const vb_tensor* grad_k_or_null, vb_tensor* gq, vb_tensor* gk, vb_tensor* gwq, vb_tensor* gwk);
+
 /* ---- optimizer ---------------------------------------------------------------------------
  * Single-tensor steps replace the CUDA branches of Tensor::adamw_step / sgd_step
  * (vearo-core/src/tensor.rs:989-1019, 1073-1092): m, v, velocity live in device slots instead

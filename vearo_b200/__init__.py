@@ -102,6 +102,9 @@ def lib():
         L.vb_memory_stats.argtypes = [c_i64p] * 4
         L.vb_dp_unique_id.argtypes = [C.POINTER(C.c_uint8)]
         L.vb_dp_init.argtypes = [C.c_int, C.c_int, C.POINTER(C.c_uint8)]
+        T = C.POINTER(VbTensor)
+        L.vb_qk_norm_rope.argtypes = [T] * 5 + [C.c_float, C.c_int, C.c_int, C.c_float] + [T] * 2
+        L.vb_qk_norm_rope_backward.argtypes = [T] * 5 + [C.c_float, C.c_int, C.c_int, C.c_float] + [T] * 6
         _lib = L
     return _lib
 

@@ -1,0 +1,133 @@
+// The extern "C" entry points of the decoder-training operators: norm and rotation of queries and keys, causal attention over
+// packed segments, and the vocabulary projection with its cross entropy.  None of them is a `BackendOps` field of the reference
+// (its layers use learned positions, equal heads, padded batches and a separate projection and loss, crates/vearo-nn/src/lib.rs:584-621,
+// 741-793); they stand beside vb_layernorm, vb_fused_attention and vb_cross_entropy for models that need them.
+#include "common.h"
+#include "qk_norm_rope.h"
+#include <cmath>
+
+using namespace vb;
+
+namespace {
+
+// The library's device for the length of a call, whatever the calling thread had current.
+struct OnDevice {
+  int before = -1;
+  OnDevice() { if (ctx().ready && cudaGetDevice(&before) == cudaSuccess && before != ctx().device) cudaSetDevice(ctx().device); }
+  ~OnDevice() { if (ctx().ready && before >= 0 && before != ctx().device) cudaSetDevice(before); }
+};
+// Outputs of a call that may still fail: what has been allocated is given back unless done() is reached.
+struct Outputs {
+  vb_tensor* t[6] = {};
+  int n = 0;
+  int add(vb_tensor* out, int rank, const i64* dims, float** p) {
+    vb_tensor fresh;
+    VB_TRY(new_output(&fresh, rank, dims));
+    *out = fresh;
+    t[n++] = out;
+    return slot_ptr(out->slot, p);
+  }
+  void done() { n = 0; }
+  ~Outputs() { for (int i = 0; i < n; ++i) { slot_release(t[i]->slot, nullptr); t[i]->slot = 0; } }
+};
+// The arena hands scratch and outputs of one call to the next, which a replay of a captured call would not know of.
+int common_checks(const char* who) {
+  if (!ctx().ready) return set_error(VB_ERR_NOT_INIT, "vb_init has not been called");
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  VB_CUDA(cudaStreamIsCapturing(ctx().stream, &st));
+  if (st != cudaStreamCaptureStatusNone) return set_error(VB_ERR_UNSUPPORTED, std::string(who) + ": not available while the compute stream is being captured");
+  return VB_OK;
+}
+
+// [tokens, heads, dk] with contiguous components: the tensor in place, or a copy where its last dimension is strided
+int head_view(const vb_tensor* x, HeadView* v, Temp& hold) {
+  float* p;
+  VB_TRY(tensor_ptr(x, &p));
+  const i64 heads = x->dims[1], dk = x->dims[2];
+  if (dk == 1 || x->strides[2] == 1) { *v = HeadView{p, x->strides[0], x->strides[1], (int)heads}; return VB_OK; }
+  const float* c;
+  VB_TRY(contiguous_ptr(x, &c, hold));
+  *v = HeadView{c, heads * dk, dk, (int)heads};
+  return VB_OK;
+}
+
+int rope_checks(const vb_tensor* q, const vb_tensor* k, const vb_tensor* wq, const vb_tensor* wk, const vb_tensor* positions, float theta,
+                int rot_dim, float eps, RopeTable* tab) {
+  VB_CHECK(q && wq && positions && (k != nullptr) == (wk != nullptr), "q, its weight and positions are needed, and k with its weight or neither");
+  VB_CHECK(q->rank == 3 && (!k || k->rank == 3), "queries and keys must be [tokens, heads, head size]");
+  const i64 T = q->dims[0], dk = q->dims[2];
+  VB_CHECK(T >= 0 && q->dims[1] >= 1 && dk >= 1, "at least one head of at least one component");
+  VB_CHECK(!k || (k->dims[0] == T && k->dims[2] == dk && k->dims[1] >= 1), "keys must have the queries' tokens and head size");
+  VB_CHECK(wq->rank == 1 && wq->dims[0] == dk && (!wk || (wk->rank == 1 && wk->dims[0] == dk)), "norm weights must be [head size]");
+  VB_CHECK(positions->rank == 1 && positions->dims[0] == T, "positions must be [tokens]");
+  VB_CHECK(rot_dim >= 0 && rot_dim <= dk && rot_dim % 2 == 0, "rot_dim must be even and at most the head size");
+  VB_CHECK(std::isfinite(theta) && theta > 0.0f && std::isfinite(eps) && eps >= 0.0f, "theta must be positive and eps not negative");
+  if (dk > 2 * kRopeMaxPairs) return set_error(VB_ERR_UNSUPPORTED, "vb_qk_norm_rope: head sizes up to 512");
+  if (T > 0x7fffffff || q->dims[1] + (k ? k->dims[1] : 0) > 65536) return set_error(VB_ERR_UNSUPPORTED, "vb_qk_norm_rope: at most 2^31 - 1 tokens and 65536 heads");
+  for (int j = 0; j < rot_dim / 2; ++j) tab->rev[j] = std::exp(-2.0 * j / rot_dim * std::log((double)theta)) / 6.283185307179586476925286766559;
+  return VB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vb_qk_norm_rope(const vb_tensor* q, const vb_tensor* k, const vb_tensor* wq, const vb_tensor* wk, const vb_tensor* positions, float theta,
+                    int rot_dim, int interleaved, float eps, vb_tensor* q_out, vb_tensor* k_out) {
+  OnDevice on;
+  VB_TRY(common_checks("vb_qk_norm_rope"));
+  RopeTable tab;
+  VB_TRY(rope_checks(q, k, wq, wk, positions, theta, rot_dim, eps, &tab));
+  VB_CHECK(q_out && (!k || k_out), "null output tensor");
+  Temp hq, hk, h1, h2, h3;
+  HeadView vq{}, vk{};
+  const float *pwq, *pwk = nullptr, *pp;
+  VB_TRY(head_view(q, &vq, hq));
+  if (k) VB_TRY(head_view(k, &vk, hk));
+  VB_TRY(contiguous_ptr(wq, &pwq, h1));
+  if (wk) VB_TRY(contiguous_ptr(wk, &pwk, h2));
+  VB_TRY(contiguous_ptr(positions, &pp, h3));
+  Outputs outs;
+  float *oq, *ok = nullptr;
+  VB_TRY(outs.add(q_out, 3, q->dims, &oq));
+  if (k) VB_TRY(outs.add(k_out, 3, k->dims, &ok));
+  if (q->dims[0] > 0) VB_TRY(launch_norm_rope(tab, vq, vk, pwq, pwk, pp, oq, ok, q->dims[0], (int)q->dims[2], rot_dim, interleaved != 0, eps));
+  outs.done();
+  return VB_OK;
+}
+
+int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k, const vb_tensor* wq, const vb_tensor* wk, const vb_tensor* positions, float theta,
+                             int rot_dim, int interleaved, float eps, const vb_tensor* grad_q, const vb_tensor* grad_k, vb_tensor* gq, vb_tensor* gk,
+                             vb_tensor* gwq, vb_tensor* gwk) {
+  OnDevice on;
+  VB_TRY(common_checks("vb_qk_norm_rope_backward"));
+  RopeTable tab;
+  VB_TRY(rope_checks(q, k, wq, wk, positions, theta, rot_dim, eps, &tab));
+  VB_CHECK(grad_q && same_shape(*q, *grad_q) && (k ? grad_k && same_shape(*k, *grad_k) : !grad_k), "gradients must have the shapes of q and k");
+  VB_CHECK(gq && gwq && (!k || (gk && gwk)), "null output tensor");
+  Temp hq, hk, hgq, hgk, h1, h2, h3;
+  HeadView vq{}, vk{}, vgq{}, vgk{};
+  const float *pwq, *pwk = nullptr, *pp;
+  VB_TRY(head_view(q, &vq, hq));
+  VB_TRY(head_view(grad_q, &vgq, hgq));
+  if (k) { VB_TRY(head_view(k, &vk, hk)); VB_TRY(head_view(grad_k, &vgk, hgk)); }
+  VB_TRY(contiguous_ptr(wq, &pwq, h1));
+  if (wk) VB_TRY(contiguous_ptr(wk, &pwk, h2));
+  VB_TRY(contiguous_ptr(positions, &pp, h3));
+  Outputs outs;
+  float *pgq, *pgk = nullptr, *pgwq, *pgwk = nullptr;
+  const i64 dk = q->dims[2];
+  VB_TRY(outs.add(gq, 3, q->dims, &pgq));
+  VB_TRY(outs.add(gwq, 1, &dk, &pgwq));
+  if (k) { VB_TRY(outs.add(gk, 3, k->dims, &pgk)); VB_TRY(outs.add(gwk, 1, &dk, &pgwk)); }
+  if (q->dims[0] > 0) {
+    VB_TRY(launch_norm_rope_backward(tab, vq, vk, vgq, vgk, pwq, pwk, pp, pgq, pgk, pgwq, pgwk, q->dims[0], (int)dk, rot_dim, interleaved != 0, eps));
+  } else {
+    VB_TRY(launch_fill(pgwq, 0.0f, dk));
+    if (k) VB_TRY(launch_fill(pgwk, 0.0f, dk));
+  }
+  outs.done();
+  return VB_OK;
+}
+
+}  // extern "C"
