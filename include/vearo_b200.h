@@ -244,6 +244,15 @@ int vb_qk_norm_rope(const vb_tensor* q, const vb_tensor* k_or_null, const vb_ten
 int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k_or_null, const vb_tensor* wq, const vb_tensor* wk_or_null,
                              const vb_tensor* positions, float theta, int rot_dim, int interleaved, float eps, const vb_tensor* grad_q,
                              const vb_tensor* grad_k_or_null, vb_tensor* gq, vb_tensor* gk, vb_tensor* gwq, vb_tensor* gwk);
+/* The vocabulary projection and its softmax cross entropy without the logits in memory: vb_linear (no bias) followed by
+ * vb_cross_entropy.  x: [.., D] (rows = all leading dims), weight: [V, D], targets: as many classes as rows.  loss (shape [1]) is the
+ * mean over the rows whose target is not ignore_index; 0 when there are none.  A negative or too large target that is not
+ * ignore_index sets the device error flag, and its row is left out.  lse (may be NULL; [rows]): log of the sum of exponentials of every
+ * row, which the backward call wants.  The backward call forms the logits again, a piece of the vocabulary at a time (at most
+ * half a gigabyte of workspace for up to 2^19 rows); gx or gw may be NULL.  V <= 2^24. */
+int vb_linear_cross_entropy(const vb_tensor* x, const vb_tensor* weight, const vb_tensor* targets, int64_t ignore_index, vb_tensor* loss, vb_tensor* lse_or_null);
+int vb_linear_cross_entropy_backward(const vb_tensor* x, const vb_tensor* weight, const vb_tensor* targets, int64_t ignore_index, const vb_tensor* lse,
+                                     const vb_tensor* grad_out, vb_tensor* gx_or_null, vb_tensor* gw_or_null);
 
 /* ---- optimizer ---------------------------------------------------------------------------
  * Single-tensor steps replace the CUDA branches of Tensor::adamw_step / sgd_step

@@ -3,6 +3,7 @@
 // (its layers use learned positions, equal heads, padded batches and a separate projection and loss, crates/vearo-nn/src/lib.rs:584-621,
 // 741-793); they stand beside vb_layernorm, vb_fused_attention and vb_cross_entropy for models that need them.
 #include "common.h"
+#include "head_loss.h"
 #include "qk_norm_rope.h"
 #include <cmath>
 
@@ -68,6 +69,20 @@ int rope_checks(const vb_tensor* q, const vb_tensor* k, const vb_tensor* wq, con
   return VB_OK;
 }
 
+int head_loss_checks(const vb_tensor* x, const vb_tensor* w, const vb_tensor* targets, i64* n) {
+  VB_CHECK(x && w && targets, "null tensor");
+  VB_CHECK(x->rank >= 2 && w->rank == 2 && targets->rank >= 1, "x must be [.., width], weight [vocabulary, width], targets [..]");
+  const i64 d = x->dims[x->rank - 1], v = w->dims[0];
+  VB_CHECK(d >= 1 && w->dims[1] == d, "Incompatible dimensions for matmul");
+  VB_CHECK(v >= 1, "Vocabulary size must be greater than 0");
+  *n = numel(*x) / d;
+  VB_CHECK(*n > 0, "Batch size must be greater than 0");
+  VB_CHECK(numel(*targets) == *n, "Targets shape must match batch size");
+  if (v > (i64)1 << 24) return set_error(VB_ERR_UNSUPPORTED, "vb_linear_cross_entropy: classes beyond 2^24 are not whole numbers of f32");
+  if (*n > (i64)1 << 30 || d > (i64)1 << 30) return set_error(VB_ERR_UNSUPPORTED, "vb_linear_cross_entropy: at most 2^30 rows and columns");
+  return VB_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -126,6 +141,48 @@ int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k, const vb_te
     VB_TRY(launch_fill(pgwq, 0.0f, dk));
     if (k) VB_TRY(launch_fill(pgwk, 0.0f, dk));
   }
+  outs.done();
+  return VB_OK;
+}
+
+int vb_linear_cross_entropy(const vb_tensor* x, const vb_tensor* weight, const vb_tensor* targets, int64_t ignore_index, vb_tensor* loss, vb_tensor* lse) {
+  OnDevice on;
+  VB_TRY(common_checks("vb_linear_cross_entropy"));
+  i64 n;
+  VB_TRY(head_loss_checks(x, weight, targets, &n));
+  VB_CHECK(loss, "null output tensor");
+  Temp hx, hw, ht, hl;
+  const float *px, *pw, *pt;
+  VB_TRY(contiguous_ptr(x, &px, hx)); VB_TRY(contiguous_ptr(weight, &pw, hw)); VB_TRY(contiguous_ptr(targets, &pt, ht));
+  Outputs outs;
+  float *ploss, *plse;
+  const i64 one = 1;
+  VB_TRY(outs.add(loss, 1, &one, &ploss));
+  if (lse) VB_TRY(outs.add(lse, 1, &n, &plse));
+  else { VB_TRY(scratch_alloc((size_t)n * sizeof(float), &hl.p)); plse = (float*)hl.p; }
+  VB_TRY(launch_head_loss(px, pw, pt, ignore_index, ploss, plse, n, weight->dims[1], weight->dims[0]));
+  outs.done();
+  return VB_OK;
+}
+
+int vb_linear_cross_entropy_backward(const vb_tensor* x, const vb_tensor* weight, const vb_tensor* targets, int64_t ignore_index, const vb_tensor* lse,
+                                     const vb_tensor* grad_out, vb_tensor* gx, vb_tensor* gw) {
+  OnDevice on;
+  VB_TRY(common_checks("vb_linear_cross_entropy_backward"));
+  i64 n;
+  VB_TRY(head_loss_checks(x, weight, targets, &n));
+  VB_CHECK(lse && grad_out && numel(*lse) == n, "lse must be [rows]");
+  VB_CHECK(numel(*grad_out) == 1, "grad_out must be a scalar");
+  Temp hx, hw, ht, hl;
+  const float *px, *pw, *pt, *pl;
+  float* pg;
+  VB_TRY(contiguous_ptr(x, &px, hx)); VB_TRY(contiguous_ptr(weight, &pw, hw)); VB_TRY(contiguous_ptr(targets, &pt, ht)); VB_TRY(contiguous_ptr(lse, &pl, hl));
+  VB_TRY(tensor_ptr(grad_out, &pg));
+  Outputs outs;
+  float *pgx = nullptr, *pgw = nullptr;
+  if (gx) VB_TRY(outs.add(gx, x->rank, x->dims, &pgx));
+  if (gw) VB_TRY(outs.add(gw, 2, weight->dims, &pgw));
+  if (gx || gw) VB_TRY(launch_head_loss_backward(px, pw, pt, ignore_index, pl, pg, pgx, pgw, n, weight->dims[1], weight->dims[0]));
   outs.done();
   return VB_OK;
 }

@@ -1,0 +1,46 @@
+// Products of f32 matrices held as half-precision pairs (split16.cuh), and the forms of the vocabulary product that the
+// projection-with-loss needs (gemm16.cu).
+#pragma once
+#include <cuda.h>
+#include "common.h"
+
+namespace vb {
+
+// [rows, cols] as two half planes (hi, then lo `plane` halves later), rows `ld` halves apart; inv: 2^-e of each 128 x 128 block.
+struct Split16 { void* planes; float* inv; i64 rows, cols, ld, plane, inv_ld; };
+inline size_t split16_bytes(i64 rows, i64 cols) {
+  const i64 ld = (cols + 7) / 8 * 8;
+  return (size_t)(2 * rows * ld) * 2 + 16 + (size_t)(((rows + 127) / 128) * ((cols + 127) / 128)) * sizeof(float);
+}
+Split16 split16_at(void* mem, i64 rows, i64 cols);                                                // lays the pair out in memory of that size
+struct SplitJob { const float* x; Split16 to; };                                                 // x: [rows, cols] contiguous
+int launch_split16(const SplitJob* jobs, int n);                                                  // n <= 2, one launch
+
+constexpr int kNoTarget = -(1 << 30);
+
+// What a product does with its tiles.
+enum class Tile16 {
+  Store,      // out (+)= alpha * product
+  RowStats,   // per row and 128 columns the (max, sum of exp) of the product, and the product at the row's target column
+  LossGrad    // exp(product - lse) - [column is the target], times 2^14, as half planes (rows without a target: 0)
+};
+// out[m, n] = sum_k A[m, k] B[n, k].  An operand is K-major ([mn, k] in memory) or, mn true, [k, mn] in memory; its extents and
+// scales are those of the Split16 (inv null: all 1).
+struct Op16 { Split16 s; bool mn; };
+struct Product16 {
+  Op16 a, b;
+  i64 M, N, K;
+  // Store
+  float* out; i64 ldo; bool add;
+  const float* alpha; float alpha_host;          // alpha (device, null: 1) times alpha_host
+  // RowStats / LossGrad
+  const int* target;                             // [M] column of the row's target, kNoTarget: none (LossGrad: the row is left out)
+  i64 col0;                                      // what the target columns call column 0 of this product
+  float2* stats;                                 // [ceil(N / 128), M]
+  float* target_value;                           // [M], written where the target lies in this product
+  const float* lse;                              // [M]
+  Split16 grad;                                  // [M, N]
+};
+int launch_gemm16(Tile16 what, const Product16* products, int n);      // n <= 2 (Store), independent of one another, one launch
+
+}  // namespace vb

@@ -1,0 +1,166 @@
+// The vocabulary projection with its softmax cross entropy, forward and backward, without the logits in memory.
+//
+//   z = x W^T,  lse_n = log sum_v exp z_nv,  loss = mean over rows with a target of (lse_n - z_n,target)
+//   dz = (exp(z - lse) - onehot) g / count,   dx = dz W,   dW = dz^T x
+//
+// Forward: one product whose tiles leave (max, sum of exp) for each row and 128 columns, 8 bytes where the logits would be 512, and
+// the target's logit; a second kernel joins the pairs of a row.  Backward: pieces of the vocabulary; a piece's logits are formed
+// again and leave the tensor core as dz in half-precision planes (the operand of the two products that follow), and one launch
+// adds the piece to dx and writes its rows of dW.  Tensor-bound: 2 N V D and 6 N V D operations, three instructions each (gemm16.cu).
+#include "gemm16.h"
+#include "head_loss.h"
+
+namespace vb {
+namespace {
+
+// Target columns as integers.  Rows whose target is `ignore` are left out; a negative or too large one is reported and left out.
+__device__ __forceinline__ int read_target(float v, i64 ignore, i64 vocab, int* err) {
+  if (v == (float)ignore || (fabsf(v) < 1e9f && (i64)roundf(v) == ignore)) return kNoTarget;
+  if (!(v > -0.5f)) { atomicOr(err, ERRBIT_NEG_ID); return kNoTarget; }
+  if (!(roundf(v) < (float)vocab)) { atomicOr(err, ERRBIT_OOB_ID); return kNoTarget; }
+  return (int)roundf(v);
+}
+// One CTA: every row's target and, for the backward pass, coef = g / (rows with a target).
+__global__ void __launch_bounds__(1024) k_targets(const float* __restrict__ targets, i64 n, i64 ignore, i64 vocab, int* __restrict__ out,
+                                                  const float* __restrict__ g, float* __restrict__ coef, int* err) {
+  __shared__ int red[32];
+  int live = 0;
+  for (i64 i = threadIdx.x; i < n; i += 1024) {
+    const int t = read_target(targets[i], ignore, vocab, err);
+    out[i] = t;
+    live += t != kNoTarget;
+  }
+  if (!coef) return;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) live += __shfl_xor_sync(0xffffffffu, live, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = live;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int c = 0;
+    for (int i = 0; i < 32; ++i) c += red[i];
+    *coef = *g / (float)(c > 0 ? c : 1);
+  }
+}
+// lse and the row's loss from its pairs: 32 rows x 32 pair lanes a CTA, pairs joined in a fixed order
+__global__ void __launch_bounds__(1024) k_join_stats(const float2* __restrict__ stats, const float* __restrict__ target_value, const int* __restrict__ target,
+                                                     float* __restrict__ lse, float* __restrict__ nll, int n, int pairs) {
+  __shared__ float sm[32][33], ss[32][33];
+  const int row = blockIdx.x * 32 + threadIdx.x;
+  float m = -INFINITY, s = 0.0f;
+  if (row < n) {
+    for (int i = threadIdx.y; i < pairs; i += 32) {
+      const float2 a = stats[(i64)i * n + row];
+      if (a.x > m) { s = s * expf(m - a.x) + a.y; m = a.x; }
+      else if (a.y != 0.0f) s += a.y * expf(a.x - m);          // (a pair of NaN sum keeps it)
+    }
+  }
+  sm[threadIdx.y][threadIdx.x] = m; ss[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  // transposed: a warp joins the 32 partial pairs of one row
+  m = sm[threadIdx.x][threadIdx.y]; s = ss[threadIdx.x][threadIdx.y];
+  float top = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  s = top > -INFINITY && m > -INFINITY ? s * expf(m - top) : s;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  const int r = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && r < n) {
+    const float l = top + logf(s);
+    lse[r] = l;
+    nll[r] = target[r] == kNoTarget ? 0.0f : l - target_value[r];
+  }
+}
+__global__ void __launch_bounds__(1024) k_mean_loss(const float* __restrict__ nll, const int* __restrict__ target, i64 n, float* __restrict__ loss) {
+  __shared__ float red[32];
+  __shared__ int cnt[32];
+  float s = 0.0f;
+  int live = 0;
+  for (i64 i = threadIdx.x; i < n; i += 1024) { s += nll[i]; live += target[i] != kNoTarget; }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); live += __shfl_xor_sync(0xffffffffu, live, o); }
+  if ((threadIdx.x & 31) == 0) { red[threadIdx.x >> 5] = s; cnt[threadIdx.x >> 5] = live; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float t = 0.0f;
+    int c = 0;
+    for (int i = 0; i < 32; ++i) { t += red[i]; c += cnt[i]; }
+    *loss = c > 0 ? t / (float)c : 0.0f;
+  }
+}
+
+// Half-precision planes of a piece of dz: at most half a gigabyte of them at a time.
+constexpr i64 kPieceBytes = (i64)512 << 20;
+
+}  // namespace
+
+int launch_head_loss(const float* x, const float* w, const float* targets, i64 ignore, float* loss, float* lse, i64 n, i64 d, i64 v) {
+  Temp hx, hw, hs, hr;
+  const i64 pairs = (v + 127) / 128;
+  VB_TRY(scratch_alloc(split16_bytes(n, d), &hx.p));
+  VB_TRY(scratch_alloc(split16_bytes(v, d), &hw.p));
+  VB_TRY(scratch_alloc((size_t)(pairs * n) * sizeof(float2), &hs.p));
+  VB_TRY(scratch_alloc((size_t)n * 12, &hr.p));
+  float* nll = (float*)hr.p; float* tv = nll + n; int* tgt = (int*)(tv + n);
+  const Split16 sx = split16_at(hx.p, n, d), sw = split16_at(hw.p, v, d);
+  const SplitJob jobs[2] = {{x, sx}, {w, sw}};
+  VB_TRY(launch_split16(jobs, 2));
+  k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, nullptr, nullptr, ctx().d_err);
+  VB_LAUNCH_CHECK();
+  Product16 g{};
+  g.a = Op16{sx, false}; g.b = Op16{sw, false}; g.M = n; g.N = v; g.K = d;
+  g.target = tgt; g.stats = (float2*)hs.p; g.target_value = tv;
+  VB_TRY(launch_gemm16(Tile16::RowStats, &g, 1));
+  k_join_stats<<<(unsigned)((n + 31) / 32), dim3(32, 32), 0, ctx().stream>>>((const float2*)hs.p, tv, tgt, lse, nll, (int)n, (int)pairs);
+  VB_LAUNCH_CHECK();
+  k_mean_loss<<<1, 1024, 0, ctx().stream>>>(nll, tgt, n, loss);
+  VB_LAUNCH_CHECK();
+  return VB_OK;
+}
+
+int launch_head_loss_backward(const float* x, const float* w, const float* targets, i64 ignore, const float* lse, const float* g, float* gx, float* gw,
+                              i64 n, i64 d, i64 v) {
+  Temp hx, hw, hz, ht;
+  i64 piece = kPieceBytes / (4 * n) / 256 * 256;
+  if (piece < 256) piece = 256;
+  const i64 pieces = (v + piece - 1) / piece;
+  piece = ((v + pieces - 1) / pieces + 255) / 256 * 256;
+  if (piece > v) piece = v;
+  VB_TRY(scratch_alloc(split16_bytes(n, d), &hx.p));
+  VB_TRY(scratch_alloc(split16_bytes(v, d), &hw.p));
+  VB_TRY(scratch_alloc(split16_bytes(n, piece), &hz.p));
+  VB_TRY(scratch_alloc((size_t)n * 4 + 16, &ht.p));
+  float* coef = (float*)ht.p; int* tgt = (int*)(coef + 4);
+  const Split16 sx = split16_at(hx.p, n, d), sw = split16_at(hw.p, v, d);
+  const SplitJob jobs[2] = {{x, sx}, {w, sw}};
+  VB_TRY(launch_split16(jobs, 2));
+  k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, g, coef, ctx().d_err);
+  VB_LAUNCH_CHECK();
+  for (i64 v0 = 0; v0 < v; v0 += piece) {
+    const i64 vc = v - v0 < piece ? v - v0 : piece;
+    Split16 wc = sw;                                     // this piece's rows of W
+    wc.planes = (uint16_t*)sw.planes + v0 * sw.ld; wc.inv = sw.inv + v0 / 128 * sw.inv_ld; wc.rows = vc;
+    Split16 z = split16_at(hz.p, n, vc);
+    Product16 f{};
+    f.a = Op16{sx, false}; f.b = Op16{wc, false}; f.M = n; f.N = vc; f.K = d;
+    f.target = tgt; f.col0 = v0; f.lse = lse; f.grad = z;
+    VB_TRY(launch_gemm16(Tile16::LossGrad, &f, 1));
+    z.inv = nullptr;
+    Product16 b[2] = {};
+    int nb = 0;
+    if (gx) {
+      Product16& q = b[nb++];
+      q.a = Op16{z, false}; q.b = Op16{wc, true}; q.M = n; q.N = d; q.K = vc;
+      q.out = gx; q.ldo = d; q.add = v0 > 0; q.alpha = coef; q.alpha_host = 1.0f / 16384.0f;
+    }
+    if (gw) {
+      Product16& q = b[nb++];
+      q.a = Op16{z, true}; q.b = Op16{sx, true}; q.M = vc; q.N = d; q.K = n;
+      q.out = gw + v0 * d; q.ldo = d; q.alpha = coef; q.alpha_host = 1.0f / 16384.0f;
+    }
+    if (nb) VB_TRY(launch_gemm16(Tile16::Store, b, nb));
+  }
+  return VB_OK;
+}
+
+}  // namespace vb
