@@ -244,6 +244,15 @@ int vb_qk_norm_rope(const vb_tensor* q, const vb_tensor* k_or_null, const vb_ten
 int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k_or_null, const vb_tensor* wq, const vb_tensor* wk_or_null,
                              const vb_tensor* positions, float theta, int rot_dim, int interleaved, float eps, const vb_tensor* grad_q,
                              const vb_tensor* grad_k_or_null, vb_tensor* gq, vb_tensor* gk, vb_tensor* gwq, vb_tensor* gwk);
+/* Causal attention with grouped heads over packed segments.  q: [T, Hq, dk]; k, v: [T, Hkv, dk], Hq a multiple of Hkv (query head h
+ * reads key head h / (Hq / Hkv)).  starts: f32 tensor [segments + 1] of row offsets, not decreasing: segment i is the rows
+ * [starts[i], starts[i + 1]), and a row sees the rows of its segment up to itself.  Segments may be empty; rows before the first or
+ * behind the last belong to none: their output and gradients are 0, their lse is -infinity.  Offsets that decrease or leave [0, T] set the
+ * device error flag.  Scores are scale * q.k; p = exp(score - lse), without the 1e-9 of vb_fused_attention.  lse (may be NULL) is
+ * [Hq, T], the natural log of a row's sum of exponentials; the backward call wants it and out.  dk <= 128, T <= 2^24. */
+int vb_segment_attention(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, vb_tensor* out, vb_tensor* lse_or_null);
+int vb_segment_attention_backward(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, const vb_tensor* out,
+                                  const vb_tensor* lse, const vb_tensor* grad_out, vb_tensor* dq, vb_tensor* dk, vb_tensor* dv);
 /* The vocabulary projection and its softmax cross entropy without the logits in memory: vb_linear (no bias) followed by
  * vb_cross_entropy.  x: [.., D] (rows = all leading dims), weight: [V, D], targets: as many classes as rows.  loss (shape [1]) is the
  * mean over the rows whose target is not ignore_index; 0 when there are none.  A negative or too large target that is not

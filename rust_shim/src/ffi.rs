@@ -110,6 +110,8 @@ unsafe extern "C" {
     // decoder training on packed texts
     pub fn vb_qk_norm_rope(q: T, k_or_null: T, wq: T, wk_or_null: T, positions: T, theta: f32, rot_dim: c_int, interleaved: c_int, eps: f32, q_out: O, k_out: O) -> c_int;
     pub fn vb_qk_norm_rope_backward(q: T, k_or_null: T, wq: T, wk_or_null: T, positions: T, theta: f32, rot_dim: c_int, interleaved: c_int, eps: f32, grad_q: T, grad_k_or_null: T, gq: O, gk: O, gwq: O, gwk: O) -> c_int;
+    pub fn vb_segment_attention(q: T, k: T, v: T, starts: T, scale: f32, out: O, lse_or_null: O) -> c_int;
+    pub fn vb_segment_attention_backward(q: T, k: T, v: T, starts: T, scale: f32, out: T, lse: T, grad_out: T, dq: O, dk: O, dv: O) -> c_int;
     pub fn vb_linear_cross_entropy(x: T, weight: T, targets: T, ignore_index: i64, loss: O, lse_or_null: O) -> c_int;
     pub fn vb_linear_cross_entropy_backward(x: T, weight: T, targets: T, ignore_index: i64, lse: T, grad_out: T, gx_or_null: O, gw_or_null: O) -> c_int;
     // optimizer

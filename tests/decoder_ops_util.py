@@ -91,3 +91,64 @@ def norm_rope_grad(x, w, pos, theta, rot, inter, eps, g):
     inv = 1.0 / np.sqrt((x * x).mean(-1, keepdims=True) + eps)
     xh = x * inv
     return inv * (g * w - xh * (g * w * xh).mean(-1, keepdims=True)), (g * xh).sum((0, 1))
+
+
+def segment_attention(q, k, v, starts, scale, g=None, err=False):
+    """(out, lse[, dq, dk, dv]) in 64 bits and, with err, a bound for every element of each.
+
+    Bounds, in units of U: a score carries 57 of scale sum |q k| (split 2^-22 twice, the dropped term, 24 truncating additions a run);
+    p = exp(s - lse) turns the score's error and two roundings of |s| + |lse| + 20 into a relative one, plus 4 for the exponential;
+    a sum over keys adds 60 (splitting and truncation) and 3 for every 128 keys (rescaling, additions) of its terms' absolute sum, and
+    what the halves' subnormals lose: 2^-38 of the largest weight for each key.  dS is held on a scale set by the row and value lengths
+    of a block: 2^-36 of the largest |do| |v| product a key."""
+    T, hq, dk = q.shape
+    hk = k.shape[1]
+    grp = hq // hk
+    f = lambda x: x.astype(np.float64)  # noqa: E731
+    q, k, v = f(q), f(k), f(v)
+    o, lse = np.zeros((T, hq, dk)), np.full((hq, T), -np.inf)
+    eo, el = np.zeros((T, hq, dk)), np.zeros((hq, T))
+    dq, dk_, dv = np.zeros((T, hq, dk)), np.zeros((T, hk, dk)), np.zeros((T, hk, dk))
+    edq, edk, edv = np.zeros((T, hq, dk)), np.zeros((T, hk, dk)), np.zeros((T, hk, dk))
+    g = None if g is None else f(g)
+    a = np.abs
+    top = 0.0 if g is None else np.sqrt((g * g).sum(-1)).max() * np.sqrt((v * v).sum(-1)).max()
+    for b, e in zip(starts[:-1], starts[1:]):
+        b, e = int(b), int(e)
+        n = e - b
+        if n <= 0:
+            continue
+        mask = np.tril(np.ones((n, n), bool))
+        for h in range(hq):
+            Q, K, V = q[b:e, h], k[b:e, h // grp], v[b:e, h // grp]
+            s = np.where(mask, Q @ K.T * scale, -np.inf)
+            m = s.max(1, keepdims=True)
+            L = m + np.log(np.exp(s - m).sum(1, keepdims=True))
+            p = np.exp(s - L)
+            o[b:e, h], lse[h, b:e] = p @ V, L[:, 0]
+            es = 57 * U * scale * (a(Q) @ a(K).T)
+            sa = np.where(mask, a(s), 0.0)
+            r = es + (4 + 2 * (sa + a(L) + 20)) * U
+            e_l = (p * r).sum(1, keepdims=True) + (20 + n / 40 + 2 * a(L)) * U
+            r = r + e_l
+            steps = (60 + 3 * n / 128 + 10) * U
+            eo[b:e, h] = (p * (r + steps)) @ a(V) + 2.0 ** -38 * (mask @ a(V))
+            el[h, b:e] = e_l[:, 0]
+            if g is None:
+                continue
+            G = g[b:e, h]
+            dp, delta = G @ V.T, (G * o[b:e, h]).sum(1, keepdims=True)
+            ds = p * (dp - delta) * scale
+            dq[b:e, h] = ds @ K
+            dk_[b:e, h // grp] += ds.T @ Q
+            dv[b:e, h // grp] += p.T @ G
+            e_dp = 57 * U * (a(G) @ a(V).T)
+            e_delta = (a(G) * (eo[b:e, h] + dk * U * a(o[b:e, h]))).sum(1, keepdims=True)
+            e_ds = scale * mask * (p * (r * a(dp - delta) + e_dp + e_delta + 8 * U * (a(dp) + a(delta))) + 2.0 ** -36 * top)
+            edq[b:e, h] = e_ds @ a(K) + steps * (a(ds) @ a(K))
+            gsteps = steps * grp
+            edk[b:e, h // grp] += e_ds.T @ a(Q) + gsteps * (a(ds).T @ a(Q))
+            edv[b:e, h // grp] += (p * (r + gsteps)).T @ a(G) + 2.0 ** -38 * (mask.T @ a(G))
+    vals = (o, lse) if g is None else (o, lse, dq, dk_, dv)
+    errs = (eo, el) if g is None else (eo, el, edq, edk, edv)
+    return (vals, errs) if err else vals

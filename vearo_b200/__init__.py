@@ -105,6 +105,8 @@ def lib():
         T = C.POINTER(VbTensor)
         L.vb_qk_norm_rope.argtypes = [T] * 5 + [C.c_float, C.c_int, C.c_int, C.c_float] + [T] * 2
         L.vb_qk_norm_rope_backward.argtypes = [T] * 5 + [C.c_float, C.c_int, C.c_int, C.c_float] + [T] * 6
+        L.vb_segment_attention.argtypes = [T] * 4 + [C.c_float] + [T] * 2
+        L.vb_segment_attention_backward.argtypes = [T] * 4 + [C.c_float] + [T] * 6
         L.vb_linear_cross_entropy.argtypes = [T] * 3 + [C.c_int64] + [T] * 2
         L.vb_linear_cross_entropy_backward.argtypes = [T] * 3 + [C.c_int64] + [T] * 4
         _lib = L

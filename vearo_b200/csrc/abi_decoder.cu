@@ -5,6 +5,7 @@
 #include "common.h"
 #include "head_loss.h"
 #include "qk_norm_rope.h"
+#include "segment_attention.h"
 #include <cmath>
 
 using namespace vb;
@@ -66,6 +67,27 @@ int rope_checks(const vb_tensor* q, const vb_tensor* k, const vb_tensor* wq, con
   if (dk > 2 * kRopeMaxPairs) return set_error(VB_ERR_UNSUPPORTED, "vb_qk_norm_rope: head sizes up to 512");
   if (T > 0x7fffffff || q->dims[1] + (k ? k->dims[1] : 0) > 65536) return set_error(VB_ERR_UNSUPPORTED, "vb_qk_norm_rope: at most 2^31 - 1 tokens and 65536 heads");
   for (int j = 0; j < rot_dim / 2; ++j) tab->rev[j] = std::exp(-2.0 * j / rot_dim * std::log((double)theta)) / 6.283185307179586476925286766559;
+  return VB_OK;
+}
+
+int segment_checks(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, SegShape* s) {
+  VB_CHECK(q && k && v && starts, "null tensor");
+  VB_CHECK(q->rank == 3 && k->rank == 3 && same_shape(*k, *v), "queries must be [tokens, heads, head size], keys and values alike");
+  VB_CHECK(q->dims[0] == k->dims[0] && q->dims[2] == k->dims[2], "keys must have the queries' tokens and head size");
+  VB_CHECK(q->dims[1] >= 1 && k->dims[1] >= 1 && q->dims[1] % k->dims[1] == 0, "the number of query heads must be a multiple of the number of key heads");
+  VB_CHECK(q->dims[2] >= 1, "head size must be greater than 0");
+  VB_CHECK(starts->rank == 1 && starts->dims[0] >= 1, "starts must be [segments + 1]");
+  VB_CHECK(std::isfinite(scale) && scale > 0.0f, "scale must be positive");
+  if (q->dims[2] > kSegMaxHead) return set_error(VB_ERR_UNSUPPORTED, "vb_segment_attention: head sizes up to 128");
+  if (q->dims[0] > (i64)1 << 24 || starts->dims[0] > (i64)1 << 24) return set_error(VB_ERR_UNSUPPORTED, "vb_segment_attention: offsets beyond 2^24 are not whole numbers of f32");
+  if (q->dims[1] > 65535) return set_error(VB_ERR_UNSUPPORTED, "vb_segment_attention: at most 65535 heads");
+  *s = SegShape{q->dims[0], (int)q->dims[1], (int)k->dims[1], (int)q->dims[2], scale};
+  return VB_OK;
+}
+int seg_view(const vb_tensor* x, SegHeads* v, Temp& hold) {
+  HeadView h;
+  VB_TRY(head_view(x, &h, hold));
+  *v = SegHeads{h.p, h.st, h.sh};
   return VB_OK;
 }
 
@@ -141,6 +163,49 @@ int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k, const vb_te
     VB_TRY(launch_fill(pgwq, 0.0f, dk));
     if (k) VB_TRY(launch_fill(pgwk, 0.0f, dk));
   }
+  outs.done();
+  return VB_OK;
+}
+
+int vb_segment_attention(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, vb_tensor* out, vb_tensor* lse) {
+  OnDevice on;
+  VB_TRY(common_checks("vb_segment_attention"));
+  SegShape s;
+  VB_TRY(segment_checks(q, k, v, starts, scale, &s));
+  VB_CHECK(out, "null output tensor");
+  Temp hq, hk, hv, hs;
+  SegHeads vq, vk, vv;
+  const float* ps;
+  VB_TRY(seg_view(q, &vq, hq)); VB_TRY(seg_view(k, &vk, hk)); VB_TRY(seg_view(v, &vv, hv));
+  VB_TRY(contiguous_ptr(starts, &ps, hs));
+  Outputs outs;
+  float *po, *pl = nullptr;
+  const i64 ld[2] = {s.hq, s.T};
+  VB_TRY(outs.add(out, 3, q->dims, &po));
+  if (lse) VB_TRY(outs.add(lse, 2, ld, &pl));
+  if (s.T > 0) VB_TRY(launch_segment_attention(s, vq, vk, vv, ps, starts->dims[0] - 1, po, pl));
+  outs.done();
+  return VB_OK;
+}
+
+int vb_segment_attention_backward(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, const vb_tensor* out,
+                                  const vb_tensor* lse, const vb_tensor* grad_out, vb_tensor* dq, vb_tensor* dk, vb_tensor* dv) {
+  OnDevice on;
+  VB_TRY(common_checks("vb_segment_attention_backward"));
+  SegShape s;
+  VB_TRY(segment_checks(q, k, v, starts, scale, &s));
+  VB_CHECK(out && lse && grad_out && same_shape(*q, *out) && same_shape(*q, *grad_out), "out and grad_out must have the shape of q");
+  VB_CHECK(lse->rank == 2 && lse->dims[0] == s.hq && lse->dims[1] == s.T, "lse must be [heads, tokens]");
+  VB_CHECK(dq && dk && dv, "null output tensor");
+  Temp hq, hk, hv, hs, ho, hl, hg;
+  SegHeads vq, vk, vv, vo, vg;
+  const float *ps, *pl;
+  VB_TRY(seg_view(q, &vq, hq)); VB_TRY(seg_view(k, &vk, hk)); VB_TRY(seg_view(v, &vv, hv)); VB_TRY(seg_view(out, &vo, ho)); VB_TRY(seg_view(grad_out, &vg, hg));
+  VB_TRY(contiguous_ptr(starts, &ps, hs)); VB_TRY(contiguous_ptr(lse, &pl, hl));
+  Outputs outs;
+  float *pdq, *pdk, *pdv;
+  VB_TRY(outs.add(dq, 3, q->dims, &pdq)); VB_TRY(outs.add(dk, 3, k->dims, &pdk)); VB_TRY(outs.add(dv, 3, v->dims, &pdv));
+  if (s.T > 0) VB_TRY(launch_segment_attention_backward(s, vq, vk, vv, ps, starts->dims[0] - 1, vo, pl, vg, pdq, pdk, pdv));
   outs.done();
   return VB_OK;
 }
