@@ -249,7 +249,9 @@ int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k_or_null, con
  * [starts[i], starts[i + 1]), and a row sees the rows of its segment up to itself.  Segments may be empty; rows before the first or
  * behind the last belong to none: their output and gradients are 0, their lse is -infinity.  Offsets that decrease or leave [0, T] set the
  * device error flag.  Scores are scale * q.k; p = exp(score - lse), without the 1e-9 of vb_fused_attention.  lse (may be NULL) is
- * [Hq, T], the natural log of a row's sum of exponentials; the backward call wants it and out.  dk <= 128, T <= 2^24. */
+ * [Hq, T], the natural log of a row's sum of exponentials; the backward call wants it and out.  dk <= 128, Hq <= 1024, T <= 2^24.
+ * Components that are not finite: a row that sees one in q, k or v has NaN output and lse, and gradients that it enters are NaN; rows that do
+ * not see it are unaffected. */
 int vb_segment_attention(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, vb_tensor* out, vb_tensor* lse_or_null);
 int vb_segment_attention_backward(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, const vb_tensor* out,
                                   const vb_tensor* lse, const vb_tensor* grad_out, vb_tensor* dq, vb_tensor* dk, vb_tensor* dv);

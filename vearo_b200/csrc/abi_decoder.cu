@@ -80,7 +80,7 @@ int segment_checks(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, c
   VB_CHECK(std::isfinite(scale) && scale > 0.0f, "scale must be positive");
   if (q->dims[2] > kSegMaxHead) return set_error(VB_ERR_UNSUPPORTED, "vb_segment_attention: head sizes up to 128");
   if (q->dims[0] > (i64)1 << 24 || starts->dims[0] > (i64)1 << 24) return set_error(VB_ERR_UNSUPPORTED, "vb_segment_attention: offsets beyond 2^24 are not whole numbers of f32");
-  if (q->dims[1] > 65535) return set_error(VB_ERR_UNSUPPORTED, "vb_segment_attention: at most 65535 heads");
+  if (q->dims[1] > 1024) return set_error(VB_ERR_UNSUPPORTED, "vb_segment_attention: at most 1024 query heads");
   *s = SegShape{q->dims[0], (int)q->dims[1], (int)k->dims[1], (int)q->dims[2], scale};
   return VB_OK;
 }
