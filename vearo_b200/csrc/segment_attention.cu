@@ -12,14 +12,14 @@
 // would carry them into rows that do not see them; a row that does see one gets a NaN sum of exponentials (forward), and
 // through its lse NaN gradients.
 //
-// The matrices of scores never leave the SM.  In every kernel eight warps hold one row each thread x half the tile's columns; the
+// The matrices of scores never leave the SM.  In every kernel a thread of the sixteen row warps holds a quarter of a row of the tile; the
 // second product takes its left operand (P, dS; hi and lo) from tensor memory, where these warps write it, and its right
 // operand from the same shared-memory tile that the first product read (MN-major instead of K-major).  The second product of each tile goes to a
 // fresh accumulator that the warps add to their registers with the running rescale, so the accumulator's truncation (split16.cuh) never
 // runs longer than a tile.
 //   k_forward   S = Q K^T, softmax with a running maximum, O += P V
-//   k_grad_v    S^T = K Q^T, P^T from the saved lse, dV += P^T dO         (all query heads of the group: no atomics)
-//   k_grad_qk   dQ: S = Q K^T, dP = dO V^T, dQ += dS K;  dK: the same with the roles of rows and columns exchanged
+//   k_backward  dV: S^T = K Q^T, P^T from the saved lse, dV += P^T dO, over the query heads of the group (no atomics)
+//               dQ: S = Q K^T, dP = dO V^T, dQ += dS K;  dK: the same with the roles of rows and columns exchanged
 // Every wait is bounded; when one runs out the CTA raises the device error word, frees its tensor memory and returns.
 #include "segment_attention.h"
 #include "split16.cuh"
@@ -28,20 +28,20 @@ namespace vb {
 namespace {
 using namespace tc;
 
-constexpr int kThreads = 320;             // warp 0: TMA, warp 1: MMA, warps 2-9: rows
+constexpr int kGroups = 4, kRowWarps = 4 * kGroups, kThreads = 32 * (2 + kRowWarps);      // warp 0: TMA, warp 1: MMA, the others: rows
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // ---- planes ------------------------------------------------------------------------------------------------------------------------
-// One of q, k, v, do: planes [2][heads][T][DP], and per head and tile the inverse scale, the largest row length and a bit for every row
-// with a component that is not finite.
+// One of q, k, v, do: planes [2][heads][T][DP], and per head and tile the inverse scale (negative where a component is not finite), the
+// largest row length and a bit for every row with a component that is not finite.
 struct PlanesDev { const float* x; i64 st, sh; __half* planes; float* inv; float* len; uint32_t* bad; int heads; bool vec; };
 struct PrepareDev {
   PlanesDev in[4];
   int n, T, tiles, dk, hq;
   const float* starts; int n_seg; int* begin; int* end; int* err;      // where the segment of each row begins and ends (begin null: not wanted)
-  const float* o; i64 o_st, o_sh; const float* lse;                     // for do: delta and the lse in base 2, padded to whole tiles
+  const float* o; i64 o_st, o_sh; bool o_vec; const float* lse;                     // for do: delta and the lse in base 2, padded to whole tiles
   float* delta; float* lse2;
 };
 
@@ -83,46 +83,64 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
   __syncthreads();
   const int c = (threadIdx.x % kLanes) * 4, r0 = threadIdx.x / kLanes;
   float4 v[kPasses];
-  float m = 0.0f;
+  const bool mine = c < p.dk;
+  const i64 t0 = (i64)tile * 128 + r0;
+  const float* src = x.x + t0 * x.st + h * x.sh + c;
 #pragma unroll
-  for (int i = 0; i < kPasses; ++i) {
-    const int r = i * kRows + r0;
-    const i64 t = (i64)tile * 128 + r;
+  for (int i = 0; i < kPasses; ++i) {      // all loads before the first use
     v[i] = make_float4(0, 0, 0, 0);
-    if (t < p.T && c < p.dk) {
-      const float* s = x.x + t * x.st + h * x.sh + c;
-      if (x.vec) v[i] = *reinterpret_cast<const float4*>(s);
+    if (mine && t0 + i * kRows < p.T) {
+      const float* s = src + i * kRows * x.st;
+      if (x.vec) v[i] = __ldcs(reinterpret_cast<const float4*>(s));
       else { v[i].x = s[0]; if (c + 1 < p.dk) v[i].y = s[1]; if (c + 2 < p.dk) v[i].z = s[2]; if (c + 3 < p.dk) v[i].w = s[3]; }
     }
-    if (p.delta && which == 3) {      // delta of the row, and its lse in base 2 (a row of no segment: +infinity, so that every p is 0)
+  }
+  if (p.delta && which == 3) {      // delta of the rows, and their lse in base 2 (a row of no segment: +infinity, so that every p is 0)
+    const float* o = p.o + t0 * p.o_st + h * p.o_sh + c;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const i64 t = t0 + i * kRows;
       float d = 0.0f;
-      if (t < p.T && c < p.dk) {
-        const float* o = p.o + t * p.o_st + h * p.o_sh + c;
-        d = v[i].x * o[0];
-        if (c + 1 < p.dk) d = fmaf(v[i].y, o[1], d);
-        if (c + 2 < p.dk) d = fmaf(v[i].z, o[2], d);
-        if (c + 3 < p.dk) d = fmaf(v[i].w, o[3], d);
+      if (mine && t < p.T) {
+        const float* oo = o + i * kRows * p.o_st;
+        if (p.o_vec) { const float4 y = *reinterpret_cast<const float4*>(oo); d = v[i].x * y.x; d = fmaf(v[i].y, y.y, d); d = fmaf(v[i].z, y.z, d); d = fmaf(v[i].w, y.w, d); }
+        else {
+          d = v[i].x * oo[0];
+          if (c + 1 < p.dk) d = fmaf(v[i].y, oo[1], d);
+          if (c + 2 < p.dk) d = fmaf(v[i].z, oo[2], d);
+          if (c + 3 < p.dk) d = fmaf(v[i].w, oo[3], d);
+        }
       }
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+      for (int k = kLanes / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
       if (c == 0) {
+        const i64 at = ((i64)h * p.tiles + tile) * 128 + i * kRows + r0;
         float l = t < p.T ? p.lse[(i64)h * p.T + t] : -INFINITY;
         const bool dead = l == -INFINITY;
         if (d != d) l = d;             // (a gradient that is not finite: dv sees it through p)
-        p.lse2[((i64)h * p.tiles + tile) * 128 + r] = dead ? INFINITY : l * kL2e;
-        p.delta[((i64)h * p.tiles + tile) * 128 + r] = dead ? 0.0f : d;
+        p.lse2[at] = dead ? INFINITY : l * kL2e;
+        p.delta[at] = dead ? 0.0f : d;
       }
     }
-    const float a = finite_abs(v[i].x), b = finite_abs(v[i].y), cc = finite_abs(v[i].z), d = finite_abs(v[i].w);
-    const bool fine = a == fabsf(v[i].x) && b == fabsf(v[i].y) && cc == fabsf(v[i].z) && d == fabsf(v[i].w);
-    if (!fine) {
-      if (a != fabsf(v[i].x)) v[i].x = 0.0f;
-      if (b != fabsf(v[i].y)) v[i].y = 0.0f;
-      if (cc != fabsf(v[i].z)) v[i].z = 0.0f;
-      if (d != fabsf(v[i].w)) v[i].w = 0.0f;
-      atomicOr(&bad[r >> 5], 1u << (r & 31));
+  }
+  float m = 0.0f;
+  bool fine = true;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const float a = fmaxf(fabsf(v[i].x), fabsf(v[i].y)), b = fmaxf(fabsf(v[i].z), fabsf(v[i].w));
+    const float sum = (v[i].x + v[i].y) * 0.0f + (v[i].z + v[i].w) * 0.0f;      // 0, or NaN where a component is not finite (or a sum overflows: looked at below)
+    fine = fine && sum == 0.0f;
+    m = fmaxf(m, fmaxf(a, b));
+  }
+  if (!fine) {
+    m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const float4 y = v[i];
+      v[i] = make_float4(is_finite(y.x) ? y.x : 0.0f, is_finite(y.y) ? y.y : 0.0f, is_finite(y.z) ? y.z : 0.0f, is_finite(y.w) ? y.w : 0.0f);
+      if (!(is_finite(y.x) && is_finite(y.y) && is_finite(y.z) && is_finite(y.w))) { const int r = i * kRows + r0; atomicOr(&bad[r >> 5], 1u << (r & 31)); }
+      m = fmaxf(m, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
     }
-    m = fmaxf(m, fmaxf(fmaxf(a, b), fmaxf(cc, d)));
   }
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
 #pragma unroll
@@ -138,7 +156,7 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
   const i64 plane = (i64)x.heads * p.T * DP;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
-    const i64 t = (i64)tile * 128 + i * kRows + r0;
+    const i64 t = t0 + i * kRows;
     const float4 y = make_float4(v[i].x * s, v[i].y * s, v[i].z * s, v[i].w * s);
     float ss = y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
 #pragma unroll
@@ -162,15 +180,15 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, red[i]);
-    x.inv[at] = inv;
+    x.inv[at] = bad[0] | bad[1] | bad[2] | bad[3] ? -inv : inv;      // (the sign: look at the tile's row bits)
     x.len[at] = sqrtf(top) * inv;
   }
   if (threadIdx.x < 4) x.bad[at * 4 + threadIdx.x] = bad[threadIdx.x];
 }
 
-// ---- what the three kernels share -------------------------------------------------------------------------------------------------
+// ---- what the kernels share ---------------------------------------------------------------------------------------------------------
 // A tile of ROWS rows in shared memory: hi plane, lo plane, each of DP / 64 chunks of ROWS x 128 bytes.
-template <int ROWS, int DP> __device__ constexpr int plane_bytes() { return ROWS * DP * 2; }
+template <int ROWS, int DP> __host__ __device__ constexpr int plane_bytes() { return ROWS * DP * 2; }
 template <int ROWS, int DP>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int head) {
   mbar_arrive_expect_tx(bar, 2 * plane_bytes<ROWS, DP>());
@@ -198,63 +216,78 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b)
     mma_f16(d, ah + oa, bh + ob, idesc, 1);
   }
 }
-// D[128, DP] = A[128, K] B[K, DP], A in tensor memory (per half of the columns: K / 4 columns of hi, then of lo), B a tile of K rows
+// D[128, DP] = A[128, K] B[K, DP], A in tensor memory (per quarter of the columns: K / 8 columns of hi, then of lo), B a tile of K rows
 template <int K, int DP>
 __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b) {
+  constexpr int kSteps = K / 16 / kGroups;       // of a quarter
   const uint32_t idesc = idesc16(128, DP, 0, 1);
   const uint64_t bh = desc16(b, K * 128), bl = desc16(b + plane_bytes<K, DP>(), K * 128);
   uint32_t on = 0;
 #pragma unroll
   for (int k = 0; k < K / 16; ++k) {
-    const uint32_t hi = a + (k / (K / 32)) * (K / 2) + (k % (K / 32)) * 8, lo = hi + K / 4;
+    const uint32_t hi = a + (k / kSteps) * (K / kGroups) + (k % kSteps) * 8, lo = hi + kSteps * 8;
     mma_f16_ta(d, lo, bh + k * 128, idesc, on);
     on = 1;
     mma_f16_ta(d, hi, bl + k * 128, idesc, 1);
   }
 #pragma unroll
   for (int k = 0; k < K / 16; ++k) {
-    const uint32_t hi = a + (k / (K / 32)) * (K / 2) + (k % (K / 32)) * 8;
+    const uint32_t hi = a + (k / kSteps) * (K / kGroups) + (k % kSteps) * 8;
     mma_f16_ta(d, hi, bh + k * 128, idesc, 1);
   }
 }
-// 16 columns of this thread's lane, from registers
+// 16 columns of this thread's lane, from and to registers
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
-// the half W of a row's columns as the left operand of product_cols: W / 2 columns of hi, W / 2 of lo
-template <int W>
-__device__ __forceinline__ void store_operand(uint32_t taddr, const float (&v)[W]) {
-#pragma unroll
-  for (int i = 0; i < W; i += 32) {
-    uint32_t hi[16], lo[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) split2_finite(v[i + 2 * j], v[i + 2 * j + 1], &hi[j], &lo[j]);
-    tmem_st16(taddr + i / 2, hi);
-    tmem_st16(taddr + W / 2 + i / 2, lo);
-  }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 template <int W>
-__device__ __forceinline__ void load_row(uint32_t taddr, float (&v)[W]) {
-#pragma unroll
-  for (int i = 0; i < W; i += 32) tmem_ld32(taddr + i, reinterpret_cast<uint32_t*>(v) + i);
+__device__ __forceinline__ void load_cols(uint32_t taddr, float (&v)[W]) {
+  static_assert(W == 16 || W == 32, "one load");
+  if constexpr (W == 32) tmem_ld32(taddr, reinterpret_cast<uint32_t*>(v)); else tmem_ld16(taddr, reinterpret_cast<uint32_t*>(v));
   tmem_wait_ld();
 }
-// acc = acc * keep + part * f over this thread's half of an accumulator
+// the quarter of a row's columns as the left operand of product_cols: W / 2 columns of hi, W / 2 of lo
+template <int W>
+__device__ __forceinline__ void store_operand(uint32_t taddr, const float (&v)[W]) {
+  uint32_t r[W];
+#pragma unroll
+  for (int j = 0; j < W / 2; ++j) split2_finite(v[2 * j], v[2 * j + 1], &r[j], &r[W / 2 + j]);
+  if constexpr (W == 32) tmem_st32(taddr, r); else tmem_st16(taddr, r);
+}
+// acc = acc * keep + part * f over this thread's quarter of an accumulator
 template <int W>
 __device__ __forceinline__ void add_part(uint32_t taddr, float (&acc)[W], float keep, float f) {
+  float v[W];
+  load_cols<W>(taddr, v);
+  const float2 k2 = make_float2(keep, keep), f2 = make_float2(f, f);
 #pragma unroll
-  for (int i = 0; i < W; i += 32) {
-    uint32_t v[32];
-    tmem_ld32(taddr + i, v);
-    tmem_wait_ld();
-#pragma unroll
-    for (int j = 0; j < 32; ++j) acc[i + j] = fmaf(__uint_as_float(v[j]), f, acc[i + j] * keep);
+  for (int j = 0; j < W; j += 2) {
+    const float2 a = fma2(make_float2(v[j], v[j + 1]), f2, mul2(make_float2(acc[j], acc[j + 1]), k2));
+    acc[j] = a.x; acc[j + 1] = a.y;
   }
 }
-// this thread's half of a row of the result, components [c0, c0 + W) of dk
+template <int W>
+__device__ __forceinline__ void add_part(uint32_t taddr, float (&acc)[W], float f) {
+  float v[W];
+  load_cols<W>(taddr, v);
+  const float2 f2 = make_float2(f, f);
+#pragma unroll
+  for (int j = 0; j < W; j += 2) {
+    const float2 a = fma2(make_float2(v[j], v[j + 1]), f2, make_float2(acc[j], acc[j + 1]));
+    acc[j] = a.x; acc[j + 1] = a.y;
+  }
+}
+// this thread's quarter of a row of the result, components [c0, c0 + W) of dk
 template <int W>
 __device__ __forceinline__ void store_row(float* row, const float (&acc)[W], int c0, int dk, float f) {
   if ((dk & 3) == 0) {
@@ -265,6 +298,31 @@ __device__ __forceinline__ void store_row(float* row, const float (&acc)[W], int
 #pragma unroll
     for (int i = 0; i < W; ++i) if (c0 + i < dk) row[c0 + i] = acc[i] * f;
   }
+}
+// p 2^14 of a quarter of a row: 2^(score - lse + 14), one lse a row or one a column
+template <int W>
+__device__ __forceinline__ void weights_of_row(float (&v)[W], float sc, float off) {
+  const float2 s2 = make_float2(sc, sc), o2 = make_float2(off, off);
+#pragma unroll
+  for (int i = 0; i < W; i += 2) {
+    const float2 x = fma2(make_float2(v[i], v[i + 1]), s2, o2);
+    v[i] = exp2_fast(x.x); v[i + 1] = exp2_fast(x.y);
+  }
+}
+template <int W>
+__device__ __forceinline__ void weights_of_cols(float (&v)[W], float sc, const float* lse2) {
+  const float2 s2 = make_float2(sc, sc), c14 = make_float2(14.0f, 14.0f), neg = make_float2(-1.0f, -1.0f);
+#pragma unroll
+  for (int i = 0; i < W; i += 4) {
+    const float4 l = *reinterpret_cast<const float4*>(lse2 + i);
+    const float2 a = fma2(make_float2(v[i], v[i + 1]), s2, fma2(lo2(l), neg, c14)), b = fma2(make_float2(v[i + 2], v[i + 3]), s2, fma2(hi2(l), neg, c14));
+    v[i] = exp2_fast(a.x); v[i + 1] = exp2_fast(a.y); v[i + 2] = exp2_fast(b.x); v[i + 3] = exp2_fast(b.y);
+  }
+}
+template <int W>
+__device__ __forceinline__ void keep_columns(float (&v)[W], int first, int last, float other) {
+#pragma unroll
+  for (int i = 0; i < W; ++i) if (i < first || i > last) v[i] = other;
 }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512u) : "memory");
@@ -292,6 +350,22 @@ __device__ __forceinline__ void range_of(int v, int* lo, int* hi, int* sm) {
   __syncthreads();
   *lo = sm[0]; *hi = sm[1];
 }
+// a row warp has written its operand (and read the last accumulator)
+__device__ __forceinline__ void operand_written(uint64_t* bar, int lane) {
+  tmem_wait_st();
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+// where a row warp's thread stands in a tile
+struct Seat {
+  int lane, quarter, group, row;
+  uint32_t lane_off;
+  __device__ __forceinline__ Seat() {
+    const int warp = threadIdx.x >> 5;
+    lane = threadIdx.x & 31; quarter = warp & 3; group = (warp - 2) >> 2; row = quarter * 32 + lane; lane_off = (uint32_t)(quarter * 32) << 16;
+  }
+};
 
 struct Side { const float* inv; const float* len; const uint32_t* bad; };
 struct AttnParams {
@@ -300,7 +374,9 @@ struct AttnParams {
   const int* begin; const int* end;
   Side q, k, v, g;
   const float* lse2; const float* delta;      // [hq][tiles * 128]
-  float* out; float* lse;                     // forward: o, lse; backward: the gradient
+  float* out; float* lse;                     // forward
+  float *dq, *dk_, *dv;                       // backward; with parts > 1 dk_ and dv are [parts][T, hk, dk], summed afterwards
+  int parts;                                  // a key head's group of query heads is dealt to this many CTAs
   int* err;
 };
 
@@ -308,29 +384,29 @@ struct AttnParams {
 template <int DP> struct FwdSmem {
   static constexpr int kTile = 2 * plane_bytes<128, DP>(), kStages = DP == 64 ? 2 : 1;
   static constexpr int kBars = 1 + 4 * kStages + 2 + 1 + 1;
-  static constexpr int kTotal = 1024 + kTile * (1 + 2 * kStages) + 512 * 4 + kBars * 8 + 64;
+  static constexpr int kTotal = 1024 + kTile * (1 + 2 * kStages) + 2 * kGroups * 128 * 4 + kBars * 8 + 64;
 };
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p) {
   using L = FwdSmem<DP>;
-  constexpr int NS = L::kStages, W = DP / 2;
+  constexpr int NS = L::kStages, W = DP / kGroups, H = 128 / kGroups;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sq = smem, *sk = smem + L::kTile, *sv = sk + NS * L::kTile;
-  float* xchg = (float*)(sv + NS * L::kTile);                 // [2 tiles][2 halves][128]
-  uint64_t* bars = (uint64_t*)(xchg + 512);
+  float* xchg = (float*)(sv + NS * L::kTile);                 // [2 tiles][groups][128]
+  uint64_t* bars = (uint64_t*)(xchg + 2 * kGroups * 128);
   uint64_t *b_q = bars, *b_kfull = bars + 1, *b_vfull = b_kfull + NS, *b_kfree = b_vfull + NS, *b_vfree = b_kfree + NS, *b_s = b_vfree + NS, *b_p = b_s + 2, *b_o = b_p + 1;
   int* ints = (int*)(b_o + 1);
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int h = blockIdx.x % p.hq, hk = h / (p.hq / p.hk), qt = p.tiles - 1 - (int)(blockIdx.x / p.hq);      // long tiles first
   if (threadIdx.x == 0) {
     mbar_init(b_q, 1);
     for (int i = 0; i < NS; ++i) { mbar_init(&b_kfull[i], 1); mbar_init(&b_vfull[i], 1); mbar_init(&b_kfree[i], 1); mbar_init(&b_vfree[i], 1); }
-    mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, 8); mbar_init(b_o, 1);
+    mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -346,7 +422,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
   const int kb0 = b_min < p.T ? b_min / 128 : qt + 1, n = qt + 1 - kb0;      // key tiles (none: no row of the tile has a segment)
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
+    if ((threadIdx.x & 31) == 0 && n > 0) {
       bool ok = true;
       load_tile<128, DP>(sq, &map_q, b_q, qt * 128, h);
       for (int j = 0; j < n && ok; ++j) {
@@ -361,7 +437,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       if (*abort_flag) let_land(bars, 1 + 2 * NS);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if ((threadIdx.x & 31) == 0 && n > 0) {
       bool ok = mbar_wait(b_q, 0, abort_flag);
       auto scores = [&](int j) -> bool {
         const int st = j % NS;
@@ -386,78 +462,69 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane, t = qt * 128 + row;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const Seat at;
+    const int t = qt * 128 + at.row;
     const int begin = t < p.T ? p.begin[t] : p.T;
     const i64 kvt = (i64)hk * p.tiles;
-    const float sc0 = p.scale * kL2e * p.q.inv[(i64)h * p.tiles + qt];
-    float acc[W], m = -INFINITY, l = 0.0f, keep = 0.0f;
+    const float q_inv = p.q.inv[(i64)h * p.tiles + qt], sc0 = p.scale * kL2e * fabsf(q_inv);
+    float acc[W], m = -INFINITY, l = 0.0f, keep = 0.0f, v_last = 0.0f;
+    float k_inv = n > 0 ? p.k.inv[kvt + kb0] : 0.0f, v_inv = n > 0 ? p.v.inv[kvt + kb0] : 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
-    bool ok = true;                             // (a wait that ran out does not end the loop: the other half of the rows meets this one in it)
+    bool ok = true;                             // (a wait that ran out does not end the loop: the other quarters of the rows meet this one in it)
     for (int j = 0; j < n; ++j) {
-      const int kb = kb0 + j, c0 = kb * 128 + half * 64;
-      const float sc = fmaxf(sc0 * p.k.inv[kvt + kb], 1e-37f);      // (masked scores are -infinity times this)
+      const int kb = kb0 + j, c0 = kb * 128 + at.group * H;
+      const float sc = fmaxf(sc0 * fabsf(k_inv), 1e-37f);      // (masked scores are -infinity times this)
+      const bool bad = k_inv < 0.0f || v_inv < 0.0f;
+      const float v_this = fabsf(v_inv);
+      if (j + 1 < n) { k_inv = p.k.inv[kvt + kb + 1]; v_inv = p.v.inv[kvt + kb + 1]; }
       ok = mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag) && ok;
       tc_fence_after();
-      float v[64];
-      load_row<64>(t_s + (j & 1) * 128 + half * 64 + lane_off, v);
-      if (kb == qt || kb * 128 < b_max) {       // the diagonal or the begin of a segment crosses the tile
-        const int a = begin - c0, z = t - c0;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) if (i < a || i > z) v[i] = -INFINITY;
+      float v[H];
+      load_cols<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
+      if (kb == qt || kb * 128 < b_max) keep_columns<H>(v, begin - c0, t - c0, -INFINITY);      // the diagonal or the begin of a segment crosses the tile
+      if (bad) {                                // a visible key or value that is not finite
+        const uint32_t bits = p.k.bad[(kvt + kb) * 4 + at.group] | p.v.bad[(kvt + kb) * 4 + at.group];
+        for (int i = 0; i < H; ++i) if (((bits >> i) & 1) && c0 + i >= begin && c0 + i <= t) l = __int_as_float(0x7fffffff);
       }
-      const uint32_t* kb_bad = p.k.bad + (kvt + kb) * 4 + half * 2;
-      const uint32_t* vb_bad = p.v.bad + (kvt + kb) * 4 + half * 2;
-      const uint32_t bad0 = kb_bad[0] | vb_bad[0], bad1 = kb_bad[1] | vb_bad[1];
-      if (bad0 | bad1) {                        // a visible key or value that is not finite
-        for (int i = 0; i < 64; ++i)
-          if (((i < 32 ? bad0 >> i : bad1 >> (i - 32)) & 1) && c0 + i >= begin && c0 + i <= t) l = __int_as_float(0x7fffffff);
-      }
-      float bm = v[0];
+      float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
 #pragma unroll
-      for (int i = 1; i < 64; ++i) bm = fmaxf(bm, v[i]);
-      float* x = xchg + (j & 1) * 256;
-      x[half * 128 + row] = bm;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");      // the two halves of these rows
-      bm = fmaxf(bm, x[(1 - half) * 128 + row]) * sc;
-      const float mn = fmaxf(m, bm), ref = mn > -INFINITY ? mn : 0.0f;
+      for (int i = 4; i < H; i += 4) { m0 = fmaxf(m0, fmaxf(v[i], v[i + 1])); m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3])); }
+      float* x = xchg + (j & 1) * kGroups * 128 + at.row;
+      x[at.group * 128] = fmaxf(m0, m1);
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");      // the four quarters of these rows
+      const float mn = fmaxf(m, fmaxf(fmaxf(x[0], x[128]), fmaxf(x[256], x[384])) * sc), ref = mn > -INFINITY ? mn : 0.0f;
       const float shrink = m > -INFINITY ? exp2_fast(m - ref) : 0.0f;
-      const float off = 14.0f - ref;
-      float sum = 0.0f;
+      weights_of_row<H>(v, sc, 14.0f - ref);
+      float2 s0 = make_float2(v[0], v[1]), s1 = make_float2(v[2], v[3]);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) { v[i] = exp2_fast(fmaf(v[i], sc, off)); sum += v[i]; }
-      l = l * shrink + sum;
+      for (int i = 4; i < H; i += 4) { s0 = add2(s0, make_float2(v[i], v[i + 1])); s1 = add2(s1, make_float2(v[i + 2], v[i + 3])); }
+      s0 = add2(s0, s1);
+      l = l * shrink + (s0.x + s0.y);
       m = mn;
       if (j > 0) {                              // the last tile's product has read P and is in its accumulator
         ok = mbar_wait(b_o, (j - 1) & 1, abort_flag) && ok;
         tc_fence_after();
-        add_part<W>(t_o + half * W + lane_off, acc, keep, p.v.inv[kvt + kb - 1]);
       }
-      store_operand<64>(t_p + half * 64 + lane_off, v);
-      keep = shrink;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b_p);
+      store_operand<H>(t_p + at.group * H + at.lane_off, v);
+      if (j > 0) add_part<W>(t_o + at.group * W + at.lane_off, acc, keep, v_last);
+      operand_written(b_p, at.lane);
+      keep = shrink; v_last = v_this;
     }
     if (n > 0) {
       ok = mbar_wait(b_o, (n - 1) & 1, abort_flag) && ok;
       tc_fence_after();
-      add_part<W>(t_o + half * W + lane_off, acc, keep, p.v.inv[kvt + qt]);
+      add_part<W>(t_o + at.group * W + at.lane_off, acc, keep, v_last);
     }
-    {
-      float* x = xchg + (n & 1) * 256;
-      x[half * 128 + row] = l;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-      l += x[(1 - half) * 128 + row];
-      if (ok && t < p.T) {
-        const uint32_t qbad = p.q.bad[((i64)h * p.tiles + qt) * 4 + quarter];
-        if (begin <= t && ((qbad >> lane) & 1)) l = __int_as_float(0x7fffffff);
-        const bool dead = l == 0.0f;
-        store_row<W>(p.out + ((i64)t * p.hq + h) * p.dk, acc, half * W, p.dk, dead ? 0.0f : 1.0f / l);
-        if (half == 0 && p.lse) p.lse[(i64)h * p.T + t] = dead ? -INFINITY : (m - 14.0f) * kLn2 + logf(l);
-      }
+    float* x = xchg + (n & 1) * kGroups * 128 + at.row;
+    x[at.group * 128] = l;
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
+    l = (x[0] + x[128]) + (x[256] + x[384]);
+    if (ok && t < p.T) {
+      if (q_inv < 0.0f && begin <= t && ((p.q.bad[((i64)h * p.tiles + qt) * 4 + at.quarter] >> at.lane) & 1)) l = __int_as_float(0x7fffffff);
+      const bool dead = l == 0.0f;
+      store_row<W>(p.out + ((i64)t * p.hq + h) * p.dk, acc, at.group * W, p.dk, dead ? 0.0f : 1.0f / l);
+      if (at.group == 0 && p.lse) p.lse[(i64)h * p.T + t] = dead ? -INFINITY : (m - 14.0f) * kLn2 + logf(l);
     }
   }
   tc_fence_before();
@@ -466,21 +533,22 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, ERRBIT_WAIT_TIMEOUT);
 }
 
-// ---- dV ---------------------------------------------------------------------------------------------------------------------------
-// One CTA per 128 keys of a key head.  Steps: every query head of the group x every tile of 128 queries from the keys' own to the last
-// one that sees them.
+// ---- backward ---------------------------------------------------------------------------------------------------------------------
+// One launch for the three gradients: CTAs that make dK come first (three products for every query head of the group), then dV (two),
+// then dQ, so that the long ones start first and the short ones fill the gaps.
+struct BwdMaps { CUtensorMap q, k, v, g, qn, kn, vn, gn; };      // boxes of 128 rows, and of N rows (GradSmem)
+
+// dV of 128 keys: every query head of the CTA's part of the group x every tile of 128 queries from the keys' own to the last one that
+// sees them.
 template <int DP> struct GradVSmem {
   static constexpr int kTile = 2 * plane_bytes<128, DP>(), kStages = DP == 64 ? 2 : 1;
   static constexpr int kBars = 1 + 4 * kStages + 2 + 1 + 1;
   static constexpr int kTotal = 1024 + kTile * (1 + 2 * kStages) + kBars * 8 + 64;
 };
 template <int DP>
-__global__ void __launch_bounds__(kThreads, 1)
-k_grad_v(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g, const __grid_constant__ AttnParams p) {
+__device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const AttnParams& p, int block) {
   using L = GradVSmem<DP>;
-  constexpr int NS = L::kStages, W = DP / 2;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  constexpr int NS = L::kStages, W = DP / kGroups, H = 128 / kGroups;
   uint8_t *sk = smem, *sq = smem + L::kTile, *sg = sq + NS * L::kTile;
   uint64_t* bars = (uint64_t*)(sg + NS * L::kTile);
   uint64_t *b_k = bars, *b_qfull = bars + 1, *b_gfull = b_qfull + NS, *b_qfree = b_gfull + NS, *b_gfree = b_qfree + NS, *b_s = b_gfree + NS, *b_p = b_s + 2, *b_o = b_p + 1;
@@ -488,12 +556,12 @@ k_grad_v(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUte
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.x % p.hk, kt = blockIdx.x / p.hk, group = p.hq / p.hk;
+  const int warp = threadIdx.x >> 5;
+  const int part = block % p.parts, hk = block / p.parts % p.hk, kt = block / p.parts / p.hk, heads = p.hq / p.hk / p.parts, h0 = (hk * p.parts + part) * heads;
   if (threadIdx.x == 0) {
     mbar_init(b_k, 1);
     for (int i = 0; i < NS; ++i) { mbar_init(&b_qfull[i], 1); mbar_init(&b_gfull[i], 1); mbar_init(&b_qfree[i], 1); mbar_init(&b_gfree[i], 1); }
-    mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, 8); mbar_init(b_o, 1);
+    mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -506,25 +574,25 @@ k_grad_v(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUte
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t t_s = tmem, t_p = tmem + 256, t_o = tmem + 384;
-  const int per = e_max > 0 ? (e_max - 1) / 128 - kt + 1 : 0, n = per * group;
+  const int per = e_max > 0 ? (e_max - 1) / 128 - kt + 1 : 0, n = per * heads;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
+    if ((threadIdx.x & 31) == 0 && n > 0) {
       bool ok = true;
-      load_tile<128, DP>(sk, &map_k, b_k, kt * 128, hk);
+      load_tile<128, DP>(sk, &maps.k, b_k, kt * 128, hk);
       for (int j = 0; j < n && ok; ++j) {
-        const int st = j % NS, ph = ((j / NS) - 1) & 1, h = hk * group + j / per, i = kt + j % per;
+        const int st = j % NS, ph = ((j / NS) - 1) & 1, h = h0 + j / per, i = kt + j % per;
         if (j >= NS) ok = mbar_wait(&b_qfree[st], ph, abort_flag);
         if (!ok) break;
-        load_tile<128, DP>(sq + st * L::kTile, &map_q, &b_qfull[st], i * 128, h);
+        load_tile<128, DP>(sq + st * L::kTile, &maps.q, &b_qfull[st], i * 128, h);
         if (j >= NS) ok = mbar_wait(&b_gfree[st], ph, abort_flag);
         if (!ok) break;
-        load_tile<128, DP>(sg + st * L::kTile, &map_g, &b_gfull[st], i * 128, h);
+        load_tile<128, DP>(sg + st * L::kTile, &maps.g, &b_gfull[st], i * 128, h);
       }
       if (*abort_flag) let_land(bars, 1 + 2 * NS);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if ((threadIdx.x & 31) == 0 && n > 0) {
       bool ok = mbar_wait(b_k, 0, abort_flag);
       auto scores = [&](int j) -> bool {
         const int st = j % NS;
@@ -549,54 +617,41 @@ k_grad_v(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUte
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane, t = kt * 128 + row;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const Seat at;
+    const int t = kt * 128 + at.row;
     const int end = t < p.T ? p.end[t] : 0;
-    const float sc0 = p.scale * kL2e * p.k.inv[(i64)hk * p.tiles + kt];
+    const float sc0 = p.scale * kL2e * fabsf(p.k.inv[(i64)hk * p.tiles + kt]);
     float acc[W], f_last = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      const i64 at = (i64)(hk * group + j / per) * p.tiles + kt + j % per;
-      const int i0 = (kt + j % per) * 128, c0 = i0 + half * 64;
-      const float sc = sc0 * p.q.inv[at];
-      const float4* lse = reinterpret_cast<const float4*>(p.lse2 + at * 128 + half * 64);
+      const int qt = kt + j % per, c0 = qt * 128 + at.group * H;
+      const i64 tile = (i64)(h0 + j / per) * p.tiles + qt;
+      const float sc = sc0 * fabsf(p.q.inv[tile]), f_this = fabsf(p.g.inv[tile]);
       if (!mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      float v[64];
-      load_row<64>(t_s + (j & 1) * 128 + half * 64 + lane_off, v);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float4 x = lse[i];
-        v[4 * i] = exp2_fast(fmaf(v[4 * i], sc, 14.0f - x.x)); v[4 * i + 1] = exp2_fast(fmaf(v[4 * i + 1], sc, 14.0f - x.y));
-        v[4 * i + 2] = exp2_fast(fmaf(v[4 * i + 2], sc, 14.0f - x.z)); v[4 * i + 3] = exp2_fast(fmaf(v[4 * i + 3], sc, 14.0f - x.w));
-      }
-      if (i0 == kt * 128 || i0 + 128 > e_min) {
-        const int a = t - c0, z = end - c0;
-#pragma unroll
-        for (int i = 0; i < 64; ++i) if (i < a || i >= z) v[i] = 0.0f;
-      }
+      float v[H];
+      load_cols<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
+      weights_of_cols<H>(v, sc, p.lse2 + tile * 128 + at.group * H);
+      if (qt == kt || qt * 128 + 128 > e_min) keep_columns<H>(v, t - c0, end - 1 - c0, 0.0f);
       if (j > 0) {
         if (!mbar_wait(b_o, (j - 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        add_part<W>(t_o + half * W + lane_off, acc, 1.0f, f_last);
       }
-      store_operand<64>(t_p + half * 64 + lane_off, v);
-      f_last = p.g.inv[at];
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b_p);
+      store_operand<H>(t_p + at.group * H + at.lane_off, v);
+      if (j > 0) add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
+      operand_written(b_p, at.lane);
+      f_last = f_this;
     }
     if (ok && n > 0) {
       ok = mbar_wait(b_o, (n - 1) & 1, abort_flag);
       if (ok) {
         tc_fence_after();
-        add_part<W>(t_o + half * W + lane_off, acc, 1.0f, f_last);
+        add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
       }
     }
-    if (ok && t < p.T) store_row<W>(p.out + ((i64)t * p.hk + hk) * p.dk, acc, half * W, p.dk, 1.0f / 16384.0f);
+    if (ok && t < p.T) store_row<W>(p.dv + (((i64)part * p.T + t) * p.hk + hk) * p.dk, acc, at.group * W, p.dk, 1.0f / 16384.0f);
   }
   tc_fence_before();
   __syncthreads();
@@ -604,8 +659,7 @@ k_grad_v(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUte
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, ERRBIT_WAIT_TIMEOUT);
 }
 
-// ---- dQ and dK --------------------------------------------------------------------------------------------------------------------
-// X (128 rows, resident: q and do, or k and v), Y streamed in tiles of N rows (k and v, or q and do):
+// dQ and dK.  X (128 rows, resident: q and do, or k and v), Y streamed in tiles of N rows (k and v, or q and do):
 //   S = X1 Y1^T, dP = X2 Y2^T, dS = p (dP - delta), result += dS Y1.
 // dS goes where S was; S has two buffers, so the next tile's S and dP are formed while dS Y1 runs.
 template <int DP> struct GradSmem {
@@ -616,13 +670,9 @@ template <int DP> struct GradSmem {
   static constexpr int kTotal = 1024 + 2 * kTileX + (2 + kStages2) * kTileY + kBars * 8 + 64;
 };
 template <int DP, bool DK>
-__global__ void __launch_bounds__(kThreads, 1)
-k_grad_qk(const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CUtensorMap map_x2, const __grid_constant__ CUtensorMap map_y1,
-          const __grid_constant__ CUtensorMap map_y2, const __grid_constant__ AttnParams p) {
+__device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, const AttnParams& p, int block) {
   using L = GradSmem<DP>;
-  constexpr int N = L::N, H = N / 2, W = DP / 2, NS2 = L::kStages2, R = 128 / N;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  constexpr int N = L::N, H = N / kGroups, W = DP / kGroups, NS2 = L::kStages2, R = 128 / N;
   uint8_t *x1 = smem, *x2 = x1 + L::kTileX, *y1 = x2 + L::kTileX, *y2 = y1 + 2 * L::kTileY;
   uint64_t* bars = (uint64_t*)(y2 + NS2 * L::kTileY);
   uint64_t *b_x = bars, *b_y1full = bars + 2, *b_y2full = b_y1full + 2, *b_y1free = b_y2full + NS2, *b_y2free = b_y1free + 2, *b_s = b_y2free + NS2, *b_dp = b_s + 2,
@@ -632,14 +682,15 @@ k_grad_qk(const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CU
   volatile int* abort_flag = ints + 3;
   float* vmax_slot = (float*)ints + 4;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = p.hq / p.hk, heads = DK ? p.hk : p.hq, hx = blockIdx.x % heads, hk = DK ? hx : hx / group;
-  const int xt = DK ? blockIdx.x / heads : p.tiles - 1 - (int)(blockIdx.x / heads);
+  const int warp = threadIdx.x >> 5;
+  const int part = DK ? block % p.parts : 0, rest = DK ? block / p.parts : block, x_heads = DK ? p.hk : p.hq;
+  const int hx = rest % x_heads, hk = DK ? hx : hx / (p.hq / p.hk), heads = DK ? p.hq / p.hk / p.parts : 1, h0 = DK ? (hk * p.parts + part) * heads : hx;
+  const int xt = DK ? rest / x_heads : p.tiles - 1 - rest / x_heads;
   if (threadIdx.x == 0) {
     mbar_init(&b_x[0], 1); mbar_init(&b_x[1], 1);
     for (int i = 0; i < 2; ++i) { mbar_init(&b_y1full[i], 1); mbar_init(&b_y1free[i], 1); mbar_init(&b_s[i], 1); }
     for (int i = 0; i < NS2; ++i) { mbar_init(&b_y2full[i], 1); mbar_init(&b_y2free[i], 1); }
-    mbar_init(b_dp, 1); mbar_init(b_ds, 8); mbar_init(b_o, 1);
+    mbar_init(b_dp, 1); mbar_init(b_ds, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     *vmax_slot = 0.0f;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -654,7 +705,7 @@ k_grad_qk(const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CU
     for (int i = threadIdx.x; i < p.tiles; i += kThreads) m = fmaxf(m, p.v.len[(i64)hk * p.tiles + i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) atomicMax((int*)vmax_slot, __float_as_int(m));      // (not negative: ordered like its bits)
+    if ((threadIdx.x & 31) == 0) atomicMax((int*)vmax_slot, __float_as_int(m));      // (not negative: ordered like its bits)
   }
   tc_fence_before();
   __syncthreads();
@@ -666,27 +717,28 @@ k_grad_qk(const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CU
   int y0, per;
   if (DK) { y0 = xt * R; per = e_max > 0 ? (e_max - 1) / N - y0 + 1 : 0; }
   else { const int last = xt * 128 + 127 < p.T ? xt * 128 + 127 : p.T - 1; y0 = e_min / N; per = e_min < p.T ? last / N - y0 + 1 : 0; }
-  const int n = DK ? per * group : per;
+  const int n = per * heads;
+  const CUtensorMap *map_x1 = DK ? &maps.k : &maps.q, *map_x2 = DK ? &maps.v : &maps.g, *map_y1 = DK ? &maps.qn : &maps.kn, *map_y2 = DK ? &maps.gn : &maps.vn;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
+    if ((threadIdx.x & 31) == 0 && n > 0) {
       bool ok = true;
-      load_tile<128, DP>(x1, &map_x1, &b_x[0], xt * 128, hx);
+      load_tile<128, DP>(x1, map_x1, &b_x[0], xt * 128, hx);
       for (int j = 0; j < n && ok; ++j) {
-        const int hy = DK ? hk * group + j / per : hk, y = (y0 + (DK ? j % per : j)) * N;
+        const int hy = DK ? h0 + j / per : hk, y = (y0 + (DK ? j % per : j)) * N;
         if (j >= 2) ok = mbar_wait(&b_y1free[j & 1], ((j >> 1) - 1) & 1, abort_flag);
         if (!ok) break;
-        load_tile<N, DP>(y1 + (j & 1) * L::kTileY, &map_y1, &b_y1full[j & 1], y, hy);
-        if (j == 0) load_tile<128, DP>(x2, &map_x2, &b_x[1], xt * 128, hx);
+        load_tile<N, DP>(y1 + (j & 1) * L::kTileY, map_y1, &b_y1full[j & 1], y, hy);
+        if (j == 0) load_tile<128, DP>(x2, map_x2, &b_x[1], xt * 128, hx);
         const int st = j % NS2;
         if (j >= NS2) ok = mbar_wait(&b_y2free[st], ((j / NS2) - 1) & 1, abort_flag);
         if (!ok) break;
-        load_tile<N, DP>(y2 + st * L::kTileY, &map_y2, &b_y2full[st], y, hy);
+        load_tile<N, DP>(y2 + st * L::kTileY, map_y2, &b_y2full[st], y, hy);
       }
       if (*abort_flag) let_land(bars, 4 + NS2);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if ((threadIdx.x & 31) == 0 && n > 0) {
       bool ok = mbar_wait(&b_x[0], 0, abort_flag);
       auto scores = [&](int j) -> bool {      // (buffer j & 1 held dS of tile j - 2, which its product has read)
         if (!mbar_wait(&b_y1full[j & 1], (j >> 1) & 1, abort_flag)) return false;
@@ -720,11 +772,11 @@ k_grad_qk(const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CU
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2, row = quarter * 32 + lane, t = xt * 128 + row;
-    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const Seat at;
+    const int t = xt * 128 + at.row;
     const int mine = DK ? (t < p.T ? p.end[t] : 0) : (t < p.T ? p.begin[t] : p.T);
-    const i64 x_at = (i64)hx * p.tiles + xt, v_row = (i64)hk * p.tiles;
-    const float s_x = p.scale * kL2e * (DK ? p.k.inv[x_at] : p.q.inv[x_at]);
+    const i64 x_at = (i64)hx * p.tiles + xt;
+    const float s_x = p.scale * kL2e * fabsf(DK ? p.k.inv[x_at] : p.q.inv[x_at]);
     // 2^e with 2 |do| |v| 2^e below 2^14, and its inverse
     auto ds_scale = [&](float len, float* inverse) -> float {
       const float b = 2.0f * len * vmax;
@@ -733,95 +785,96 @@ k_grad_qk(const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CU
       *inverse = __uint_as_float((uint32_t)(127 - e) << 23);
       return __uint_as_float((uint32_t)(127 + e) << 23);
     };
-    float back, f_last = 0.0f, lse_row = 0.0f, delta_row = 0.0f, f2 = 0.0f, fx = 0.0f;
+    float back, f_last = 0.0f, lse_row = 0.0f, delta_row = 0.0f, f2 = 0.0f, fx = DK ? fabsf(p.v.inv[x_at]) : 0.0f;
     if (!DK) {
       f2 = ds_scale(p.g.len[x_at], &back) * (1.0f / 16384.0f);      // (p carries 2^14)
-      fx = p.g.inv[x_at] * f2;
-      lse_row = 14.0f - p.lse2[x_at * 128 + row];
-      delta_row = p.delta[x_at * 128 + row] * f2;
+      fx = fabsf(p.g.inv[x_at]) * f2;
+      lse_row = 14.0f - p.lse2[x_at * 128 + at.row];
+      delta_row = -p.delta[x_at * 128 + at.row] * f2;
     }
     float acc[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      const int hy = DK ? hk * group + j / per : hk, y = (y0 + (DK ? j % per : j)) * N, c0 = y + half * H;
-      const i64 y_at = (i64)hy * p.tiles + y / 128;
-      const float sc = s_x * (DK ? p.q.inv[y_at] : p.k.inv[y_at]);
+      const int hy = DK ? h0 + j / per : hk, y = (y0 + (DK ? j % per : j)) * N, c0 = y + at.group * H;
+      const i64 y_at = (i64)hy * p.tiles + y / 128, col = (i64)hy * p.tiles * 128 + c0;
+      const float sc = s_x * fabsf(DK ? p.q.inv[y_at] : p.k.inv[y_at]);
       float f1, f_this;
-      const float4 *lse4 = nullptr, *delta4 = nullptr;
       if (DK) {
         f2 = ds_scale(p.g.len[y_at], &back) * (1.0f / 16384.0f);
-        f1 = p.g.inv[y_at] * f2 * p.v.inv[x_at];
-        f_this = p.q.inv[y_at] * back;
-        lse4 = reinterpret_cast<const float4*>(p.lse2 + (i64)hy * p.tiles * 128 + c0);
-        delta4 = reinterpret_cast<const float4*>(p.delta + (i64)hy * p.tiles * 128 + c0);
+        f1 = fabsf(p.g.inv[y_at]) * f2 * fx;
+        f_this = fabsf(p.q.inv[y_at]) * back;
       } else {
-        f1 = fx * p.v.inv[y_at];
-        f_this = p.k.inv[y_at] * back;
+        f1 = fx * fabsf(p.v.inv[y_at]);
+        f_this = fabsf(p.k.inv[y_at]) * back;
       }
       if (!mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
       float v[H];
-      load_row<H>(t_s + (j & 1) * 128 + half * H + lane_off, v);
-      if (DK) {
-#pragma unroll
-        for (int i = 0; i < H / 4; ++i) {
-          const float4 x = lse4[i];
-          v[4 * i] = exp2_fast(fmaf(v[4 * i], sc, 14.0f - x.x)); v[4 * i + 1] = exp2_fast(fmaf(v[4 * i + 1], sc, 14.0f - x.y));
-          v[4 * i + 2] = exp2_fast(fmaf(v[4 * i + 2], sc, 14.0f - x.z)); v[4 * i + 3] = exp2_fast(fmaf(v[4 * i + 3], sc, 14.0f - x.w));
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < H; ++i) v[i] = exp2_fast(fmaf(v[i], sc, lse_row));
-      }
+      load_cols<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
+      if (DK) weights_of_cols<H>(v, sc, p.lse2 + col);
+      else weights_of_row<H>(v, sc, lse_row);
       const bool crossed = DK ? y < xt * 128 + 128 || y + N > e_min : y + N > xt * 128 || y < e_max;
       if (!mbar_wait(b_dp, j & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
+      {
+        float d[H];
+        load_cols<H>(t_dp + at.group * H + at.lane_off, d);
+        const float2 f12 = make_float2(f1, f1), f22 = make_float2(-f2, -f2);
+        float2 de = make_float2(delta_row, delta_row);
 #pragma unroll
-      for (int c = 0; c < H; c += 32) {
-        uint32_t d[32];
-        tmem_ld32(t_dp + half * H + c + lane_off, d);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 de = make_float4(delta_row, delta_row, delta_row, delta_row);
-          if (DK) { de = delta4[(c + i) / 4]; de.x *= f2; de.y *= f2; de.z *= f2; de.w *= f2; }
-          v[c + i] *= fmaf(__uint_as_float(d[i]), f1, -de.x); v[c + i + 1] *= fmaf(__uint_as_float(d[i + 1]), f1, -de.y);
-          v[c + i + 2] *= fmaf(__uint_as_float(d[i + 2]), f1, -de.z); v[c + i + 3] *= fmaf(__uint_as_float(d[i + 3]), f1, -de.w);
+        for (int i = 0; i < H; i += 2) {
+          if (DK) de = mul2(*reinterpret_cast<const float2*>(p.delta + col + i), f22);
+          const float2 x = mul2(make_float2(v[i], v[i + 1]), fma2(make_float2(d[i], d[i + 1]), f12, de));
+          v[i] = x.x; v[i + 1] = x.y;
         }
       }
-      if (crossed) {
-        const int a = (DK ? t : mine) - c0, z = (DK ? mine - 1 : t) - c0;
-#pragma unroll
-        for (int i = 0; i < H; ++i) if (i < a || i > z) v[i] = 0.0f;
-      }
+      if (crossed) keep_columns<H>(v, (DK ? t : mine) - c0, (DK ? mine - 1 : t) - c0, 0.0f);
+      // (a quarter's dS lies within its own quarter of S)
+      store_operand<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
       if (j > 0) {
         if (!mbar_wait(b_o, (j - 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        add_part<W>(t_o + half * W + lane_off, acc, 1.0f, f_last);
+        add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
       }
-      // (both halves of these rows have read S before either writes dS over it: dS of a half lies within its own half of S)
-      store_operand<H>(t_s + (j & 1) * 128 + half * H + lane_off, v);
+      operand_written(b_ds, at.lane);
       f_last = f_this;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(b_ds);
     }
     if (ok && n > 0) {
       ok = mbar_wait(b_o, (n - 1) & 1, abort_flag);
       if (ok) {
         tc_fence_after();
-        add_part<W>(t_o + half * W + lane_off, acc, 1.0f, f_last);
+        add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
       }
     }
-    if (ok && t < p.T) store_row<W>(p.out + ((i64)t * (DK ? p.hk : p.hq) + hx) * p.dk, acc, half * W, p.dk, p.scale);
+    if (ok && t < p.T) {
+      float* row = DK ? p.dk_ + (((i64)part * p.T + t) * p.hk + hk) * p.dk : p.dq + ((i64)t * p.hq + hx) * p.dk;
+      store_row<W>(row, acc, at.group * W, p.dk, p.scale);
+    }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) { tc_fence_after(); tmem_free(tmem); }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, ERRBIT_WAIT_TIMEOUT);
+}
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) k_backward(const __grid_constant__ BwdMaps maps, const __grid_constant__ AttnParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int keys = p.tiles * p.hk * p.parts, b = blockIdx.x;
+  if (b < keys) grad_qk<DP, true>(smem, maps, p, b);
+  else if (b < 2 * keys) grad_v<DP>(smem, maps, p, b - keys);
+  else grad_qk<DP, false>(smem, maps, p, b - 2 * keys);
+}
+// the parts of dK and dV added in order
+__global__ void __launch_bounds__(256) k_add_parts(const float* __restrict__ a, const float* __restrict__ b, float* __restrict__ oa, float* __restrict__ ob, i64 n, int parts) {
+  for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (i64)gridDim.x * 256) {
+    const float* src = i < n ? a + i : b + (i - n);
+    float s = src[0];
+    for (int k = 1; k < parts; ++k) s += src[(i64)k * n];
+    if (i < n) oa[i] = s; else ob[i - n] = s;
+  }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
@@ -881,7 +934,8 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
     all += heads[i];
   }
   d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.err = ctx().d_err;
-  if (o) { d.o = o->p; d.o_st = o->st; d.o_sh = o->sh; d.lse = lse; d.delta = (float*)(base + delta); d.lse2 = (float*)(base + lse2); }
+  if (o) { d.o = o->p; d.o_st = o->st; d.o_sh = o->sh; d.lse = lse;
+           d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lse2 = (float*)(base + lse2); }
   AttnParams& p = w.p;
   p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.scale = s.scale;
   p.begin = d.begin; p.end = d.end; p.lse2 = d.lse2; p.delta = d.delta; p.err = ctx().d_err;
@@ -909,23 +963,33 @@ int forward(Work& w) {
 }
 template <int DP>
 int backward(Work& w, float* dq, float* dk, float* dv) {
-  static const int ready_v = allow_smem(k_grad_v<DP>, GradVSmem<DP>::kTotal), ready_q = allow_smem(k_grad_qk<DP, false>, GradSmem<DP>::kTotal),
-                   ready_k = allow_smem(k_grad_qk<DP, true>, GradSmem<DP>::kTotal);
-  VB_TRY(ready_v); VB_TRY(ready_q); VB_TRY(ready_k);
-  constexpr int N = GradSmem<DP>::N;
-  CUtensorMap q, k, v, g, qn, kn, vn, gn;
+  constexpr int N = GradSmem<DP>::N, kSmem = GradSmem<DP>::kTotal > GradVSmem<DP>::kTotal ? GradSmem<DP>::kTotal : GradVSmem<DP>::kTotal;
+  static const int ready = allow_smem(k_backward<DP>, kSmem);
+  VB_TRY(ready);
+  BwdMaps m;
   const PlanesDev* in = w.prep.in;
-  VB_TRY(make_map(&q, in[0], w.p.T, DP, 128)); VB_TRY(make_map(&k, in[1], w.p.T, DP, 128)); VB_TRY(make_map(&v, in[2], w.p.T, DP, 128)); VB_TRY(make_map(&g, in[3], w.p.T, DP, 128));
-  VB_TRY(make_map(&qn, in[0], w.p.T, DP, N)); VB_TRY(make_map(&kn, in[1], w.p.T, DP, N)); VB_TRY(make_map(&vn, in[2], w.p.T, DP, N)); VB_TRY(make_map(&gn, in[3], w.p.T, DP, N));
-  w.p.out = dv;
-  k_grad_v<DP><<<(unsigned)w.p.hk * w.p.tiles, kThreads, GradVSmem<DP>::kTotal, ctx().stream>>>(k, q, g, w.p);
+  AttnParams& p = w.p;
+  VB_TRY(make_map(&m.q, in[0], p.T, DP, 128)); VB_TRY(make_map(&m.k, in[1], p.T, DP, 128)); VB_TRY(make_map(&m.v, in[2], p.T, DP, 128)); VB_TRY(make_map(&m.g, in[3], p.T, DP, 128));
+  VB_TRY(make_map(&m.qn, in[0], p.T, DP, N)); VB_TRY(make_map(&m.kn, in[1], p.T, DP, N)); VB_TRY(make_map(&m.vn, in[2], p.T, DP, N)); VB_TRY(make_map(&m.gn, in[3], p.T, DP, N));
+  // A CTA that walks the query heads of a whole group is the longest of the launch: where dK and dV have fewer than four CTAs for
+  // every SM the group is dealt to several, whose sums are added afterwards.
+  const int group = p.hq / p.hk;
+  p.parts = 1;
+  for (int d = 2; d <= group && (i64)p.tiles * p.hk * p.parts < 4 * ctx().sm_count; ++d) if (group % d == 0) p.parts = d;
+  const i64 n = (i64)p.T * p.hk * p.dk;
+  Temp hold;
+  p.dq = dq; p.dk_ = dk; p.dv = dv;
+  if (p.parts > 1) {
+    VB_TRY(scratch_alloc((size_t)(2 * p.parts * n) * sizeof(float), &hold.p));
+    p.dk_ = (float*)hold.p; p.dv = p.dk_ + p.parts * n;
+  }
+  k_backward<DP><<<(unsigned)(p.tiles * (2 * p.hk * p.parts + p.hq)), kThreads, kSmem, ctx().stream>>>(m, p);
   VB_LAUNCH_CHECK();
-  w.p.out = dk;
-  k_grad_qk<DP, true><<<(unsigned)w.p.hk * w.p.tiles, kThreads, GradSmem<DP>::kTotal, ctx().stream>>>(k, v, qn, gn, w.p);
-  VB_LAUNCH_CHECK();
-  w.p.out = dq;
-  k_grad_qk<DP, false><<<(unsigned)w.p.hq * w.p.tiles, kThreads, GradSmem<DP>::kTotal, ctx().stream>>>(q, g, kn, vn, w.p);
-  VB_LAUNCH_CHECK();
+  if (p.parts > 1) {
+    const i64 ctas = (2 * n + 1023) / 1024, cap = (i64)ctx().sm_count * 8;
+    k_add_parts<<<(unsigned)(ctas < cap ? ctas : cap), 256, 0, ctx().stream>>>(p.dk_, p.dv, dk, dv, n, p.parts);
+    VB_LAUNCH_CHECK();
+  }
   return VB_OK;
 }
 

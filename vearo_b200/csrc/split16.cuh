@@ -28,6 +28,7 @@ __device__ __forceinline__ float block_scale(float amax, float* inverse) {
   *inverse = __uint_as_float((uint32_t)(127 - e) << 23);
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 __device__ __forceinline__ float finite_abs(float x) { const float a = fabsf(x); return a <= 3.402823466e38f ? a : 0.0f; }
 
 // hi and lo of a scaled pair, packed (a value that is not finite has lo = 0, so that hi alone carries it)
@@ -44,8 +45,8 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t*
 // the same for values known to be finite and below 2^15
 __device__ __forceinline__ void split2_finite(float a, float b, uint32_t* hi, uint32_t* lo) {
   const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  const float2 d = fma2(__half22float2(h), make_float2(-1.0f, -1.0f), make_float2(a, b));
+  const __half2 l = __floats2half2_rn(d.x, d.y);
   *hi = *reinterpret_cast<const uint32_t*>(&h);
   *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
