@@ -146,37 +146,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t it = 0, run = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
-        const uint32_t idesc = idesc16(kBM, kBN, q.a.mn, q.b.mn);
-        const uint64_t step_a = (q.a.mn ? 2048 : 32) >> 4, step_b = (q.b.mn ? 2048 : 32) >> 4;
-        for (int k0 = 0; k0 < q.K && ok; k0 += 2 * kBK, ++run) {
-          const int acc = run & 1;
-          if (run >= 2 && !mbar_wait(&bars[B_RUNFREE + acc], ((run >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
-          const uint32_t d = tmem + acc * kBN;
-          uint32_t on = 0;
-          for (int k = k0; k < q.K && k < k0 + 2 * kBK; k += kBK, ++it) {
-            const int st = it % kStages;
-            if (!mbar_wait(&bars[B_FULL + st], (it / kStages) & 1, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            const uint32_t base = smem_u32(smem + st * kStage);
-            const uint64_t ah = desc16(base, 8192), al = desc16(base + kAPlane, 8192);
-            const uint64_t bh = desc16(base + 2 * kAPlane, 8192), bl = desc16(base + 2 * kAPlane + kBPlane, 8192);
+    const uint32_t leader = elect_leader();
+    uint32_t it = 0, run = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
+      const uint32_t idesc = idesc16(kBM, kBN, q.a.mn, q.b.mn);
+      const uint64_t step_a = (q.a.mn ? 2048 : 32) >> 4, step_b = (q.b.mn ? 2048 : 32) >> 4;
+      for (int k0 = 0; k0 < q.K && ok; k0 += 2 * kBK, ++run) {
+        const int acc = run & 1;
+        if (run >= 2 && !warp_wait(&bars[B_RUNFREE + acc], ((run >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+        const uint32_t d = tmem + acc * kBN;
+        uint32_t on = 0;
+        for (int k = k0; k < q.K && k < k0 + 2 * kBK; k += kBK, ++it) {
+          const int st = it % kStages;
+          if (!warp_wait(&bars[B_FULL + st], (it / kStages) & 1, abort_flag)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t base = smem_u32(smem + st * kStage);
+          const uint64_t ah = desc16(base, 8192), al = desc16(base + kAPlane, 8192);
+          const uint64_t bh = desc16(base + 2 * kAPlane, 8192), bl = desc16(base + 2 * kAPlane + kBPlane, 8192);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              mma_f16(d, al + s * step_a, bh + s * step_b, idesc, on);
-              on = 1;
-              mma_f16(d, ah + s * step_a, bl + s * step_b, idesc, 1);
-            }
-#pragma unroll
-            for (int s = 0; s < 4; ++s) mma_f16(d, ah + s * step_a, bh + s * step_b, idesc, 1);
-            mma_commit(&bars[B_EMPTY + st]);
+          for (int s = 0; s < 4; ++s) {
+            mma_f16(leader, d, al + s * step_a, bh + s * step_b, idesc, on);
+            on = 1;
+            mma_f16(leader, d, ah + s * step_a, bl + s * step_b, idesc, 1);
           }
-          if (ok) mma_commit(&bars[B_RUN + acc]);
+#pragma unroll
+          for (int s = 0; s < 4; ++s) mma_f16(leader, d, ah + s * step_a, bh + s * step_b, idesc, 1);
+          commit_by(leader, &bars[B_EMPTY + st]);
         }
+        if (ok) commit_by(leader, &bars[B_RUN + acc]);
       }
     }
   } else {

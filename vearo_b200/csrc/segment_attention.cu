@@ -190,6 +190,12 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
 // A tile of ROWS rows in shared memory: hi plane, lo plane, each of DP / 64 chunks of ROWS x 128 bytes.
 template <int ROWS, int DP> __host__ __device__ constexpr int plane_bytes() { return ROWS * DP * 2; }
 template <int ROWS, int DP>
+__device__ __forceinline__ void load_plane(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int head, int pl) {
+  mbar_arrive_expect_tx(bar, plane_bytes<ROWS, DP>());
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * ROWS * 128, map, bar, c * 64, row, head, pl);
+}
+template <int ROWS, int DP>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int head) {
   mbar_arrive_expect_tx(bar, 2 * plane_bytes<ROWS, DP>());
 #pragma unroll
@@ -197,44 +203,28 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + pl * plane_bytes<ROWS, DP>() + c * ROWS * 128, map, bar, c * 64, row, head, pl);
 }
-// D[128, N] = A[128, DP] B[N, DP]^T, both K-major tiles; the cross products first
+// D[128, N] (+)= A[128, DP] B[N, DP]^T for one plane of each, K-major tiles in shared memory; or A in tensor memory (DP / 2 columns)
 template <int N, int DP>
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b) {
-  const uint32_t idesc = idesc16(128, N, 0, 0);
-  const uint64_t ah = desc16(a, 0), al = desc16(a + plane_bytes<128, DP>(), 0), bh = desc16(b, 0), bl = desc16(b + plane_bytes<N, DP>(), 0);
-  uint32_t on = 0;
+__device__ __forceinline__ void rows_by_rows(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t on) {
+  const uint64_t da = desc16(a, 0), db = desc16(b, 0);
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k) {
-    const uint64_t oa = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4, ob = ((k >> 2) * N * 128 + (k & 3) * 32) >> 4;
-    mma_f16(d, al + oa, bh + ob, idesc, on);
-    on = 1;
-    mma_f16(d, ah + oa, bl + ob, idesc, 1);
-  }
-#pragma unroll
-  for (int k = 0; k < DP / 16; ++k) {
-    const uint64_t oa = ((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4, ob = ((k >> 2) * N * 128 + (k & 3) * 32) >> 4;
-    mma_f16(d, ah + oa, bh + ob, idesc, 1);
-  }
+  for (int k = 0; k < DP / 16; ++k, on = 1)
+    mma_f16(leader, d, da + (((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4), db + (((k >> 2) * N * 128 + (k & 3) * 32) >> 4), idesc16(128, N, 0, 0), on);
 }
-// D[128, DP] = A[128, K] B[K, DP], A in tensor memory (per quarter of the columns: K / 8 columns of hi, then of lo), B a tile of K rows
-template <int K, int DP>
-__device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b) {
+template <int N, int DP>
+__device__ __forceinline__ void kept_by_rows(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t on) {
+  const uint64_t db = desc16(b, 0);
+#pragma unroll
+  for (int k = 0; k < DP / 16; ++k, on = 1) mma_f16_ta(leader, d, a + k * 8, db + (((k >> 2) * N * 128 + (k & 3) * 32) >> 4), idesc16(128, N, 0, 0), on);
+}
+// D[128, DP] (+)= A[128, K] B[K, DP], A in tensor memory (per quarter of the columns: K / 8 columns of hi, then of lo), B a plane of K rows
+template <int K, int DP, bool LO>
+__device__ __forceinline__ void kept_by_cols(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t on) {
   constexpr int kSteps = K / 16 / kGroups;       // of a quarter
-  const uint32_t idesc = idesc16(128, DP, 0, 1);
-  const uint64_t bh = desc16(b, K * 128), bl = desc16(b + plane_bytes<K, DP>(), K * 128);
-  uint32_t on = 0;
+  const uint64_t db = desc16(b, K * 128);
 #pragma unroll
-  for (int k = 0; k < K / 16; ++k) {
-    const uint32_t hi = a + (k / kSteps) * (K / kGroups) + (k % kSteps) * 8, lo = hi + kSteps * 8;
-    mma_f16_ta(d, lo, bh + k * 128, idesc, on);
-    on = 1;
-    mma_f16_ta(d, hi, bl + k * 128, idesc, 1);
-  }
-#pragma unroll
-  for (int k = 0; k < K / 16; ++k) {
-    const uint32_t hi = a + (k / kSteps) * (K / kGroups) + (k % kSteps) * 8;
-    mma_f16_ta(d, hi, bh + k * 128, idesc, 1);
-  }
+  for (int k = 0; k < K / 16; ++k, on = 1)
+    mma_f16_ta(leader, d, a + (k / kSteps) * (K / kGroups) + (k % kSteps) * 8 + (LO ? kSteps * 8 : 0), db + k * 128, idesc16(128, DP, 0, 1), on);
 }
 // 16 columns of this thread's lane, from and to registers
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
@@ -367,7 +357,7 @@ struct Seat {
   }
 };
 
-struct Side { const float* inv; const float* len; const uint32_t* bad; };
+struct Side { const __half* planes; const float* inv; const float* len; const uint32_t* bad; };
 struct AttnParams {
   int T, tiles, hq, hk, dk;
   float scale;
@@ -381,31 +371,41 @@ struct AttnParams {
 };
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------
-template <int DP> struct FwdSmem {
-  static constexpr int kTile = 2 * plane_bytes<128, DP>(), kStages = DP == 64 ? 2 : 1;
-  static constexpr int kBars = 1 + 4 * kStages + 2 + 1 + 1;
-  static constexpr int kTotal = 1024 + kTile * (1 + 2 * kStages) + 2 * kGroups * 128 * 4 + kBars * 8 + 64;
+// The resident tile (Q, or K in the dV kernel) and a ring of planes, streamed in the order in which the products take them: half a tile
+// at a time, so that 128-wide heads too have a product's worth of planes in flight.
+template <int DP> struct StreamSmem {
+  static constexpr int kPlane = plane_bytes<128, DP>(), kSlots = DP == 64 ? 10 : 5;
+  static constexpr int kBars = 1 + 2 * kSlots + 2 + 1 + 1;
+  static constexpr int kTotal = 1024 + kPlane * (2 + kSlots) + kBars * 8 + 64;
+  // the forward kernel's row maxima: two buffers, or one where there is no room for two
+  static constexpr int kBuffers = DP == 64 ? 2 : 1, kExchange = kBuffers * kGroups * 128 * 4;
+  static constexpr int kForward = kTotal + kExchange < 232448 ? kTotal + kExchange : 232448;      // (227 KB: with 128-wide heads 840 of the 1024 bytes for alignment are left)
 };
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p) {
-  using L = FwdSmem<DP>;
-  constexpr int NS = L::kStages, W = DP / kGroups, H = 128 / kGroups;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t *sq = smem, *sk = smem + L::kTile, *sv = sk + NS * L::kTile;
-  float* xchg = (float*)(sv + NS * L::kTile);                 // [2 tiles][groups][128]
-  uint64_t* bars = (uint64_t*)(xchg + 2 * kGroups * 128);
-  uint64_t *b_q = bars, *b_kfull = bars + 1, *b_vfull = b_kfull + NS, *b_kfree = b_vfull + NS, *b_vfree = b_kfree + NS, *b_s = b_vfree + NS, *b_p = b_s + 2, *b_o = b_p + 1;
+  using L = StreamSmem<DP>;
+  constexpr int NS = L::kSlots, W = DP / kGroups, H = 128 / kGroups;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t shift = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
+  uint8_t* smem = smem_raw + shift;
+  if (shift + L::kTotal - 1024 + L::kExchange > L::kForward) {      // (an aligned base, as every launch has had, always fits)
+    if (threadIdx.x == 0) atomicOr(p.err, ERRBIT_BOUNDS);
+    return;
+  }
+  uint8_t *sq = smem, *ring = smem + 2 * L::kPlane;
+  uint64_t* bars = (uint64_t*)(ring + NS * L::kPlane);
+  uint64_t *b_x = bars, *b_full = bars + 1, *b_free = b_full + NS, *b_s = b_free + NS, *b_p = b_s + 2, *b_o = b_p + 1;
   int* ints = (int*)(b_o + 1);
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
+  float* xchg = (float*)(ints + 4);                           // [kBuffers tiles][groups][128]
 
   const int warp = threadIdx.x >> 5;
   const int h = blockIdx.x % p.hq, hk = h / (p.hq / p.hk), qt = p.tiles - 1 - (int)(blockIdx.x / p.hq);      // long tiles first
   if (threadIdx.x == 0) {
-    mbar_init(b_q, 1);
-    for (int i = 0; i < NS; ++i) { mbar_init(&b_kfull[i], 1); mbar_init(&b_vfull[i], 1); mbar_init(&b_kfree[i], 1); mbar_init(&b_vfree[i], 1); }
+    mbar_init(b_x, 1);
+    for (int i = 0; i < NS; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_free[i], 1); }
     mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -423,41 +423,53 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
 
   if (warp == 0) {
     if ((threadIdx.x & 31) == 0 && n > 0) {
-      bool ok = true;
-      load_tile<128, DP>(sq, &map_q, b_q, qt * 128, h);
-      for (int j = 0; j < n && ok; ++j) {
-        const int st = j % NS, ph = ((j / NS) - 1) & 1;
-        if (j >= NS) ok = mbar_wait(&b_kfree[st], ph, abort_flag);
-        if (!ok) break;
-        load_tile<128, DP>(sk + st * L::kTile, &map_k, &b_kfull[st], (kb0 + j) * 128, hk);
-        if (j >= NS) ok = mbar_wait(&b_vfree[st], ph, abort_flag);
-        if (!ok) break;
-        load_tile<128, DP>(sv + st * L::kTile, &map_v, &b_vfull[st], (kb0 + j) * 128, hk);
-      }
-      if (*abort_flag) let_land(bars, 1 + 2 * NS);
+      load_tile<128, DP>(sq, &map_q, b_x, qt * 128, h);
+      uint32_t slot = 0, phase = 1;      // (the first round waits on the phase before the first: free)
+      auto fetch = [&](const CUtensorMap* map, int j) -> bool {      // lo, then hi: the order in which the products take them
+        for (int pl = 1; pl >= 0; --pl) {
+          if (!mbar_wait(&b_free[slot], phase, abort_flag)) return false;
+          load_plane<128, DP>(ring + slot * L::kPlane, map, &b_full[slot], (kb0 + j) * 128, hk, pl);
+          if (++slot == NS) { slot = 0; phase ^= 1; }
+        }
+        return true;
+      };
+      bool ok = fetch(&map_k, 0) && (n < 2 || fetch(&map_k, 1));
+      for (int j = 0; j < n && ok; ++j) ok = fetch(&map_v, j) && (j + 2 >= n || fetch(&map_k, j + 2));
+      if (*abort_flag) let_land(bars, 1 + NS);
     }
   } else if (warp == 1) {
-    if ((threadIdx.x & 31) == 0 && n > 0) {
-      bool ok = mbar_wait(b_q, 0, abort_flag);
+    if (n > 0) {
+      const uint32_t leader = elect_leader();
+      uint32_t slot = 0, phase = 0;
+      bool ok = warp_wait(b_x, 0, abort_flag);
+      auto next = [&]() -> bool { const bool r = warp_wait(&b_full[slot], phase, abort_flag); tc_fence_after(); return r; };
+      auto release = [&]() { commit_by(leader, &b_free[slot]); if (++slot == NS) { slot = 0; phase ^= 1; } };
+      const uint32_t x_hi = smem_u32(sq), x_lo = x_hi + L::kPlane, r0 = smem_u32(ring);
       auto scores = [&](int j) -> bool {
-        const int st = j % NS;
-        if (!mbar_wait(&b_kfull[st], (j / NS) & 1, abort_flag)) return false;
-        tc_fence_after();
-        product_rows<128, DP>(t_s + (j & 1) * 128, smem_u32(sq), smem_u32(sk + st * L::kTile));
-        mma_commit(&b_kfree[st]);
-        mma_commit(&b_s[j & 1]);
+        const uint32_t d = t_s + (j & 1) * 128;
+        if (!next()) return false;
+        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 0);
+        release();
+        if (!next()) return false;
+        rows_by_rows<128, DP>(leader, d, x_lo, r0 + slot * L::kPlane, 1);
+        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 1);
+        release();
+        commit_by(leader, &b_s[j & 1]);
         return true;
       };
       if (ok) ok = scores(0);
       if (ok && n > 1) ok = scores(1);
       for (int j = 0; j < n && ok; ++j) {
-        const int st = j % NS;
-        ok = mbar_wait(b_p, j & 1, abort_flag) && mbar_wait(&b_vfull[st], (j / NS) & 1, abort_flag);
+        ok = warp_wait(b_p, j & 1, abort_flag) && next();
         if (!ok) break;
-        tc_fence_after();
-        product_cols<128, DP>(t_o, t_p, smem_u32(sv + st * L::kTile));
-        mma_commit(&b_vfree[st]);
-        mma_commit(b_o);
+        kept_by_cols<128, DP, false>(leader, t_o, t_p, r0 + slot * L::kPlane, 0);
+        release();
+        ok = next();
+        if (!ok) break;
+        kept_by_cols<128, DP, true>(leader, t_o, t_p, r0 + slot * L::kPlane, 1);
+        kept_by_cols<128, DP, false>(leader, t_o, t_p, r0 + slot * L::kPlane, 1);
+        release();
+        commit_by(leader, b_o);
         if (j + 2 < n) ok = scores(j + 2);      // (this tile's scores have been read: P says so)
       }
     }
@@ -490,7 +502,8 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
 #pragma unroll
       for (int i = 4; i < H; i += 4) { m0 = fmaxf(m0, fmaxf(v[i], v[i + 1])); m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3])); }
-      float* x = xchg + (j & 1) * kGroups * 128 + at.row;
+      float* x = xchg + (j & (L::kBuffers - 1)) * kGroups * 128 + at.row;
+      if (L::kBuffers == 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
       x[at.group * 128] = fmaxf(m0, m1);
       asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");      // the four quarters of these rows
       const float mn = fmaxf(m, fmaxf(fmaxf(x[0], x[128]), fmaxf(x[256], x[384])) * sc), ref = mn > -INFINITY ? mn : 0.0f;
@@ -516,7 +529,8 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       tc_fence_after();
       add_part<W>(t_o + at.group * W + at.lane_off, acc, keep, v_last);
     }
-    float* x = xchg + (n & 1) * kGroups * 128 + at.row;
+    float* x = xchg + (n & (L::kBuffers - 1)) * kGroups * 128 + at.row;
+    if (L::kBuffers == 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
     x[at.group * 128] = l;
     asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
     l = (x[0] + x[128]) + (x[256] + x[384]);
@@ -536,22 +550,17 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
 // ---- backward ---------------------------------------------------------------------------------------------------------------------
 // One launch for the three gradients: CTAs that make dK come first (three products for every query head of the group), then dV (two),
 // then dQ, so that the long ones start first and the short ones fill the gaps.
-struct BwdMaps { CUtensorMap q, k, v, g, qn, kn, vn, gn; };      // boxes of 128 rows, and of N rows (GradSmem)
+struct BwdMaps { CUtensorMap q, k, g, qn, kn, vn, gn; };      // boxes of 128 rows, and of N rows (GradSmem)
 
 // dV of 128 keys: every query head of the CTA's part of the group x every tile of 128 queries from the keys' own to the last one that
 // sees them.
-template <int DP> struct GradVSmem {
-  static constexpr int kTile = 2 * plane_bytes<128, DP>(), kStages = DP == 64 ? 2 : 1;
-  static constexpr int kBars = 1 + 4 * kStages + 2 + 1 + 1;
-  static constexpr int kTotal = 1024 + kTile * (1 + 2 * kStages) + kBars * 8 + 64;
-};
 template <int DP>
 __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const AttnParams& p, int block) {
-  using L = GradVSmem<DP>;
-  constexpr int NS = L::kStages, W = DP / kGroups, H = 128 / kGroups;
-  uint8_t *sk = smem, *sq = smem + L::kTile, *sg = sq + NS * L::kTile;
-  uint64_t* bars = (uint64_t*)(sg + NS * L::kTile);
-  uint64_t *b_k = bars, *b_qfull = bars + 1, *b_gfull = b_qfull + NS, *b_qfree = b_gfull + NS, *b_gfree = b_qfree + NS, *b_s = b_gfree + NS, *b_p = b_s + 2, *b_o = b_p + 1;
+  using L = StreamSmem<DP>;
+  constexpr int NS = L::kSlots, W = DP / kGroups, H = 128 / kGroups;
+  uint8_t *sk = smem, *ring = smem + 2 * L::kPlane;
+  uint64_t* bars = (uint64_t*)(ring + NS * L::kPlane);
+  uint64_t *b_x = bars, *b_full = bars + 1, *b_free = b_full + NS, *b_s = b_free + NS, *b_p = b_s + 2, *b_o = b_p + 1;
   int* ints = (int*)(b_o + 1);
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
@@ -559,8 +568,8 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
   const int warp = threadIdx.x >> 5;
   const int part = block % p.parts, hk = block / p.parts % p.hk, kt = block / p.parts / p.hk, heads = p.hq / p.hk / p.parts, h0 = (hk * p.parts + part) * heads;
   if (threadIdx.x == 0) {
-    mbar_init(b_k, 1);
-    for (int i = 0; i < NS; ++i) { mbar_init(&b_qfull[i], 1); mbar_init(&b_gfull[i], 1); mbar_init(&b_qfree[i], 1); mbar_init(&b_gfree[i], 1); }
+    mbar_init(b_x, 1);
+    for (int i = 0; i < NS; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_free[i], 1); }
     mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -578,42 +587,54 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
 
   if (warp == 0) {
     if ((threadIdx.x & 31) == 0 && n > 0) {
-      bool ok = true;
-      load_tile<128, DP>(sk, &maps.k, b_k, kt * 128, hk);
-      for (int j = 0; j < n && ok; ++j) {
-        const int st = j % NS, ph = ((j / NS) - 1) & 1, h = h0 + j / per, i = kt + j % per;
-        if (j >= NS) ok = mbar_wait(&b_qfree[st], ph, abort_flag);
-        if (!ok) break;
-        load_tile<128, DP>(sq + st * L::kTile, &maps.q, &b_qfull[st], i * 128, h);
-        if (j >= NS) ok = mbar_wait(&b_gfree[st], ph, abort_flag);
-        if (!ok) break;
-        load_tile<128, DP>(sg + st * L::kTile, &maps.g, &b_gfull[st], i * 128, h);
-      }
-      if (*abort_flag) let_land(bars, 1 + 2 * NS);
+      load_tile<128, DP>(sk, &maps.k, b_x, kt * 128, hk);
+      uint32_t slot = 0, phase = 1;      // (the first round waits on the phase before the first: free)
+      auto fetch = [&](const CUtensorMap* map, int j) -> bool {      // lo, then hi: the order in which the products take them
+        for (int pl = 1; pl >= 0; --pl) {
+          if (!mbar_wait(&b_free[slot], phase, abort_flag)) return false;
+          load_plane<128, DP>(ring + slot * L::kPlane, map, &b_full[slot], (kt + j % per) * 128, h0 + j / per, pl);
+          if (++slot == NS) { slot = 0; phase ^= 1; }
+        }
+        return true;
+      };
+      bool ok = fetch(&maps.q, 0) && (n < 2 || fetch(&maps.q, 1));
+      for (int j = 0; j < n && ok; ++j) ok = fetch(&maps.g, j) && (j + 2 >= n || fetch(&maps.q, j + 2));
+      if (*abort_flag) let_land(bars, 1 + NS);
     }
   } else if (warp == 1) {
-    if ((threadIdx.x & 31) == 0 && n > 0) {
-      bool ok = mbar_wait(b_k, 0, abort_flag);
+    if (n > 0) {
+      const uint32_t leader = elect_leader();
+      uint32_t slot = 0, phase = 0;
+      bool ok = warp_wait(b_x, 0, abort_flag);
+      auto next = [&]() -> bool { const bool r = warp_wait(&b_full[slot], phase, abort_flag); tc_fence_after(); return r; };
+      auto release = [&]() { commit_by(leader, &b_free[slot]); if (++slot == NS) { slot = 0; phase ^= 1; } };
+      const uint32_t x_hi = smem_u32(sk), x_lo = x_hi + L::kPlane, r0 = smem_u32(ring);
       auto scores = [&](int j) -> bool {
-        const int st = j % NS;
-        if (!mbar_wait(&b_qfull[st], (j / NS) & 1, abort_flag)) return false;
-        tc_fence_after();
-        product_rows<128, DP>(t_s + (j & 1) * 128, smem_u32(sk), smem_u32(sq + st * L::kTile));
-        mma_commit(&b_qfree[st]);
-        mma_commit(&b_s[j & 1]);
+        const uint32_t d = t_s + (j & 1) * 128;
+        if (!next()) return false;
+        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 0);
+        release();
+        if (!next()) return false;
+        rows_by_rows<128, DP>(leader, d, x_lo, r0 + slot * L::kPlane, 1);
+        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 1);
+        release();
+        commit_by(leader, &b_s[j & 1]);
         return true;
       };
       if (ok) ok = scores(0);
       if (ok && n > 1) ok = scores(1);
       for (int j = 0; j < n && ok; ++j) {
-        const int st = j % NS;
-        ok = mbar_wait(b_p, j & 1, abort_flag) && mbar_wait(&b_gfull[st], (j / NS) & 1, abort_flag);
+        ok = warp_wait(b_p, j & 1, abort_flag) && next();
         if (!ok) break;
-        tc_fence_after();
-        product_cols<128, DP>(t_o, t_p, smem_u32(sg + st * L::kTile));
-        mma_commit(&b_gfree[st]);
-        mma_commit(b_o);
-        if (j + 2 < n) ok = scores(j + 2);
+        kept_by_cols<128, DP, false>(leader, t_o, t_p, r0 + slot * L::kPlane, 0);
+        release();
+        ok = next();
+        if (!ok) break;
+        kept_by_cols<128, DP, true>(leader, t_o, t_p, r0 + slot * L::kPlane, 1);
+        kept_by_cols<128, DP, false>(leader, t_o, t_p, r0 + slot * L::kPlane, 1);
+        release();
+        commit_by(leader, b_o);
+        if (j + 2 < n) ok = scores(j + 2);      // (this tile's scores have been read: P says so)
       }
     }
   } else {
@@ -661,23 +682,24 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
 
 // dQ and dK.  X (128 rows, resident: q and do, or k and v), Y streamed in tiles of N rows (k and v, or q and do):
 //   S = X1 Y1^T, dP = X2 Y2^T, dS = p (dP - delta), result += dS Y1.
-// dS goes where S was; S has two buffers, so the next tile's S and dP are formed while dS Y1 runs.
+// dS goes where S was; S has two buffers, so the next tile's S and dP are formed while dS Y1 runs.  Y1 is held from S to the last
+// product, so it has three buffers; X2 is kept in tensor memory, as the left operand of dP, to leave room for them.
 template <int DP> struct GradSmem {
-  static constexpr int N = DP == 64 ? 128 : 64;                       // 128-wide heads: 64 rows of Y at a time fit beside X
+  static constexpr int N = DP == 64 ? 128 : 64;                       // 128-wide heads: 64 rows of Y at a time
   static constexpr int kTileX = 2 * plane_bytes<128, DP>(), kTileY = 2 * plane_bytes<N, DP>();
-  static constexpr int kStages2 = DP == 64 ? 2 : 1;                   // Y1 is held through the last product (two tiles), Y2 is not
-  static constexpr int kBars = 2 + 4 + 2 * kStages2 + 2 + 1 + 1 + 1;
-  static constexpr int kTotal = 1024 + 2 * kTileX + (2 + kStages2) * kTileY + kBars * 8 + 64;
+  static constexpr int kY1 = 3, kY2 = 2;
+  static constexpr int kBars = 2 + 2 * kY1 + 2 * kY2 + 2 + 1 + 1 + 1;
+  static constexpr int kTotal = 1024 + kTileX + (kY1 + kY2) * kTileY + kBars * 8 + 64;
 };
 template <int DP, bool DK>
 __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, const AttnParams& p, int block) {
   using L = GradSmem<DP>;
-  constexpr int N = L::N, H = N / kGroups, W = DP / kGroups, NS2 = L::kStages2, R = 128 / N;
-  uint8_t *x1 = smem, *x2 = x1 + L::kTileX, *y1 = x2 + L::kTileX, *y2 = y1 + 2 * L::kTileY;
-  uint64_t* bars = (uint64_t*)(y2 + NS2 * L::kTileY);
-  uint64_t *b_x = bars, *b_y1full = bars + 2, *b_y2full = b_y1full + 2, *b_y1free = b_y2full + NS2, *b_y2free = b_y1free + 2, *b_s = b_y2free + NS2, *b_dp = b_s + 2,
-           *b_ds = b_dp + 1, *b_o = b_ds + 1;
-  int* ints = (int*)(b_o + 1);
+  constexpr int N = L::N, H = N / kGroups, W = DP / kGroups, N1 = L::kY1, N2 = L::kY2, R = 128 / N;
+  uint8_t *x1 = smem, *y1 = x1 + L::kTileX, *y2 = y1 + N1 * L::kTileY;
+  uint64_t* bars = (uint64_t*)(y2 + N2 * L::kTileY);
+  uint64_t *b_x = bars, *b_y1full = bars + 1, *b_y2full = b_y1full + N1, *b_y1free = b_y2full + N2, *b_y2free = b_y1free + N1, *b_s = b_y2free + N2, *b_dp = b_s + 2,
+           *b_ds = b_dp + 1, *b_o = b_ds + 1, *b_x2 = b_o + 1;
+  int* ints = (int*)(b_x2 + 1);
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
   float* vmax_slot = (float*)ints + 4;
@@ -687,9 +709,9 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
   const int hx = rest % x_heads, hk = DK ? hx : hx / (p.hq / p.hk), heads = DK ? p.hq / p.hk / p.parts : 1, h0 = DK ? (hk * p.parts + part) * heads : hx;
   const int xt = DK ? rest / x_heads : p.tiles - 1 - rest / x_heads;
   if (threadIdx.x == 0) {
-    mbar_init(&b_x[0], 1); mbar_init(&b_x[1], 1);
-    for (int i = 0; i < 2; ++i) { mbar_init(&b_y1full[i], 1); mbar_init(&b_y1free[i], 1); mbar_init(&b_s[i], 1); }
-    for (int i = 0; i < NS2; ++i) { mbar_init(&b_y2full[i], 1); mbar_init(&b_y2free[i], 1); }
+    mbar_init(b_x, 1); mbar_init(b_x2, kRowWarps); mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1);
+    for (int i = 0; i < N1; ++i) { mbar_init(&b_y1full[i], 1); mbar_init(&b_y1free[i], 1); }
+    for (int i = 0; i < N2; ++i) { mbar_init(&b_y2full[i], 1); mbar_init(&b_y2free[i], 1); }
     mbar_init(b_dp, 1); mbar_init(b_ds, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     *vmax_slot = 0.0f;
@@ -711,63 +733,71 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t t_s = tmem, t_dp = tmem + 256, t_o = tmem + 384;
+  const uint32_t t_s = tmem, t_dp = tmem + 2 * N, t_x2 = tmem + 3 * N, t_o = t_x2 + DP;      // (DP columns of X2: hi, lo)
   const float vmax = *vmax_slot;
   // tiles of Y, in steps of N rows
   int y0, per;
   if (DK) { y0 = xt * R; per = e_max > 0 ? (e_max - 1) / N - y0 + 1 : 0; }
   else { const int last = xt * 128 + 127 < p.T ? xt * 128 + 127 : p.T - 1; y0 = e_min / N; per = e_min < p.T ? last / N - y0 + 1 : 0; }
   const int n = per * heads;
-  const CUtensorMap *map_x1 = DK ? &maps.k : &maps.q, *map_x2 = DK ? &maps.v : &maps.g, *map_y1 = DK ? &maps.qn : &maps.kn, *map_y2 = DK ? &maps.gn : &maps.vn;
+  const CUtensorMap *map_x1 = DK ? &maps.k : &maps.q, *map_y1 = DK ? &maps.qn : &maps.kn, *map_y2 = DK ? &maps.gn : &maps.vn;
 
   if (warp == 0) {
     if ((threadIdx.x & 31) == 0 && n > 0) {
       bool ok = true;
-      load_tile<128, DP>(x1, map_x1, &b_x[0], xt * 128, hx);
+      load_tile<128, DP>(x1, map_x1, b_x, xt * 128, hx);
       for (int j = 0; j < n && ok; ++j) {
-        const int hy = DK ? h0 + j / per : hk, y = (y0 + (DK ? j % per : j)) * N;
-        if (j >= 2) ok = mbar_wait(&b_y1free[j & 1], ((j >> 1) - 1) & 1, abort_flag);
+        const int hy = DK ? h0 + j / per : hk, y = (y0 + (DK ? j % per : j)) * N, s1 = j % N1, s2 = j % N2;
+        if (j >= N1) ok = mbar_wait(&b_y1free[s1], ((j / N1) - 1) & 1, abort_flag);
         if (!ok) break;
-        load_tile<N, DP>(y1 + (j & 1) * L::kTileY, map_y1, &b_y1full[j & 1], y, hy);
-        if (j == 0) load_tile<128, DP>(x2, map_x2, &b_x[1], xt * 128, hx);
-        const int st = j % NS2;
-        if (j >= NS2) ok = mbar_wait(&b_y2free[st], ((j / NS2) - 1) & 1, abort_flag);
+        load_tile<N, DP>(y1 + s1 * L::kTileY, map_y1, &b_y1full[s1], y, hy);
+        if (j >= N2) ok = mbar_wait(&b_y2free[s2], ((j / N2) - 1) & 1, abort_flag);
         if (!ok) break;
-        load_tile<N, DP>(y2 + st * L::kTileY, map_y2, &b_y2full[st], y, hy);
+        load_tile<N, DP>(y2 + s2 * L::kTileY, map_y2, &b_y2full[s2], y, hy);
       }
-      if (*abort_flag) let_land(bars, 4 + NS2);
+      if (*abort_flag) let_land(bars, 1 + N1 + N2);
     }
   } else if (warp == 1) {
-    if ((threadIdx.x & 31) == 0 && n > 0) {
-      bool ok = mbar_wait(&b_x[0], 0, abort_flag);
+    if (n > 0) {
+      const uint32_t leader = elect_leader();
+      constexpr int kPX = plane_bytes<128, DP>(), kPY = plane_bytes<N, DP>();
+      bool ok = warp_wait(b_x, 0, abort_flag);
       auto scores = [&](int j) -> bool {      // (buffer j & 1 held dS of tile j - 2, which its product has read)
-        if (!mbar_wait(&b_y1full[j & 1], (j >> 1) & 1, abort_flag)) return false;
-        if (j >= 2 && !mbar_wait(b_o, j & 1, abort_flag)) return false;
+        if (!warp_wait(&b_y1full[j % N1], (j / N1) & 1, abort_flag)) return false;
+        if (j >= 2 && !warp_wait(b_o, j & 1, abort_flag)) return false;
         tc_fence_after();
-        product_rows<N, DP>(t_s + (j & 1) * 128, smem_u32(x1), smem_u32(y1 + (j & 1) * L::kTileY));
-        mma_commit(&b_s[j & 1]);
+        const uint32_t d = t_s + (j & 1) * N, x = smem_u32(x1), y = smem_u32(y1 + (j % N1) * L::kTileY);
+        rows_by_rows<N, DP>(leader, d, x + kPX, y, 0);
+        rows_by_rows<N, DP>(leader, d, x, y + kPY, 1);
+        rows_by_rows<N, DP>(leader, d, x, y, 1);
+        commit_by(leader, &b_s[j & 1]);
         return true;
       };
       auto other = [&](int j) -> bool {
-        const int st = j % NS2;
-        if (!mbar_wait(&b_y2full[st], (j / NS2) & 1, abort_flag)) return false;
+        if (!warp_wait(&b_y2full[j % N2], (j / N2) & 1, abort_flag)) return false;
         tc_fence_after();
-        product_rows<N, DP>(t_dp, smem_u32(x2), smem_u32(y2 + st * L::kTileY));
-        mma_commit(&b_y2free[st]);
-        mma_commit(b_dp);
+        const uint32_t y = smem_u32(y2 + (j % N2) * L::kTileY);
+        kept_by_rows<N, DP>(leader, t_dp, t_x2 + DP / 2, y, 0);
+        kept_by_rows<N, DP>(leader, t_dp, t_x2, y + kPY, 1);
+        kept_by_rows<N, DP>(leader, t_dp, t_x2, y, 1);
+        commit_by(leader, &b_y2free[j % N2]);
+        commit_by(leader, b_dp);
         return true;
       };
-      if (ok) ok = scores(0) && mbar_wait(&b_x[1], 0, abort_flag) && other(0);
+      if (ok) ok = scores(0) && warp_wait(b_x2, 0, abort_flag) && other(0);
       if (ok && n > 1) ok = scores(1);
       for (int j = 0; j < n && ok; ++j) {
-        ok = mbar_wait(b_ds, j & 1, abort_flag);
+        ok = warp_wait(b_ds, j & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
         if (j + 1 < n) ok = other(j + 1);
         if (!ok) break;
-        product_cols<N, DP>(t_o, t_s + (j & 1) * 128, smem_u32(y1 + (j & 1) * L::kTileY));
-        mma_commit(&b_y1free[j & 1]);
-        mma_commit(b_o);
+        const uint32_t ds = t_s + (j & 1) * N, y = smem_u32(y1 + (j % N1) * L::kTileY);
+        kept_by_cols<N, DP, true>(leader, t_o, ds, y, 0);
+        kept_by_cols<N, DP, false>(leader, t_o, ds, y + kPY, 1);
+        kept_by_cols<N, DP, false>(leader, t_o, ds, y, 1);
+        commit_by(leader, &b_y1free[j % N1]);
+        commit_by(leader, b_o);
         if (j + 2 < n) ok = scores(j + 2);
       }
     }
@@ -775,6 +805,16 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     const Seat at;
     const int t = xt * 128 + at.row;
     const int mine = DK ? (t < p.T ? p.end[t] : 0) : (t < p.T ? p.begin[t] : p.T);
+    {   // X2 into tensor memory: hi from groups 0 and 1, lo from 2 and 3, half a row each
+      uint4 w[DP / 16];
+      const Side& x2 = DK ? p.v : p.g;
+      const uint4* src = reinterpret_cast<const uint4*>(x2.planes + ((i64)(at.group >> 1) * x_heads * p.T + (i64)hx * p.T + t) * DP) + (at.group & 1) * (DP / 16);
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) w[i] = t < p.T ? src[i] : make_uint4(0, 0, 0, 0);
+      if constexpr (DP == 64) tmem_st16(t_x2 + at.group * 16 + at.lane_off, reinterpret_cast<const uint32_t*>(w));
+      else tmem_st32(t_x2 + at.group * 32 + at.lane_off, reinterpret_cast<const uint32_t*>(w));
+      operand_written(b_x2, at.lane);
+    }
     const i64 x_at = (i64)hx * p.tiles + xt;
     const float s_x = p.scale * kL2e * fabsf(DK ? p.k.inv[x_at] : p.q.inv[x_at]);
     // 2^e with 2 |do| |v| 2^e below 2^14, and its inverse
@@ -812,7 +852,7 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
       if (!mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
       float v[H];
-      load_cols<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
+      load_cols<H>(t_s + (j & 1) * N + at.group * H + at.lane_off, v);
       if (DK) weights_of_cols<H>(v, sc, p.lse2 + col);
       else weights_of_row<H>(v, sc, lse_row);
       const bool crossed = DK ? y < xt * 128 + 128 || y + N > e_min : y + N > xt * 128 || y < e_max;
@@ -832,7 +872,7 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
       }
       if (crossed) keep_columns<H>(v, (DK ? t : mine) - c0, (DK ? mine - 1 : t) - c0, 0.0f);
       // (a quarter's dS lies within its own quarter of S)
-      store_operand<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
+      store_operand<H>(t_s + (j & 1) * N + at.group * H + at.lane_off, v);
       if (j > 0) {
         if (!mbar_wait(b_o, (j - 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
@@ -930,7 +970,7 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
   for (int i = 0; i < n; ++i) {
     d.in[i] = PlanesDev{in[i].p, in[i].st, in[i].sh, (__half*)(base + planes[i]), (float*)(base + inv[i]), (float*)(base + len[i]), (uint32_t*)(base + bad[i]), heads[i],
                         s.dk % 4 == 0 && in[i].st % 4 == 0 && in[i].sh % 4 == 0 && (reinterpret_cast<uintptr_t>(in[i].p) & 15) == 0};
-    *sides[i] = Side{d.in[i].inv, d.in[i].len, d.in[i].bad};
+    *sides[i] = Side{d.in[i].planes, d.in[i].inv, d.in[i].len, d.in[i].bad};
     all += heads[i];
   }
   d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.err = ctx().d_err;
@@ -953,23 +993,23 @@ int allow_smem(K kernel, int bytes) {
 
 template <int DP>
 int forward(Work& w) {
-  static const int ready = allow_smem(k_forward<DP>, FwdSmem<DP>::kTotal);
+  static const int ready = allow_smem(k_forward<DP>, StreamSmem<DP>::kForward);
   VB_TRY(ready);
   CUtensorMap mq, mk, mv;
   VB_TRY(make_map(&mq, w.prep.in[0], w.p.T, DP, 128)); VB_TRY(make_map(&mk, w.prep.in[1], w.p.T, DP, 128)); VB_TRY(make_map(&mv, w.prep.in[2], w.p.T, DP, 128));
-  k_forward<DP><<<(unsigned)w.p.hq * w.p.tiles, kThreads, FwdSmem<DP>::kTotal, ctx().stream>>>(mq, mk, mv, w.p);
+  k_forward<DP><<<(unsigned)w.p.hq * w.p.tiles, kThreads, StreamSmem<DP>::kForward, ctx().stream>>>(mq, mk, mv, w.p);
   VB_LAUNCH_CHECK();
   return VB_OK;
 }
 template <int DP>
 int backward(Work& w, float* dq, float* dk, float* dv) {
-  constexpr int N = GradSmem<DP>::N, kSmem = GradSmem<DP>::kTotal > GradVSmem<DP>::kTotal ? GradSmem<DP>::kTotal : GradVSmem<DP>::kTotal;
+  constexpr int N = GradSmem<DP>::N, kSmem = GradSmem<DP>::kTotal > StreamSmem<DP>::kTotal ? GradSmem<DP>::kTotal : StreamSmem<DP>::kTotal;
   static const int ready = allow_smem(k_backward<DP>, kSmem);
   VB_TRY(ready);
   BwdMaps m;
   const PlanesDev* in = w.prep.in;
   AttnParams& p = w.p;
-  VB_TRY(make_map(&m.q, in[0], p.T, DP, 128)); VB_TRY(make_map(&m.k, in[1], p.T, DP, 128)); VB_TRY(make_map(&m.v, in[2], p.T, DP, 128)); VB_TRY(make_map(&m.g, in[3], p.T, DP, 128));
+  VB_TRY(make_map(&m.q, in[0], p.T, DP, 128)); VB_TRY(make_map(&m.k, in[1], p.T, DP, 128)); VB_TRY(make_map(&m.g, in[3], p.T, DP, 128));
   VB_TRY(make_map(&m.qn, in[0], p.T, DP, N)); VB_TRY(make_map(&m.kn, in[1], p.T, DP, N)); VB_TRY(make_map(&m.vn, in[2], p.T, DP, N)); VB_TRY(make_map(&m.gn, in[3], p.T, DP, N));
   // A CTA that walks the query heads of a whole group is the longest of the launch: where dK and dV have fewer than four CTAs for
   // every SM the group is dealt to several, whose sums are added afterwards.
