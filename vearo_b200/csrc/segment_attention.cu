@@ -299,6 +299,22 @@ __device__ __forceinline__ void weights_of_row(float (&v)[W], float sc, float of
     v[i] = exp2_fast(x.x); v[i + 1] = exp2_fast(x.y);
   }
 }
+// the same as the left operand of product_cols (W / 2 registers of hi, W / 2 of lo), and their sum
+template <int W>
+__device__ __forceinline__ float split_weights(const float (&v)[W], float sc, float off, uint32_t (&r)[W]) {
+  const float2 s2 = make_float2(sc, sc), o2 = make_float2(off, off);
+  float2 a = make_float2(0.0f, 0.0f), b = a;
+#pragma unroll
+  for (int i = 0; i < W; i += 4) {
+    float2 x = fma2(make_float2(v[i], v[i + 1]), s2, o2), y = fma2(make_float2(v[i + 2], v[i + 3]), s2, o2);
+    x.x = exp2_fast(x.x); x.y = exp2_fast(x.y); y.x = exp2_fast(y.x); y.y = exp2_fast(y.y);
+    a = add2(a, x); b = add2(b, y);
+    split2_finite(x.x, x.y, &r[i / 2], &r[W / 2 + i / 2]);
+    split2_finite(y.x, y.y, &r[i / 2 + 1], &r[W / 2 + i / 2 + 1]);
+  }
+  a = add2(a, b);
+  return a.x + a.y;
+}
 template <int W>
 __device__ __forceinline__ void weights_of_cols(float (&v)[W], float sc, const float* lse2) {
   const float2 s2 = make_float2(sc, sc), c14 = make_float2(14.0f, 14.0f), neg = make_float2(-1.0f, -1.0f);
@@ -314,12 +330,12 @@ __device__ __forceinline__ void keep_columns(float (&v)[W], int first, int last,
 #pragma unroll
   for (int i = 0; i < W; ++i) if (i < first || i > last) v[i] = other;
 }
-__device__ __forceinline__ void tmem_alloc(uint32_t* slot) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(512u) : "memory");
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_free(uint32_t tmem) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 // copies already issued get a bounded time to land before a CTA that gave up exits
 __device__ __forceinline__ void let_land(uint64_t* bars, int n) {
@@ -377,19 +393,25 @@ template <int DP> struct StreamSmem {
   static constexpr int kPlane = plane_bytes<128, DP>(), kSlots = DP == 64 ? 10 : 5;
   static constexpr int kBars = 1 + 2 * kSlots + 2 + 1 + 1;
   static constexpr int kTotal = 1024 + kPlane * (2 + kSlots) + kBars * 8 + 64;
-  // the forward kernel's row maxima: two buffers, or one where there is no room for two
-  static constexpr int kBuffers = DP == 64 ? 2 : 1, kExchange = kBuffers * kGroups * 128 * 4;
-  static constexpr int kForward = kTotal + kExchange < 232448 ? kTotal + kExchange : 232448;      // (227 KB: with 128-wide heads 840 of the 1024 bytes for alignment are left)
+};
+// One CTA an SM, sixteen row warps.  Scores have two buffers, so the next tile's are formed while the row warps are at this one's; a
+// weight is split into its halves where its exponential comes out, so that the special-function and the arithmetic pipes work at
+// the same time, and before the wait for the last product, which still reads the last P.
+template <int DP> struct FwdCfg {
+  static constexpr int kPlane = plane_bytes<128, DP>(), kSlots = DP == 64 ? 10 : 5, kBars = 1 + 2 * kSlots + 2 + 1 + 1;
+  static constexpr int kBuffers = DP == 64 ? 2 : 1, kExchange = kBuffers * kGroups * 128 * 4;      // row maxima, and accumulators: one buffer where there is no room for two
+  static constexpr int kNeed = kPlane * (2 + kSlots) + kExchange + kBars * 8 + 64;
+  static constexpr int kTotal = kNeed + 1024 < 232448 ? kNeed + 1024 : 232448;               // (227 KB: with wide heads 840 of the 1024 bytes for alignment are left)
 };
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1)
 k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnParams p) {
-  using L = StreamSmem<DP>;
-  constexpr int NS = L::kSlots, W = DP / kGroups, H = 128 / kGroups;
+  using L = FwdCfg<DP>;
+  constexpr int NS = L::kSlots, G = kGroups, W = DP / G, H = 128 / G, NB = L::kBuffers;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t shift = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + shift;
-  if (shift + L::kTotal - 1024 + L::kExchange > L::kForward) {      // (an aligned base, as every launch has had, always fits)
+  if (shift + L::kNeed > L::kTotal) {      // (an aligned base, as every launch has had, always fits)
     if (threadIdx.x == 0) atomicOr(p.err, ERRBIT_BOUNDS);
     return;
   }
@@ -399,7 +421,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
   int* ints = (int*)(b_o + 1);
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
-  float* xchg = (float*)(ints + 4);                           // [kBuffers tiles][groups][128]
+  float* xchg = (float*)(ints + 4);                           // [NB tiles][groups][128]
 
   const int warp = threadIdx.x >> 5;
   const int h = blockIdx.x % p.hq, hk = h / (p.hq / p.hk), qt = p.tiles - 1 - (int)(blockIdx.x / p.hq);      // long tiles first
@@ -410,7 +432,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(tmem_slot);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   const int first = threadIdx.x < 128 && qt * 128 + (int)threadIdx.x < p.T ? p.begin[qt * 128 + threadIdx.x] : p.T;
   int b_min, b_max;
   range_of(first, &b_min, &b_max, ints);
@@ -418,7 +440,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t t_s = tmem, t_p = tmem + 256, t_o = tmem + 384;
+  const uint32_t t_s = tmem, t_p = tmem + 256, t_o = tmem + 384, o_step = (NB - 1) * DP;      // (from one accumulator to the next)
   const int kb0 = b_min < p.T ? b_min / 128 : qt + 1, n = qt + 1 - kb0;      // key tiles (none: no row of the tile has a segment)
 
   if (warp == 0) {
@@ -462,12 +484,12 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       for (int j = 0; j < n && ok; ++j) {
         ok = warp_wait(b_p, j & 1, abort_flag) && next();
         if (!ok) break;
-        kept_by_cols<128, DP, false>(leader, t_o, t_p, r0 + slot * L::kPlane, 0);
+        kept_by_cols<128, DP, false>(leader, t_o + (j & 1) * o_step, t_p, r0 + slot * L::kPlane, 0);
         release();
         ok = next();
         if (!ok) break;
-        kept_by_cols<128, DP, true>(leader, t_o, t_p, r0 + slot * L::kPlane, 1);
-        kept_by_cols<128, DP, false>(leader, t_o, t_p, r0 + slot * L::kPlane, 1);
+        kept_by_cols<128, DP, true>(leader, t_o + (j & 1) * o_step, t_p, r0 + slot * L::kPlane, 1);
+        kept_by_cols<128, DP, false>(leader, t_o + (j & 1) * o_step, t_p, r0 + slot * L::kPlane, 1);
         release();
         commit_by(leader, b_o);
         if (j + 2 < n) ok = scores(j + 2);      // (this tile's scores have been read: P says so)
@@ -488,13 +510,14 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       const int kb = kb0 + j, c0 = kb * 128 + at.group * H;
       const float sc = fmaxf(sc0 * fabsf(k_inv), 1e-37f);      // (masked scores are -infinity times this)
       const bool bad = k_inv < 0.0f || v_inv < 0.0f;
+      const bool crossed = kb == qt || kb * 128 < b_max;       // by the diagonal or the begin of a segment
       const float v_this = fabsf(v_inv);
       if (j + 1 < n) { k_inv = p.k.inv[kvt + kb + 1]; v_inv = p.v.inv[kvt + kb + 1]; }
       ok = mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag) && ok;
       tc_fence_after();
       float v[H];
       load_cols<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
-      if (kb == qt || kb * 128 < b_max) keep_columns<H>(v, begin - c0, t - c0, -INFINITY);      // the diagonal or the begin of a segment crosses the tile
+      if (crossed) keep_columns<H>(v, begin - c0, t - c0, -INFINITY);
       if (bad) {                                // a visible key or value that is not finite
         const uint32_t bits = p.k.bad[(kvt + kb) * 4 + at.group] | p.v.bad[(kvt + kb) * 4 + at.group];
         for (int i = 0; i < H; ++i) if (((bits >> i) & 1) && c0 + i >= begin && c0 + i <= t) l = __int_as_float(0x7fffffff);
@@ -502,35 +525,32 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
 #pragma unroll
       for (int i = 4; i < H; i += 4) { m0 = fmaxf(m0, fmaxf(v[i], v[i + 1])); m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3])); }
-      float* x = xchg + (j & (L::kBuffers - 1)) * kGroups * 128 + at.row;
-      if (L::kBuffers == 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
+      float* x = xchg + (j & (NB - 1)) * G * 128 + at.row;
+      if (NB == 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
       x[at.group * 128] = fmaxf(m0, m1);
       asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");      // the four quarters of these rows
       const float mn = fmaxf(m, fmaxf(fmaxf(x[0], x[128]), fmaxf(x[256], x[384])) * sc), ref = mn > -INFINITY ? mn : 0.0f;
       const float shrink = m > -INFINITY ? exp2_fast(m - ref) : 0.0f;
-      weights_of_row<H>(v, sc, 14.0f - ref);
-      float2 s0 = make_float2(v[0], v[1]), s1 = make_float2(v[2], v[3]);
-#pragma unroll
-      for (int i = 4; i < H; i += 4) { s0 = add2(s0, make_float2(v[i], v[i + 1])); s1 = add2(s1, make_float2(v[i + 2], v[i + 3])); }
-      s0 = add2(s0, s1);
-      l = l * shrink + (s0.x + s0.y);
+      uint32_t r[H];
+      l = l * shrink + split_weights<H>(v, sc, 14.0f - ref, r);
       m = mn;
       if (j > 0) {                              // the last tile's product has read P and is in its accumulator
         ok = mbar_wait(b_o, (j - 1) & 1, abort_flag) && ok;
         tc_fence_after();
       }
-      store_operand<H>(t_p + at.group * H + at.lane_off, v);
-      if (j > 0) add_part<W>(t_o + at.group * W + at.lane_off, acc, keep, v_last);
+      tmem_st32(t_p + at.group * H + at.lane_off, r);
+      if (j > 0 && NB == 1) add_part<W>(t_o + at.group * W + at.lane_off, acc, keep, v_last);
       operand_written(b_p, at.lane);
+      if (j > 0 && NB == 2) add_part<W>(t_o + ((j - 1) & 1) * o_step + at.group * W + at.lane_off, acc, keep, v_last);
       keep = shrink; v_last = v_this;
     }
     if (n > 0) {
       ok = mbar_wait(b_o, (n - 1) & 1, abort_flag) && ok;
       tc_fence_after();
-      add_part<W>(t_o + at.group * W + at.lane_off, acc, keep, v_last);
+      add_part<W>(t_o + ((n - 1) & 1) * o_step + at.group * W + at.lane_off, acc, keep, v_last);
     }
-    float* x = xchg + (n & (L::kBuffers - 1)) * kGroups * 128 + at.row;
-    if (L::kBuffers == 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
+    float* x = xchg + (n & (NB - 1)) * G * 128 + at.row;
+    if (NB == 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
     x[at.group * 128] = l;
     asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
     l = (x[0] + x[128]) + (x[256] + x[384]);
@@ -543,7 +563,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) { tc_fence_after(); tmem_free(tmem); }
+  if (warp == 1) { tc_fence_after(); tmem_free(tmem, 512); }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, ERRBIT_WAIT_TIMEOUT);
 }
 
@@ -574,7 +594,7 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(tmem_slot);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   const int last = threadIdx.x < 128 && kt * 128 + (int)threadIdx.x < p.T ? p.end[kt * 128 + threadIdx.x] : 0;
   int e_min, e_max;
   range_of(last, &e_min, &e_max, ints);
@@ -676,7 +696,7 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) { tc_fence_after(); tmem_free(tmem); }
+  if (warp == 1) { tc_fence_after(); tmem_free(tmem, 512); }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, ERRBIT_WAIT_TIMEOUT);
 }
 
@@ -717,7 +737,7 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     *vmax_slot = 0.0f;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) tmem_alloc(tmem_slot);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   const int tx = xt * 128 + (int)threadIdx.x;
   const int edge = DK ? (threadIdx.x < 128 && tx < p.T ? p.end[tx] : 0) : (threadIdx.x < 128 && tx < p.T ? p.begin[tx] : p.T);
   int e_min, e_max;
@@ -895,7 +915,7 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) { tc_fence_after(); tmem_free(tmem); }
+  if (warp == 1) { tc_fence_after(); tmem_free(tmem, 512); }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, ERRBIT_WAIT_TIMEOUT);
 }
 template <int DP>
@@ -993,11 +1013,11 @@ int allow_smem(K kernel, int bytes) {
 
 template <int DP>
 int forward(Work& w) {
-  static const int ready = allow_smem(k_forward<DP>, StreamSmem<DP>::kForward);
+  static const int ready = allow_smem(k_forward<DP>, FwdCfg<DP>::kTotal);
   VB_TRY(ready);
   CUtensorMap mq, mk, mv;
   VB_TRY(make_map(&mq, w.prep.in[0], w.p.T, DP, 128)); VB_TRY(make_map(&mk, w.prep.in[1], w.p.T, DP, 128)); VB_TRY(make_map(&mv, w.prep.in[2], w.p.T, DP, 128));
-  k_forward<DP><<<(unsigned)w.p.hq * w.p.tiles, kThreads, StreamSmem<DP>::kForward, ctx().stream>>>(mq, mk, mv, w.p);
+  k_forward<DP><<<(unsigned)w.p.hq * w.p.tiles, kThreads, FwdCfg<DP>::kTotal, ctx().stream>>>(mq, mk, mv, w.p);
   VB_LAUNCH_CHECK();
   return VB_OK;
 }
