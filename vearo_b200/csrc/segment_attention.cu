@@ -40,33 +40,67 @@ struct PlanesDev { const float* x; i64 st, sh; __half* planes; float* inv; float
 struct PrepareDev {
   PlanesDev in[4];
   int n, T, tiles, dk, hq;
-  const float* starts; int n_seg; int* begin; int* end; int* err;      // where the segment of each row begins and ends (begin null: not wanted)
+  const float* starts; int n_seg; int* begin; int* end; int4* ranges; int* order; int* err;      // where the segment of each row begins and ends, and the ranges of a tile's rows
   const float* o; i64 o_st, o_sh; bool o_vec; const float* lse;                     // for do: delta and the lse in base 2, padded to whole tiles
   float* delta; float* lse2;
 };
 
-// Where the segment of row t begins and ends (rows of no segment: an empty range).  Offsets that decrease or leave [0, T] are
-// reported; whatever they are, every range stays inside [0, T].
-__device__ __forceinline__ void find_segment(const PrepareDev& p, int t) {
-  for (int i = t; i <= p.n_seg; i += p.tiles * 128) {
-    const float s = p.starts[i];
-    if (!(s > -0.5f)) atomicOr(p.err, ERRBIT_NEG_ID);
-    else if (!(s < (float)p.T + 0.5f) || (i > 0 && !(p.starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
-  }
-  if (t >= p.T) return;
+// The offset of the segment that row t is in (-1: none), as an index into the offsets.
+__device__ __forceinline__ int segment_of(const PrepareDev& p, int t) {
   int lo = 0, hi = p.n_seg + 1;          // offsets [0, lo) are <= t
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (roundf(p.starts[mid]) <= (float)t) lo = mid + 1; else hi = mid;
   }
+  return lo > 0 && lo <= p.n_seg ? lo - 1 : -1;
+}
+// Where the segment of row t begins and ends (rows of no segment: an empty range).  Offsets that decrease or leave [0, T] are
+// reported; whatever they are, every range stays inside [0, T].
+__device__ __forceinline__ int2 find_segment(const PrepareDev& p, int t) {
+  for (int i = t; i <= p.n_seg; i += p.tiles * 128) {
+    const float s = p.starts[i];
+    if (!(s > -0.5f)) atomicOr(p.err, ERRBIT_NEG_ID);
+    else if (!(s < (float)p.T + 0.5f) || (i > 0 && !(p.starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
+  }
+  if (t >= p.T) return make_int2(p.T, 0);
   int b = p.T, e = 0;
-  if (lo > 0 && lo <= p.n_seg) {
-    const float fb = roundf(p.starts[lo - 1]), fe = roundf(p.starts[lo]);
+  const int s = segment_of(p, t);
+  if (s >= 0) {
+    const float fb = roundf(p.starts[s]), fe = roundf(p.starts[s + 1]);
     b = fb > 0.0f ? (int)fb : 0;
     e = fe < (float)p.T ? (int)fe : p.T;
     if (!(b <= t && t < e)) { b = p.T; e = 0; }
   }
   p.begin[t] = b; p.end[t] = e;
+  return make_int2(b, e);
+}
+
+// Tiles in the order of the work that their rows have ahead of them (which = 0: as queries, how far back their segment begins; 1: as keys,
+// how far on it ends), the most first: a sort by count into 1024 classes.
+__device__ void plan_order(const PrepareDev& p, int which, int* classes) {
+  int* order = p.order + which * p.tiles;
+  for (int i = threadIdx.x; i < 1024; i += 256) classes[i] = 0;
+  __syncthreads();
+  auto class_of = [&](int tile) -> int {
+    const int t = which == 0 ? tile * 128 : min(p.T - 1, tile * 128 + 127), s = segment_of(p, t);
+    int n = 0;
+    if (s >= 0) n = which == 0 ? tile - (int)fmaxf(roundf(p.starts[s]), 0.0f) / 128 : ((int)fminf(roundf(p.starts[s + 1]), (float)p.T) - 1) / 128 - tile;
+    return 1023 - max(0, min(n, 1023));
+  };
+  for (int i = threadIdx.x; i < p.tiles; i += 256) atomicAdd(&classes[class_of(i)], 1);
+  __syncthreads();
+  if (threadIdx.x < 32) {                // counts into places: 32 classes a lane
+    int sum = 0;
+    for (int i = 0; i < 32; ++i) { const int c = classes[threadIdx.x * 32 + i]; classes[threadIdx.x * 32 + i] = sum; sum += c; }
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if ((int)threadIdx.x >= o) before += x; }
+    before -= sum;
+    for (int i = 0; i < 32; ++i) classes[threadIdx.x * 32 + i] += before;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.tiles; i += 256) order[atomicAdd(&classes[class_of(i)], 1)] = i;
+  __syncthreads();
 }
 
 template <int DP>
@@ -74,13 +108,30 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
   constexpr int kLanes = DP / 4, kRows = 256 / kLanes, kPasses = 128 / kRows;      // lanes of a row, rows of a pass
   __shared__ float red[8];
   __shared__ uint32_t bad[4];
+  __shared__ int4 range[4];
+  __shared__ int classes[1024];
   const int tile = blockIdx.x;
+  if (tile == p.tiles) {                 // one CTA more than there are tiles plans their order
+    if (blockIdx.y == 0) { plan_order(p, 0, classes); if (p.delta) plan_order(p, 1, classes); }
+    return;
+  }
   int h = blockIdx.y, which = 0;
   while (h >= p.in[which].heads) h -= p.in[which++].heads;
   const PlanesDev& x = p.in[which];
-  if (p.begin && blockIdx.y == 0 && threadIdx.x < 128) find_segment(p, tile * 128 + threadIdx.x);
   if (threadIdx.x < 4) bad[threadIdx.x] = 0;
-  __syncthreads();
+  if (blockIdx.y == 0) {                 // the rows' segments and the range of their ends
+    if (threadIdx.x < 128) {
+      const int2 s = find_segment(p, tile * 128 + threadIdx.x);
+      const int4 r = make_int4(__reduce_min_sync(0xffffffffu, s.x), __reduce_max_sync(0xffffffffu, s.x), __reduce_min_sync(0xffffffffu, s.y), __reduce_max_sync(0xffffffffu, s.y));
+      if ((threadIdx.x & 31) == 0) range[threadIdx.x >> 5] = r;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      int4 r = range[0];
+      for (int i = 1; i < 4; ++i) { r.x = min(r.x, range[i].x); r.y = max(r.y, range[i].y); r.z = min(r.z, range[i].z); r.w = max(r.w, range[i].w); }
+      p.ranges[tile] = r;
+    }
+  } else __syncthreads();
   const int c = (threadIdx.x % kLanes) * 4, r0 = threadIdx.x / kLanes;
   float4 v[kPasses];
   const bool mine = c < p.dk;
@@ -277,16 +328,25 @@ __device__ __forceinline__ void add_part(uint32_t taddr, float (&acc)[W], float 
     acc[j] = a.x; acc[j + 1] = a.y;
   }
 }
-// this thread's quarter of a row of the result, components [c0, c0 + W) of dk
+// This warp's 32 rows x W components of the result, through its own part of a tile buffer that no product reads any more: a thread holds
+// a row, but a store that takes 16 bytes of each of 32 rows costs an instruction's time for every one of them (4000 cycles a
+// tile; so 600).  out: row 0 of the warp's rows, component 0 of the head; c0: the warp's first component; live: rows that exist.
 template <int W>
-__device__ __forceinline__ void store_row(float* row, const float (&acc)[W], int c0, int dk, float f) {
-  if ((dk & 3) == 0) {
+__device__ __forceinline__ void store_rows(float4* stage, const float (&acc)[W], float f, float* out, i64 stride, int live, int c0, int dk, int lane) {
+  constexpr int C = W / 4, R = 32 / C;            // 16-byte pieces of a row, rows of one store
+  constexpr int kShift = W == 16 ? 1 : 0;
 #pragma unroll
-    for (int i = 0; i < W; i += 4)
-      if (c0 + i < dk) *reinterpret_cast<float4*>(row + c0 + i) = make_float4(acc[i] * f, acc[i + 1] * f, acc[i + 2] * f, acc[i + 3] * f);
-  } else {
+  for (int c = 0; c < C; ++c) stage[lane * C + (c ^ ((lane >> kShift) & (C - 1)))] = make_float4(acc[4 * c] * f, acc[4 * c + 1] * f, acc[4 * c + 2] * f, acc[4 * c + 3] * f);
+  __syncwarp();
+  const int c = lane % C, at = c0 + 4 * c;
 #pragma unroll
-    for (int i = 0; i < W; ++i) if (c0 + i < dk) row[c0 + i] = acc[i] * f;
+  for (int i = 0; i < 32 / R; ++i) {
+    const int r = i * R + lane / C;
+    const float4 v = stage[r * C + (c ^ ((r >> kShift) & (C - 1)))];
+    if (r >= live || at >= dk) continue;
+    float* o = out + r * stride + at;
+    if ((dk & 3) == 0) *reinterpret_cast<float4*>(o) = v;
+    else { o[0] = v.x; if (at + 1 < dk) o[1] = v.y; if (at + 2 < dk) o[2] = v.z; if (at + 3 < dk) o[3] = v.w; }
   }
 }
 // p 2^14 of a quarter of a row: 2^(score - lse + 14), one lse a row or one a column
@@ -330,6 +390,9 @@ __device__ __forceinline__ void keep_columns(float (&v)[W], int first, int last,
 #pragma unroll
   for (int i = 0; i < W; ++i) if (i < first || i > last) v[i] = other;
 }
+// The kernels are launched while k_prepare still runs (programmatic dependent launch): they set up, then wait for what it writes.
+__device__ __forceinline__ void wait_for_prepare() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -344,17 +407,6 @@ __device__ __forceinline__ void let_land(uint64_t* bars, int n) {
     for (uint32_t k = 0; k < (1u << 14) && !done; ++k)
       asm volatile("{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(done) : "r"(addr), "r"(0u) : "memory");
   }
-}
-// smallest and largest of an int over the first 128 threads, for all of the CTA
-__device__ __forceinline__ void range_of(int v, int* lo, int* hi, int* sm) {
-  if (threadIdx.x == 0) { sm[0] = 0x7fffffff; sm[1] = -1; }
-  __syncthreads();
-  if (threadIdx.x < 128) {
-    const int a = __reduce_min_sync(0xffffffffu, v), b = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) { atomicMin(&sm[0], a); atomicMax(&sm[1], b); }
-  }
-  __syncthreads();
-  *lo = sm[0]; *hi = sm[1];
 }
 // a row warp has written its operand (and read the last accumulator)
 __device__ __forceinline__ void operand_written(uint64_t* bar, int lane) {
@@ -378,6 +430,8 @@ struct AttnParams {
   int T, tiles, hq, hk, dk;
   float scale;
   const int* begin; const int* end;
+  const int* order;                           // [2][tiles] tiles by the work they have as queries, and as keys, the most first
+  const int4* ranges;                         // [tiles] smallest and largest begin, smallest and largest end of the tile's rows
   Side q, k, v, g;
   const float* lse2; const float* delta;      // [hq][tiles * 128]
   float* out; float* lse;                     // forward
@@ -424,7 +478,8 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
   float* xchg = (float*)(ints + 4);                           // [NB tiles][groups][128]
 
   const int warp = threadIdx.x >> 5;
-  const int h = blockIdx.x % p.hq, hk = h / (p.hq / p.hk), qt = p.tiles - 1 - (int)(blockIdx.x / p.hq);      // long tiles first
+  const int h = blockIdx.x % p.hq, hk = h / (p.hq / p.hk);
+  if (warp == 0) { prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); }
   if (threadIdx.x == 0) {
     mbar_init(b_x, 1);
     for (int i = 0; i < NS; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_free[i], 1); }
@@ -433,9 +488,10 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
-  const int first = threadIdx.x < 128 && qt * 128 + (int)threadIdx.x < p.T ? p.begin[qt * 128 + threadIdx.x] : p.T;
-  int b_min, b_max;
-  range_of(first, &b_min, &b_max, ints);
+  wait_for_prepare();
+  const int qt = p.order[blockIdx.x / p.hq];
+  const int4 range = p.ranges[qt];
+  const int b_min = range.x, b_max = range.y;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -554,11 +610,13 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     x[at.group * 128] = l;
     asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
     l = (x[0] + x[128]) + (x[256] + x[384]);
-    if (ok && t < p.T) {
-      if (q_inv < 0.0f && begin <= t && ((p.q.bad[((i64)h * p.tiles + qt) * 4 + at.quarter] >> at.lane) & 1)) l = __int_as_float(0x7fffffff);
-      const bool dead = l == 0.0f;
-      store_row<W>(p.out + ((i64)t * p.hq + h) * p.dk, acc, at.group * W, p.dk, dead ? 0.0f : 1.0f / l);
-      if (at.group == 0 && p.lse) p.lse[(i64)h * p.T + t] = dead ? -INFINITY : (m - 14.0f) * kLn2 + logf(l);
+    if (q_inv < 0.0f && begin <= t && ((p.q.bad[((i64)h * p.tiles + qt) * 4 + at.quarter] >> at.lane) & 1)) l = __int_as_float(0x7fffffff);
+    const bool dead = l == 0.0f;
+    const int row0 = qt * 128 + at.quarter * 32;
+    if (ok) {
+      store_rows<W>((float4*)sq + (at.quarter * G + at.group) * 8 * W, acc, dead ? 0.0f : 1.0f / l, p.out + ((i64)row0 * p.hq + h) * p.dk, (i64)p.hq * p.dk, p.T - row0,
+                    at.group * W, p.dk, at.lane);
+      if (t < p.T && at.group == 0 && p.lse) p.lse[(i64)h * p.T + t] = dead ? -INFINITY : (m - 14.0f) * kLn2 + logf(l);
     }
   }
   tc_fence_before();
@@ -586,7 +644,7 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
   volatile int* abort_flag = ints + 3;
 
   const int warp = threadIdx.x >> 5;
-  const int part = block % p.parts, hk = block / p.parts % p.hk, kt = block / p.parts / p.hk, heads = p.hq / p.hk / p.parts, h0 = (hk * p.parts + part) * heads;
+  const int part = block % p.parts, hk = block / p.parts % p.hk, heads = p.hq / p.hk / p.parts, h0 = (hk * p.parts + part) * heads;
   if (threadIdx.x == 0) {
     mbar_init(b_x, 1);
     for (int i = 0; i < NS; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_free[i], 1); }
@@ -595,9 +653,10 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
-  const int last = threadIdx.x < 128 && kt * 128 + (int)threadIdx.x < p.T ? p.end[kt * 128 + threadIdx.x] : 0;
-  int e_min, e_max;
-  range_of(last, &e_min, &e_max, ints);
+  wait_for_prepare();
+  const int kt = p.order[p.tiles + block / p.parts / p.hk];
+  const int4 range = p.ranges[kt];
+  const int e_min = range.z, e_max = range.w;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -692,7 +751,10 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
         add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
       }
     }
-    if (ok && t < p.T) store_row<W>(p.dv + (((i64)part * p.T + t) * p.hk + hk) * p.dk, acc, at.group * W, p.dk, 1.0f / 16384.0f);
+    const int row0 = kt * 128 + at.quarter * 32;
+    if (ok)
+      store_rows<W>((float4*)sk + (at.quarter * kGroups + at.group) * 8 * W, acc, 1.0f / 16384.0f, p.dv + (((i64)part * p.T + row0) * p.hk + hk) * p.dk,
+                    (i64)p.hk * p.dk, p.T - row0, at.group * W, p.dk, at.lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -727,7 +789,6 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
   const int warp = threadIdx.x >> 5;
   const int part = DK ? block % p.parts : 0, rest = DK ? block / p.parts : block, x_heads = DK ? p.hk : p.hq;
   const int hx = rest % x_heads, hk = DK ? hx : hx / (p.hq / p.hk), heads = DK ? p.hq / p.hk / p.parts : 1, h0 = DK ? (hk * p.parts + part) * heads : hx;
-  const int xt = DK ? rest / x_heads : p.tiles - 1 - rest / x_heads;
   if (threadIdx.x == 0) {
     mbar_init(b_x, 1); mbar_init(b_x2, kRowWarps); mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1);
     for (int i = 0; i < N1; ++i) { mbar_init(&b_y1full[i], 1); mbar_init(&b_y1free[i], 1); }
@@ -738,10 +799,11 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
-  const int tx = xt * 128 + (int)threadIdx.x;
-  const int edge = DK ? (threadIdx.x < 128 && tx < p.T ? p.end[tx] : 0) : (threadIdx.x < 128 && tx < p.T ? p.begin[tx] : p.T);
-  int e_min, e_max;
-  range_of(edge, &e_min, &e_max, ints);
+  wait_for_prepare();
+  const int xt = p.order[(DK ? p.tiles : 0) + rest / x_heads];
+  const int4 range = p.ranges[xt];
+  const int e_min = DK ? range.z : range.x, e_max = DK ? range.w : range.y;
+  __syncthreads();                 // (vmax_slot is 0)
   {   // longest value row of the head: the scale of dS has to hold |do| |v| twice
     float m = 0.0f;
     for (int i = threadIdx.x; i < p.tiles; i += kThreads) m = fmaxf(m, p.v.len[(i64)hk * p.tiles + i]);
@@ -908,10 +970,11 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
         add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
       }
     }
-    if (ok && t < p.T) {
-      float* row = DK ? p.dk_ + (((i64)part * p.T + t) * p.hk + hk) * p.dk : p.dq + ((i64)t * p.hq + hx) * p.dk;
-      store_row<W>(row, acc, at.group * W, p.dk, p.scale);
-    }
+    const int row0 = xt * 128 + at.quarter * 32;
+    if (ok)
+      store_rows<W>((float4*)x1 + (at.quarter * kGroups + at.group) * 8 * W, acc, p.scale,
+                    DK ? p.dk_ + (((i64)part * p.T + row0) * p.hk + hk) * p.dk : p.dq + ((i64)row0 * p.hq + hx) * p.dk, (i64)x_heads * p.dk, p.T - row0, at.group * W,
+                    p.dk, at.lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -979,7 +1042,7 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
     planes[i] = take((size_t)2 * heads[i] * s.T * dp * 2);
     inv[i] = take((size_t)heads[i] * tiles * 4); len[i] = take((size_t)heads[i] * tiles * 4); bad[i] = take((size_t)heads[i] * tiles * 16);
   }
-  const size_t begin = take((size_t)s.T * 4), end = take((size_t)s.T * 4);
+  const size_t begin = take((size_t)s.T * 4), end = take((size_t)s.T * 4), ranges = take((size_t)tiles * sizeof(int4)), order = take((size_t)tiles * 8);
   const size_t delta = o ? take((size_t)s.hq * tiles * 512) : 0, lse2 = o ? take((size_t)s.hq * tiles * 512) : 0;
   VB_TRY(scratch_alloc(at, &w.hold.p));
   uint8_t* base = (uint8_t*)w.hold.p;
@@ -993,15 +1056,27 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
     *sides[i] = Side{d.in[i].planes, d.in[i].inv, d.in[i].len, d.in[i].bad};
     all += heads[i];
   }
-  d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.err = ctx().d_err;
+  d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.ranges = (int4*)(base + ranges); d.order = (int*)(base + order); d.err = ctx().d_err;
   if (o) { d.o = o->p; d.o_st = o->st; d.o_sh = o->sh; d.lse = lse;
            d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lse2 = (float*)(base + lse2); }
   AttnParams& p = w.p;
   p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.scale = s.scale;
-  p.begin = d.begin; p.end = d.end; p.lse2 = d.lse2; p.delta = d.delta; p.err = ctx().d_err;
+  p.begin = d.begin; p.end = d.end; p.ranges = d.ranges; p.order = d.order; p.lse2 = d.lse2; p.delta = d.delta; p.err = ctx().d_err;
   ProfScope prof("segment_attn_prepare", 8.0 * (double)s.T * all * s.dk);
-  if (dp == 64) k_prepare<64><<<dim3(tiles, all), 256, 0, ctx().stream>>>(d);
-  else k_prepare<128><<<dim3(tiles, all), 256, 0, ctx().stream>>>(d);
+  if (dp == 64) k_prepare<64><<<dim3(tiles + 1, all), 256, 0, ctx().stream>>>(d);
+  else k_prepare<128><<<dim3(tiles + 1, all), 256, 0, ctx().stream>>>(d);
+  VB_LAUNCH_CHECK();
+  return VB_OK;
+}
+// a kernel that may start while the one ahead of it in the stream still runs
+template <class... P, class... A>
+int launch_early(void (*kernel)(P...), unsigned ctas, int smem, A... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(ctas); c.blockDim = dim3(kThreads); c.dynamicSmemBytes = (size_t)smem; c.stream = ctx().stream; c.attrs = &at; c.numAttrs = 1;
+  VB_CUDA(cudaLaunchKernelEx(&c, kernel, args...));
   VB_LAUNCH_CHECK();
   return VB_OK;
 }
@@ -1017,9 +1092,7 @@ int forward(Work& w) {
   VB_TRY(ready);
   CUtensorMap mq, mk, mv;
   VB_TRY(make_map(&mq, w.prep.in[0], w.p.T, DP, 128)); VB_TRY(make_map(&mk, w.prep.in[1], w.p.T, DP, 128)); VB_TRY(make_map(&mv, w.prep.in[2], w.p.T, DP, 128));
-  k_forward<DP><<<(unsigned)w.p.hq * w.p.tiles, kThreads, FwdCfg<DP>::kTotal, ctx().stream>>>(mq, mk, mv, w.p);
-  VB_LAUNCH_CHECK();
-  return VB_OK;
+  return launch_early(k_forward<DP>, (unsigned)w.p.hq * w.p.tiles, FwdCfg<DP>::kTotal, mq, mk, mv, w.p);
 }
 template <int DP>
 int backward(Work& w, float* dq, float* dk, float* dv) {
@@ -1043,8 +1116,7 @@ int backward(Work& w, float* dq, float* dk, float* dv) {
     VB_TRY(scratch_alloc((size_t)(2 * p.parts * n) * sizeof(float), &hold.p));
     p.dk_ = (float*)hold.p; p.dv = p.dk_ + p.parts * n;
   }
-  k_backward<DP><<<(unsigned)(p.tiles * (2 * p.hk * p.parts + p.hq)), kThreads, kSmem, ctx().stream>>>(m, p);
-  VB_LAUNCH_CHECK();
+  VB_TRY(launch_early(k_backward<DP>, (unsigned)(p.tiles * (2 * p.hk * p.parts + p.hq)), kSmem, m, p));
   if (p.parts > 1) {
     const i64 ctas = (2 * n + 1023) / 1024, cap = (i64)ctx().sm_count * 8;
     k_add_parts<<<(unsigned)(ctas < cap ? ctas : cap), 256, 0, ctx().stream>>>(p.dk_, p.dv, dk, dv, n, p.parts);
