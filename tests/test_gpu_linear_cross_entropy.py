@@ -129,6 +129,30 @@ def test_nan_and_infinity_stay_in_their_rows(vb):
     assert not np.isfinite(gx[[3, 131]]).all() and np.isfinite(np.delete(gx, [3, 131], 0)).all()
 
 
+def test_rows_of_unequal_size(vb):
+    """Neighbouring rows of x that differ by 2^60: each has an exponent of its own in the logits and in its gradient."""
+    x, w, t = rnd(43, 130, 96), rnd(44, 150, 96, scale=0.2), np.arange(130, dtype=np.float32)
+    x[::3] *= 2.0 ** -60
+    (lse, loss, gx, _), (e_lse, e_loss, egx, _) = truth(x, w, t, -100)
+    D = [Dev(vb, a) for a in (x, w, t)]
+    got, got_lse = outputs(vb, vb.lib().vb_linear_cross_entropy, *D, -100, n=2)
+    a, _ = outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *D, -100, Dev(vb, got_lse), Dev(vb, np.ones(1, np.float32)), n=2)
+    assert (np.abs(got_lse - lse) <= e_lse).all() and abs(got[0] - loss) <= e_loss and (np.abs(a - gx) <= egx).all()
+
+
+def test_rows_left_out_may_hold_anything(vb):
+    x, w = rnd(40, 150, 64), rnd(41, 200, 64)
+    t = np.random.default_rng(42).integers(0, 200, 150).astype(np.float32)
+    t[[5, 60, 149]] = -100
+    (_, loss, gx, gw), (_, e_loss, egx, egw) = truth(x, w, t, -100)
+    x[5], x[60], x[149] = np.nan, np.inf, 1e30
+    D = [Dev(vb, a) for a in (x, w, t)]
+    got, lse = outputs(vb, vb.lib().vb_linear_cross_entropy, *D, -100, n=2)
+    a, b = outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *D, -100, Dev(vb, lse), Dev(vb, np.ones(1, np.float32)), n=2)
+    assert abs(got[0] - loss) <= e_loss and (np.abs(b - gw) <= egw).all()
+    assert (a[[5, 60, 149]] == 0).all() and (np.abs(a - gx) <= egx).all()
+
+
 def test_views_leading_dims_and_one_gradient(vb):
     x, w = rnd(12, 2, 15, 40), rnd(13, 90, 40)
     t = np.random.default_rng(14).integers(0, 90, (2, 15)).astype(np.float32)

@@ -2,8 +2,9 @@
 //
 //   out[m, n] = sum over 128-wide runs of k of 2^-(eA + eB) (lo hi' + hi lo' + hi hi')[run]
 //
-// Persistent, one CTA per SM, 320 threads: warp 0 fetches operand tiles by TMA (no multicast), warp 1 issues the MMAs from one
-// thread, warps 2-9 add the finished runs to registers (thread = one row x 128 of the tile's 256 columns) and store the tile.  Stage
+// Persistent, one CTA per SM, 320 threads: warp 0 takes tiles from a counter and fetches their operands by TMA (no multicast), warp 1
+// issues the MMAs, warps 2-9 add the finished runs to registers (thread = one row x 128 of the tile's 256 columns) and store the
+// tile, 32 x 32 blocks at a time, by TMA.  Stage
 // = 64 k values of a 128 x 256 tile, both planes: 96 KB, two stages.  A run of k is one accumulator of 256 tensor-memory columns, two of them
 // in flight, so the adding warps work on one while the next is formed; a tile's epilogue hides under the next tile's first
 // runs the same way.  Both operands may lie K-major or MN-major in memory: half precision takes either through the same
@@ -15,52 +16,62 @@ namespace vb {
 namespace {
 using namespace tc;
 
-constexpr int kThreads = 320, kBM = 128, kBN = 256, kBK = 64, kStages = 2;
+constexpr int kThreads = 320, kBM = 128, kBN = 256, kBK = 64, kStages = 2, kEpiWarps = 8;
 constexpr int kAPlane = kBM * kBK * 2, kBPlane = kBN * kBK * 2;               // 16 KB, 32 KB
 constexpr int kStage = 2 * kAPlane + 2 * kBPlane;
-constexpr int kPitch = 33;                                                    // words of a staged row of 32
-constexpr int kStaging = 32 * kPitch * 4;
-constexpr int kSmem = 1024 + kStages * kStage + 8 * kStaging + 128;
+constexpr int kStaging = 4096;                                                // a warp's 32 x 32 block: f32, or both planes of halves
+constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kStaging + 256;
 constexpr float kGradScale = 16384.0f;
 
 // ---- splitting ------------------------------------------------------------------------------------------------------------------
-struct SplitDev { const float* x; __half* planes; float* inv; i64 rows, cols, ld, plane; int cb, blocks; bool vec; };
-__global__ void __launch_bounds__(256) k_split16(SplitDev j0, SplitDev j1) {
+struct SplitDev { const float* x; const int* keep; __half* planes; float* inv; i64 rows, cols, ld, plane, inv_ld; int cb, blocks; bool vec, by_row; };
+struct SplitJobs { SplitDev job[3]; };
+__global__ void __launch_bounds__(256) k_split16(const __grid_constant__ SplitJobs jobs) {
   __shared__ float red[8];
-  const bool second = (int)blockIdx.x >= j0.blocks;
-  const SplitDev& j = second ? j1 : j0;
-  const int blk = second ? (int)blockIdx.x - j0.blocks : (int)blockIdx.x;
+  int blk = blockIdx.x, which = 0;
+  while (blk >= jobs.job[which].blocks) blk -= jobs.job[which++].blocks;
+  const SplitDev& j = jobs.job[which];
   const int rb = blk / j.cb, cbi = blk - rb * j.cb;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const i64 c0 = (i64)cbi * 128 + lane * 4;
   float4 v[16];
-  float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
+  for (int i = 0; i < 16; ++i) {      // (a warp has whole rows of the block)
     const i64 r = (i64)rb * 128 + i * 8 + wid;
     v[i] = make_float4(0, 0, 0, 0);
-    if (r < j.rows && c0 < j.cols) {
+    if (r < j.rows && c0 < j.cols && (!j.keep || j.keep[r] != kNoTarget)) {
       const float* p = j.x + r * j.cols + c0;
       if (j.vec) v[i] = *reinterpret_cast<const float4*>(p);
       else { v[i].x = p[0]; if (c0 + 1 < j.cols) v[i].y = p[1]; if (c0 + 2 < j.cols) v[i].z = p[2]; if (c0 + 3 < j.cols) v[i].w = p[3]; }
     }
-    m = fmaxf(m, fmaxf(fmaxf(finite_abs(v[i].x), finite_abs(v[i].y)), fmaxf(finite_abs(v[i].z), finite_abs(v[i].w))));
   }
+  float m = 0.0f, s = 1.0f;
+  if (!j.by_row) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[wid] = m;
-  __syncthreads();
-  m = red[0];
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, fmaxf(fmaxf(finite_abs(v[i].x), finite_abs(v[i].y)), fmaxf(finite_abs(v[i].z), finite_abs(v[i].w))));
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
-  float inv;
-  const float s = block_scale(m, &inv);
-  if (threadIdx.x == 0) j.inv[blk] = inv;
-  if (c0 >= j.ld) return;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) red[wid] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
+    float inv;
+    s = block_scale(m, &inv);
+    if (threadIdx.x == 0) j.inv[rb * j.inv_ld + cbi] = inv;
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const i64 r = (i64)rb * 128 + i * 8 + wid;
-    if (r >= j.rows) continue;
+    if (j.by_row) {
+      m = fmaxf(fmaxf(finite_abs(v[i].x), finite_abs(v[i].y)), fmaxf(finite_abs(v[i].z), finite_abs(v[i].w)));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float inv;
+      s = block_scale(m, &inv);
+      if (lane == 0 && r < j.rows) j.inv[cbi * j.inv_ld + r] = inv;
+    }
+    if (r >= j.rows || c0 >= j.ld) continue;
     uint2 h, l;
     split2(v[i].x * s, v[i].y * s, &h.x, &l.x);
     split2(v[i].z * s, v[i].w * s, &h.y, &l.y);
@@ -70,36 +81,51 @@ __global__ void __launch_bounds__(256) k_split16(SplitDev j0, SplitDev j1) {
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------
-struct OperandDev { CUtensorMap map; const float* inv; int inv_ld; int mn; };
+struct OperandDev { CUtensorMap map; const float* inv; i64 inv_ld; int mn, by_row; };
 struct ProblemDev {
   OperandDev a, b;
+  CUtensorMap out_map;                       // Store: f32, where `by_copy`; LossGrad: the planes
   int M, N, K, tiles_m, tiles;
-  float* out; i64 ldo; int add;
+  float* out; i64 ldo; int add, by_copy;
   const float* alpha; float alpha_host;
 };
 struct Params {
   ProblemDev prob[2];
   const int* target; int col0; float2* stats; float* target_value; const float* lse;
-  __half* grad; i64 grad_ld, grad_plane;
+  int* counter;                              // 0: tiles handed out beyond the first of every CTA
   int* err;
 };
-enum { B_FULL = 0, B_EMPTY = B_FULL + kStages, B_RUN = B_EMPTY + kStages, B_RUNFREE = B_RUN + 2, B_COUNT = B_RUNFREE + 2 };
+enum { B_FULL = 0, B_EMPTY = B_FULL + kStages, B_RUN = B_EMPTY + kStages, B_RUNFREE = B_RUN + 2, B_POST = B_RUNFREE + 2, B_TAKEN = B_POST + 2, B_COUNT = B_TAKEN + 2 };
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+// (as an instruction of its own: the compiler's form of atomicAdd waits for the answer on the spot)
+__device__ __forceinline__ int next_tile(int* counter) {
+  int r;
+  asm volatile("atom.global.add.s32 %0, [%1], 1;" : "=r"(r) : "l"(counter) : "memory");
+  return r;
+}
+__device__ __forceinline__ void store_block(const CUtensorMap* map, const void* src, int c, int r, int plane) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(c), "r"(r), "r"(plane) : "memory");
+}
+__device__ __forceinline__ void add_block(const CUtensorMap* map, const void* src, int c, int r, int plane) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(c), "r"(r), "r"(plane) : "memory");
+}
+__device__ __forceinline__ void commit_blocks() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 template <Tile16 WHAT>
 __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint32_t* staging = (uint32_t*)(smem + kStages * kStage);
-  uint64_t* bars = (uint64_t*)((uint8_t*)staging + 8 * kStaging);
+  uint8_t* staging = smem + kStages * kStage;
+  uint64_t* bars = (uint64_t*)(staging + kEpiWarps * kStaging);
   uint32_t* tmem_slot = (uint32_t*)(bars + B_COUNT);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  volatile int* posted = abort_flag + 1;       // [2] tiles handed to the other roles
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) { mbar_init(&bars[B_FULL + i], 1); mbar_init(&bars[B_EMPTY + i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bars[B_RUN + i], 1); mbar_init(&bars[B_RUNFREE + i], 8); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars[B_RUN + i], 1); mbar_init(&bars[B_RUNFREE + i], kEpiWarps); mbar_init(&bars[B_POST + i], 1); mbar_init(&bars[B_TAKEN + i], 1 + kEpiWarps); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -112,12 +138,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.prob[0].tiles + p.prob[1].tiles;
+  // the i-th tile of the CTA for a whole warp; false where there are no more (or a wait ran out)
+  auto take = [&](uint32_t i, int* t) -> bool {
+    const bool ok = warp_wait(&bars[B_POST + (i & 1)], (i >> 1) & 1, abort_flag);
+    *t = posted[i & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[B_TAKEN + (i & 1)]);
+    return ok && *t < tiles;
+  };
 
   if (warp == 0) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int t = blockIdx.x, next = 0;
+      for (uint32_t i = 0; ok; ++i, t = (int)gridDim.x + next) {
+        if (!mbar_wait(&bars[B_TAKEN + (i & 1)], ((i >> 1) & 1) ^ 1, abort_flag)) break;
+        posted[i & 1] = t;
+        mbar_arrive(&bars[B_POST + (i & 1)]);
+        if (t >= tiles) break;
+        next = next_tile(p.counter);
         const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
         const int lt = t < p.prob[0].tiles ? t : t - p.prob[0].tiles;
         const int m0 = (lt % q.tiles_m) * kBM, n0 = (lt / q.tiles_m) * kBN;
@@ -131,9 +171,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
             uint8_t* a = base + pl * kAPlane;
             uint8_t* b = base + 2 * kAPlane + pl * kBPlane;
             if (!q.a.mn) tma_load_3d(a, &q.a.map, full, k0, m0, pl);
-            else for (int i = 0; i < kBM / 64; ++i) tma_load_3d(a + i * 8192, &q.a.map, full, m0 + 64 * i, k0, pl);
+            else for (int x = 0; x < kBM / 64; ++x) tma_load_3d(a + x * 8192, &q.a.map, full, m0 + 64 * x, k0, pl);
             if (!q.b.mn) tma_load_3d(b, &q.b.map, full, k0, n0, pl);
-            else for (int i = 0; i < kBN / 64; ++i) tma_load_3d(b + i * 8192, &q.b.map, full, n0 + 64 * i, k0, pl);
+            else for (int x = 0; x < kBN / 64; ++x) tma_load_3d(b + x * 8192, &q.b.map, full, n0 + 64 * x, k0, pl);
           }
         }
       }
@@ -149,7 +189,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
     const uint32_t leader = elect_leader();
     uint32_t it = 0, run = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    int t;
+    for (uint32_t i = 0; ok && take(i, &t); ++i) {
       const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
       const uint32_t idesc = idesc16(kBM, kBN, q.a.mn, q.b.mn);
       const uint64_t step_a = (q.a.mn ? 2048 : 32) >> 4, step_b = (q.b.mn ? 2048 : 32) >> 4;
@@ -181,108 +222,163 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
   } else {
     const int w = warp - 2, quarter = warp & 3, half = w >> 2;
     const int row = quarter * 32 + lane;
-    uint32_t* stg = staging + w * 32 * kPitch;
+    uint8_t* stg = staging + w * kStaging;
     uint32_t run = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    int t;
+    for (uint32_t i = 0; ok && take(i, &t); ++i) {
       const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
       const int lt = t < p.prob[0].tiles ? t : t - p.prob[0].tiles;
       const int tm = lt % q.tiles_m, tn = lt / q.tiles_m;
       const int m = tm * kBM + row, n0 = tn * kBN + half * 128;
+      int target = kNoTarget;
+      float off = 0.0f;
+      if (WHAT != Tile16::Store && m < q.M) {
+        target = p.target[m];
+        if (WHAT == Tile16::LossGrad) off = p.lse[m];
+      }
       float acc[128];
 #pragma unroll
-      for (int i = 0; i < 128; ++i) acc[i] = 0.0f;
+      for (int c = 0; c < 128; ++c) acc[c] = 0.0f;
       const int nb = n0 < q.N ? tn * 2 + half : tn * 2;          // (a half tile past the last column has no scale of its own)
-      for (int kb = 0; kb * 128 < q.K; ++kb, ++run) {
+      auto scale_of = [&](int kb) -> float {
         float s = 1.0f;
-        if (q.a.inv) s = q.a.mn ? q.a.inv[(i64)kb * q.a.inv_ld + tm] : q.a.inv[(i64)tm * q.a.inv_ld + kb];
+        if (q.a.by_row) s = m < q.M ? q.a.inv[kb * q.a.inv_ld + m] : 0.0f;
+        else if (q.a.inv) s = q.a.mn ? q.a.inv[(i64)kb * q.a.inv_ld + tm] : q.a.inv[(i64)tm * q.a.inv_ld + kb];
         if (q.b.inv) s *= q.b.mn ? q.b.inv[(i64)kb * q.b.inv_ld + nb] : q.b.inv[(i64)nb * q.b.inv_ld + kb];
+        return s;
+      };
+      float s = scale_of(0);
+      for (int kb = 0; kb * 128 < q.K; ++kb, ++run) {
+        const float s_next = (kb + 1) * 128 < q.K ? scale_of(kb + 1) : 0.0f;
         if (!mbar_wait(&bars[B_RUN + (run & 1)], (run >> 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const uint32_t src = tmem + (run & 1) * kBN + half * 128 + ((uint32_t)(quarter * 32) << 16);
+        const float2 s2 = make_float2(s, s);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 128; c += 32) {
           uint32_t v[32];
-          tmem_ld32(src + c * 32, v);
+          tmem_ld32(src + c, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[c * 32 + i] = fmaf(__uint_as_float(v[i]), s, acc[c * 32 + i]);
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), s2, make_float2(acc[c + e], acc[c + e + 1]));
+            acc[c + e] = x.x; acc[c + e + 1] = x.y;
+          }
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[B_RUNFREE + (run & 1)]);
+        s = s_next;
       }
       if (!ok) break;
+      constexpr float kL2e = 1.4426950408889634f;
+      const int mrow = tm * kBM + quarter * 32;
       if constexpr (WHAT == Tile16::Store) {
         const float alpha = (q.alpha ? *q.alpha : 1.0f) * q.alpha_host;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          // 16-byte pieces of a 128-byte row, in the copy engine's 128-byte swizzle
+          if (lane == 0) tma_store_wait_read();
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) stg[lane * kPitch + i] = __float_as_uint(acc[c * 32 + i] * alpha);
-          __syncwarp();
-          const int col = n0 + c * 32 + lane;
-          const int mrow = tm * kBM + quarter * 32;
-          if (col < q.N) {
-            float* o = q.out + (i64)mrow * q.ldo + col;
+          for (int e = 0; e < 8; ++e)
+            *reinterpret_cast<float4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                make_float4(acc[c * 32 + 4 * e] * alpha, acc[c * 32 + 4 * e + 1] * alpha, acc[c * 32 + 4 * e + 2] * alpha, acc[c * 32 + 4 * e + 3] * alpha);
+          const int col = n0 + c * 32;
+          if (q.by_copy) {
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0 && col < q.N && mrow < q.M) {
+              if (q.add) add_block(&q.out_map, stg, col, mrow, 0); else store_block(&q.out_map, stg, col, mrow, 0);
+              commit_blocks();
+            }
+          } else {
+            __syncwarp();
             const int live = q.M - mrow < 32 ? q.M - mrow : 32;
-            if (q.add) for (int r = 0; r < live; ++r) o[(i64)r * q.ldo] += __uint_as_float(stg[r * kPitch + lane]);
-            else for (int r = 0; r < live; ++r) o[(i64)r * q.ldo] = __uint_as_float(stg[r * kPitch + lane]);
+            if (col + lane < q.N) {
+              float* o = q.out + (i64)mrow * q.ldo + col + lane;
+              for (int r = 0; r < live; ++r) {
+                const float x = *reinterpret_cast<const float*>(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                o[(i64)r * q.ldo] = q.add ? o[(i64)r * q.ldo] + x : x;
+              }
+            }
           }
         }
       } else if constexpr (WHAT == Tile16::RowStats) {
         const int live = q.N - n0;                     // columns of this half that exist
-        if (m < q.M && live > 0) {
-          const int tgt = p.target[m] - p.col0 - n0;
-          constexpr float kL2e = 1.4426950408889634f;
-          float mx = -INFINITY;
+        if (live > 0) {
+          const int tgt = target - p.col0 - n0;
+          if (live < 128) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            if (i == tgt && i < live) p.target_value[m] = acc[i];
-            if (i >= live) acc[i] = -INFINITY;
-            mx = fmaxf(mx, acc[i]);
+            for (int c = 0; c < 128; ++c) if (c >= live) acc[c] = -INFINITY;
           }
-          float sum = 0.0f;
-          if (mx > -INFINITY) {
-            const float off = -mx * kL2e;
+          if (__any_sync(0xffffffffu, tgt >= 0 && tgt < 128 && tgt < live)) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i) sum += exp2_fast(fmaf(acc[i], kL2e, off));
+            for (int c = 0; c < 128; ++c) if (c == tgt && c < live) p.target_value[m] = acc[c];
           }
-          p.stats[(i64)(tn * 2 + half) * q.M + m] = make_float2(mx, sum);
+          float mx[4] = {acc[0], acc[1], acc[2], acc[3]};
+#pragma unroll
+          for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], acc[c]);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const float lift = top > -INFINITY ? -top * kL2e : 0.0f;
+          const float2 k2 = make_float2(kL2e, kL2e), l2 = make_float2(lift, lift);
+          float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
+#pragma unroll
+          for (int c = 0; c < 128; c += 4) {
+            const float2 x = fma2(make_float2(acc[c], acc[c + 1]), k2, l2), y = fma2(make_float2(acc[c + 2], acc[c + 3]), k2, l2);
+            sum0 = add2(sum0, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+            sum1 = add2(sum1, make_float2(exp2_fast(y.x), exp2_fast(y.y)));
+          }
+          sum0 = add2(sum0, sum1);
+          if (m < q.M) p.stats[(i64)(tn * 2 + half) * q.M + m] = make_float2(top, sum0.x + sum0.y);
         }
       } else {
-        const int tgt0 = m < q.M ? p.target[m] : kNoTarget;
-        const int tgt = tgt0 - p.col0 - n0;
-        constexpr float kL2e = 1.4426950408889634f;
-        const float off = m < q.M ? -p.lse[m] * kL2e + 14.0f : 0.0f;     // 2^14 rides in the exponent
-        const bool live_row = tgt0 != kNoTarget;
+        const int tgt = target - p.col0 - n0;
+        off = target != kNoTarget ? 14.0f - off * kL2e : -INFINITY;     // (2^14 rides in the exponent; a row without a target is 0: its logits are finite, the row of x was read as 0)
+        const float2 k2 = make_float2(kL2e, kL2e), o2 = make_float2(off, off);
+#pragma unroll
+        for (int c = 0; c < 128; c += 2) {
+          const float2 x = fma2(make_float2(acc[c], acc[c + 1]), k2, o2);
+          acc[c] = exp2_fast(x.x); acc[c + 1] = exp2_fast(x.y);
+        }
+        if (__any_sync(0xffffffffu, tgt >= 0 && tgt < 128)) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) if (c == tgt) acc[c] -= kGradScale;
+        }
+        if (q.N - n0 < 128) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c) if (n0 + c >= q.N) acc[c] = 0.0f;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          // 16-byte pieces of a plane's 64-byte row, in the copy engine's 64-byte swizzle
+          if (lane == 0) tma_store_wait_read();
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float d[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int j = c * 32 + i + e;
-              d[e] = exp2_fast(fmaf(acc[j], kL2e, off)) - (j == tgt ? kGradScale : 0.0f);
-              if (!live_row || n0 + j >= q.N) d[e] = 0.0f;
-            }
-            uint32_t h, l;
-            split2(d[0], d[1], &h, &l);
-            stg[lane * kPitch + i / 2] = h;
-            stg[lane * kPitch + 16 + i / 2] = l;
+          for (int e = 0; e < 4; ++e) {
+            uint4 h, l;
+            split2_finite(acc[c * 32 + 8 * e], acc[c * 32 + 8 * e + 1], &h.x, &l.x);
+            split2_finite(acc[c * 32 + 8 * e + 2], acc[c * 32 + 8 * e + 3], &h.y, &l.y);
+            split2_finite(acc[c * 32 + 8 * e + 4], acc[c * 32 + 8 * e + 5], &h.z, &l.z);
+            split2_finite(acc[c * 32 + 8 * e + 6], acc[c * 32 + 8 * e + 7], &h.w, &l.w);
+            const int at = lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4);
+            *reinterpret_cast<uint4*>(stg + at) = h;
+            *reinterpret_cast<uint4*>(stg + 2048 + at) = l;
           }
+          fence_async_smem();
           __syncwarp();
-          const int col = n0 + c * 32, mrow = tm * kBM + quarter * 32;
-          const int live = q.M - mrow < 32 ? q.M - mrow : 32;
-          if (col + 2 * (lane & 15) < p.grad_ld) {
-            uint32_t* o = reinterpret_cast<uint32_t*>(p.grad + (lane < 16 ? 0 : p.grad_plane) + (i64)mrow * p.grad_ld + col) + (lane & 15);
-            for (int r = 0; r < live; ++r) o[(i64)r * (p.grad_ld / 2)] = stg[r * kPitch + lane];
+          const int col = n0 + c * 32;
+          if (lane == 0 && col < q.N && mrow < q.M) {
+            store_block(&q.out_map, stg, col, mrow, 0);
+            store_block(&q.out_map, stg + 2048, col, mrow, 1);
+            commit_blocks();
           }
         }
       }
     }
+    if (WHAT != Tile16::RowStats && lane == 0) tma_store_wait_read();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -314,7 +410,19 @@ int make_operand(const Op16& o, int box_mn, OperandDev* d) {
   CUresult r = encode_fn()(&d->map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, o.s.planes, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(VB_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
-  d->inv = o.s.inv; d->inv_ld = (int)o.s.inv_ld; d->mn = o.mn;
+  d->inv = o.s.inv; d->inv_ld = o.s.inv_ld; d->mn = o.mn; d->by_row = o.s.by_row;
+  return VB_OK;
+}
+
+// map of a result for the epilogue's 32 x 32 blocks: f32 rows of `ld` (128-byte swizzle), or the two planes of halves (64-byte swizzle)
+int make_result(CUtensorMap* map, void* base, i64 cols, i64 rows, i64 ld, i64 plane, bool half) {
+  const cuuint64_t size = half ? 2 : 4;
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, half ? 2u : 1u}, strides[2] = {(cuuint64_t)ld * size, (cuuint64_t)(half ? plane : ld * rows) * size};
+  cuuint32_t box[3] = {32, 32, 1}, estr[3] = {1, 1, 1};
+  CUresult r = encode_fn()(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, half ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(VB_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
   return VB_OK;
 }
 
@@ -332,35 +440,37 @@ int launch(const Params& p, int ctas) {
 
 }  // namespace
 
-Split16 split16_at(void* mem, i64 rows, i64 cols) {
+Split16 split16_at(void* mem, i64 rows, i64 cols, bool by_row) {
   Split16 s{};
-  s.rows = rows; s.cols = cols; s.ld = (cols + 7) / 8 * 8; s.plane = rows * s.ld; s.inv_ld = (cols + 127) / 128;
+  s.rows = rows; s.cols = cols; s.ld = (cols + 7) / 8 * 8; s.plane = rows * s.ld; s.by_row = by_row; s.inv_ld = by_row ? rows : (cols + 127) / 128;
   s.planes = mem;
   s.inv = reinterpret_cast<float*>(static_cast<uint8_t*>(mem) + ((size_t)(2 * s.plane) * 2 + 15) / 16 * 16);
   return s;
 }
 
 int launch_split16(const SplitJob* jobs, int n) {
-  SplitDev d[2] = {};
+  SplitJobs d{};
   double bytes = 0.0;
+  i64 all = 0;
   for (int i = 0; i < n; ++i) {
     const Split16& s = jobs[i].to;
-    const i64 blocks = ((s.rows + 127) / 128) * s.inv_ld;
-    if (blocks > 0x3fffffff) return set_error(VB_ERR_UNSUPPORTED, "matrix too large to split");
-    d[i] = SplitDev{jobs[i].x, (__half*)s.planes, s.inv, s.rows, s.cols, s.ld, s.plane, (int)s.inv_ld, (int)blocks,
-                    s.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(jobs[i].x) & 15) == 0};
+    const i64 cb = (s.cols + 127) / 128, blocks = ((s.rows + 127) / 128) * cb;
+    d.job[i] = SplitDev{jobs[i].x, jobs[i].keep, (__half*)s.planes, s.inv, s.rows, s.cols, s.ld, s.plane, s.inv_ld, (int)cb, (int)blocks,
+                        s.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(jobs[i].x) & 15) == 0, s.by_row};
+    all += blocks;
     bytes += 8.0 * (double)s.rows * (double)s.cols;
   }
-  const int blocks = d[0].blocks + d[1].blocks;
-  if (blocks == 0) return VB_OK;
+  if (all > 0x7fffffff) return set_error(VB_ERR_UNSUPPORTED, "matrix too large to split");
+  if (all == 0) return VB_OK;
   ProfScope prof("split16", bytes);
-  k_split16<<<blocks, 256, 0, ctx().stream>>>(d[0], d[1]);
+  k_split16<<<(unsigned)all, 256, 0, ctx().stream>>>(d);
   VB_LAUNCH_CHECK();
   return VB_OK;
 }
 
-int launch_gemm16(Tile16 what, const Product16* products, int n) {
+int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter) {
   Params p{};
+  p.counter = counter;
   double flops = 0.0;
   for (int i = 0; i < n; ++i) {
     const Product16& g = products[i];
@@ -371,10 +481,13 @@ int launch_gemm16(Tile16 what, const Product16* products, int n) {
     VB_TRY(make_operand(g.a, kBM, &q.a));
     VB_TRY(make_operand(g.b, kBN, &q.b));
     q.out = g.out; q.ldo = g.ldo; q.add = g.add; q.alpha = g.alpha; q.alpha_host = g.alpha_host;
+    // (the copy engine stores rows that begin on 16 bytes)
+    q.by_copy = what == Tile16::Store && g.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+    if (q.by_copy) VB_TRY(make_result(&q.out_map, g.out, g.N, g.M, g.ldo, 0, false));
+    if (what == Tile16::LossGrad) VB_TRY(make_result(&q.out_map, g.grad.planes, g.N, g.M, g.grad.ld, g.grad.plane, true));
     flops += 2.0 * (double)g.M * (double)g.N * (double)g.K;
   }
   p.target = products[0].target; p.col0 = (int)products[0].col0; p.stats = products[0].stats; p.target_value = products[0].target_value; p.lse = products[0].lse;
-  p.grad = (__half*)products[0].grad.planes; p.grad_ld = products[0].grad.ld; p.grad_plane = products[0].grad.plane;
   p.err = ctx().d_err;
   const int tiles = p.prob[0].tiles + p.prob[1].tiles;
   if (tiles == 0) return VB_OK;

@@ -6,17 +6,18 @@
 
 namespace vb {
 
-// [rows, cols] as two half planes (hi, then lo `plane` halves later), rows `ld` halves apart; inv: 2^-e of each 128 x 128 block.
-struct Split16 { void* planes; float* inv; i64 rows, cols, ld, plane, inv_ld; };
-inline size_t split16_bytes(i64 rows, i64 cols) {
+// [rows, cols] as two half planes (hi, then lo `plane` halves later), rows `ld` halves apart; inv: 2^-e of each 128 x 128 block, [row
+// block][column block], or, `by_row`, of 128 columns of each row, [column block][row].  By row, a row keeps its bits beside one that is
+// many times as large: for the M side of a product over its columns, where a row's scale costs nothing.
+struct Split16 { void* planes; float* inv; i64 rows, cols, ld, plane, inv_ld; bool by_row; };
+inline size_t split16_bytes(i64 rows, i64 cols, bool by_row = false) {
   const i64 ld = (cols + 7) / 8 * 8;
-  return (size_t)(2 * rows * ld) * 2 + 16 + (size_t)(((rows + 127) / 128) * ((cols + 127) / 128)) * sizeof(float);
+  return (size_t)(2 * rows * ld) * 2 + 16 + (size_t)((by_row ? rows : (rows + 127) / 128) * ((cols + 127) / 128)) * sizeof(float);
 }
-Split16 split16_at(void* mem, i64 rows, i64 cols);                                                // lays the pair out in memory of that size
-struct SplitJob { const float* x; Split16 to; };                                                 // x: [rows, cols] contiguous
-int launch_split16(const SplitJob* jobs, int n);                                                  // n <= 2, one launch
-
+Split16 split16_at(void* mem, i64 rows, i64 cols, bool by_row = false);                           // lays the pair out in memory of that size
 constexpr int kNoTarget = -(1 << 30);
+struct SplitJob { const float* x; Split16 to; const int* keep = nullptr; };                       // x: [rows, cols] contiguous; keep[row] == kNoTarget: read as 0
+int launch_split16(const SplitJob* jobs, int n);                                                  // n <= 3, one launch
 
 // What a product does with its tiles.
 enum class Tile16 {
@@ -41,6 +42,7 @@ struct Product16 {
   const float* lse;                              // [M]
   Split16 grad;                                  // [M, N]
 };
-int launch_gemm16(Tile16 what, const Product16* products, int n);      // n <= 2 (Store), independent of one another, one launch
+// n <= 2 (Store), independent of one another, one launch; counter: an int on the device that is 0 when the launch begins
+int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter);
 
 }  // namespace vb

@@ -20,10 +20,11 @@ __device__ __forceinline__ int read_target(float v, i64 ignore, i64 vocab, int* 
   if (!(roundf(v) < (float)vocab)) { atomicOr(err, ERRBIT_OOB_ID); return kNoTarget; }
   return (int)roundf(v);
 }
-// One CTA: every row's target and, for the backward pass, coef = g / (rows with a target).
+// One CTA: every row's target, the products' tile counters and, for the backward pass, coef = g / (rows with a target).
 __global__ void __launch_bounds__(1024) k_targets(const float* __restrict__ targets, i64 n, i64 ignore, i64 vocab, int* __restrict__ out,
-                                                  const float* __restrict__ g, float* __restrict__ coef, int* err) {
+                                                  const float* __restrict__ g, float* __restrict__ coef, int* counters, int n_counters, int* err) {
   __shared__ int red[32];
+  for (int i = threadIdx.x; i < n_counters; i += 1024) counters[i] = 0;      // of the products that follow
   int live = 0;
   for (i64 i = threadIdx.x; i < n; i += 1024) {
     const int t = read_target(targets[i], ignore, vocab, err);
@@ -97,20 +98,20 @@ constexpr i64 kPieceBytes = (i64)512 << 20;
 int launch_head_loss(const float* x, const float* w, const float* targets, i64 ignore, float* loss, float* lse, i64 n, i64 d, i64 v) {
   Temp hx, hw, hs, hr;
   const i64 pairs = (v + 127) / 128;
-  VB_TRY(scratch_alloc(split16_bytes(n, d), &hx.p));
+  VB_TRY(scratch_alloc(split16_bytes(n, d, true), &hx.p));
   VB_TRY(scratch_alloc(split16_bytes(v, d), &hw.p));
   VB_TRY(scratch_alloc((size_t)(pairs * n) * sizeof(float2), &hs.p));
-  VB_TRY(scratch_alloc((size_t)n * 12, &hr.p));
-  float* nll = (float*)hr.p; float* tv = nll + n; int* tgt = (int*)(tv + n);
-  const Split16 sx = split16_at(hx.p, n, d), sw = split16_at(hw.p, v, d);
+  VB_TRY(scratch_alloc((size_t)n * 12 + 4, &hr.p));
+  float* nll = (float*)hr.p; float* tv = nll + n; int* tgt = (int*)(tv + n); int* counter = tgt + n;
+  const Split16 sx = split16_at(hx.p, n, d, true), sw = split16_at(hw.p, v, d);
   const SplitJob jobs[2] = {{x, sx}, {w, sw}};
   VB_TRY(launch_split16(jobs, 2));
-  k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, nullptr, nullptr, ctx().d_err);
+  k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, nullptr, nullptr, counter, 1, ctx().d_err);
   VB_LAUNCH_CHECK();
   Product16 g{};
   g.a = Op16{sx, false}; g.b = Op16{sw, false}; g.M = n; g.N = v; g.K = d;
   g.target = tgt; g.stats = (float2*)hs.p; g.target_value = tv;
-  VB_TRY(launch_gemm16(Tile16::RowStats, &g, 1));
+  VB_TRY(launch_gemm16(Tile16::RowStats, &g, 1, counter));
   k_join_stats<<<(unsigned)((n + 31) / 32), dim3(32, 32), 0, ctx().stream>>>((const float2*)hs.p, tv, tgt, lse, nll, (int)n, (int)pairs);
   VB_LAUNCH_CHECK();
   k_mean_loss<<<1, 1024, 0, ctx().stream>>>(nll, tgt, n, loss);
@@ -120,23 +121,25 @@ int launch_head_loss(const float* x, const float* w, const float* targets, i64 i
 
 int launch_head_loss_backward(const float* x, const float* w, const float* targets, i64 ignore, const float* lse, const float* g, float* gx, float* gw,
                               i64 n, i64 d, i64 v) {
-  Temp hx, hw, hz, ht;
+  Temp hx, hk, hw, hz, ht;
   i64 piece = kPieceBytes / (4 * n) / 256 * 256;
   if (piece < 256) piece = 256;
   const i64 pieces = (v + piece - 1) / piece;
   piece = ((v + pieces - 1) / pieces + 255) / 256 * 256;
   if (piece > v) piece = v;
-  VB_TRY(scratch_alloc(split16_bytes(n, d), &hx.p));
+  VB_TRY(scratch_alloc(split16_bytes(n, d, true), &hx.p));
+  if (gw) VB_TRY(scratch_alloc(split16_bytes(n, d), &hk.p));
   VB_TRY(scratch_alloc(split16_bytes(v, d), &hw.p));
   VB_TRY(scratch_alloc(split16_bytes(n, piece), &hz.p));
-  VB_TRY(scratch_alloc((size_t)n * 4 + 16, &ht.p));
-  float* coef = (float*)ht.p; int* tgt = (int*)(coef + 4);
-  const Split16 sx = split16_at(hx.p, n, d), sw = split16_at(hw.p, v, d);
-  const SplitJob jobs[2] = {{x, sx}, {w, sw}};
-  VB_TRY(launch_split16(jobs, 2));
-  k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, g, coef, ctx().d_err);
+  VB_TRY(scratch_alloc((size_t)(n + 2 * pieces) * 4 + 16, &ht.p));
+  float* coef = (float*)ht.p; int* tgt = (int*)(coef + 4); int* counters = tgt + n;
+  const Split16 sx = split16_at(hx.p, n, d, true), sw = split16_at(hw.p, v, d);      // x for the logits, where its rows are the product's,
+  const Split16 sk = gw ? split16_at(hk.p, n, d) : sx;                                  // and for dW, which sums over them
+  k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, g, coef, counters, (int)(2 * pieces), ctx().d_err);
   VB_LAUNCH_CHECK();
-  for (i64 v0 = 0; v0 < v; v0 += piece) {
+  const SplitJob jobs[3] = {{w, sw}, {x, sx, tgt}, {x, sk, tgt}};        // (rows that are left out may hold anything: they must not reach dW)
+  VB_TRY(launch_split16(jobs, gw ? 3 : 2));
+  for (i64 v0 = 0; v0 < v; v0 += piece, counters += 2) {
     const i64 vc = v - v0 < piece ? v - v0 : piece;
     Split16 wc = sw;                                     // this piece's rows of W
     wc.planes = (uint16_t*)sw.planes + v0 * sw.ld; wc.inv = sw.inv + v0 / 128 * sw.inv_ld; wc.rows = vc;
@@ -144,7 +147,7 @@ int launch_head_loss_backward(const float* x, const float* w, const float* targe
     Product16 f{};
     f.a = Op16{sx, false}; f.b = Op16{wc, false}; f.M = n; f.N = vc; f.K = d;
     f.target = tgt; f.col0 = v0; f.lse = lse; f.grad = z;
-    VB_TRY(launch_gemm16(Tile16::LossGrad, &f, 1));
+    VB_TRY(launch_gemm16(Tile16::LossGrad, &f, 1, counters));
     z.inv = nullptr;
     Product16 b[2] = {};
     int nb = 0;
@@ -155,10 +158,10 @@ int launch_head_loss_backward(const float* x, const float* w, const float* targe
     }
     if (gw) {
       Product16& q = b[nb++];
-      q.a = Op16{z, true}; q.b = Op16{sx, true}; q.M = vc; q.N = d; q.K = n;
+      q.a = Op16{z, true}; q.b = Op16{sk, true}; q.M = vc; q.N = d; q.K = n;
       q.out = gw + v0 * d; q.ldo = d; q.alpha = coef; q.alpha_host = 1.0f / 16384.0f;
     }
-    if (nb) VB_TRY(launch_gemm16(Tile16::Store, b, nb));
+    if (nb) VB_TRY(launch_gemm16(Tile16::Store, b, nb, counters + 1));
   }
   return VB_OK;
 }
