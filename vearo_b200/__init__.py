@@ -109,6 +109,10 @@ def lib():
         L.vb_segment_attention_backward.argtypes = [T] * 4 + [C.c_float] + [T] * 6
         L.vb_linear_cross_entropy.argtypes = [T] * 3 + [C.c_int64] + [T] * 2
         L.vb_linear_cross_entropy_backward.argtypes = [T] * 3 + [C.c_int64] + [T] * 4
+        L.vh_norm_rope.argtypes = [C.c_int] * 3 + [C.c_float, C.c_int, C.c_int, C.c_float]
+        L.vh_qk_norm_rope.argtypes = [C.c_int] * 5 + [C.c_float, C.c_int, C.c_int, C.c_float, c_intp]
+        L.vh_segment_attention.argtypes = [C.c_int] * 4 + [C.c_float]
+        L.vh_linear_cross_entropy.argtypes = [C.c_int] * 3 + [C.c_int64]
         _lib = L
     return _lib
 
@@ -233,6 +237,28 @@ class Tensor:
     def fused_attention_packed(self, n_head, mask=None):
         """self = [B, S, 3*D] with column blocks q | k | v; returns the [B, S, D] context."""
         return Tensor(lib().vh_fused_attention_packed(self.h, int(n_head), -1 if mask is None else mask.h))
+
+    def norm_rope(self, w, positions, theta=10000.0, rot_dim=None, interleaved=False, eps=1e-6):
+        """self = [T, H, dk]: RMS norm of every head with weight w [dk], then the rotary turn of its first rot_dim components (all of
+        them by default) by positions [T]."""
+        rot = self.shape[-1] if rot_dim is None else rot_dim
+        return Tensor(lib().vh_norm_rope(self.h, w.h, positions.h, theta, rot, int(interleaved), eps))
+
+    def qk_norm_rope(self, k, wq, wk, positions, theta=10000.0, rot_dim=None, interleaved=False, eps=1e-6):
+        """norm_rope of queries (self) and keys k in one launch; returns both."""
+        rot = self.shape[-1] if rot_dim is None else rot_dim
+        out = (C.c_int * 2)()
+        _chk(lib().vh_qk_norm_rope(self.h, k.h, wq.h, wk.h, positions.h, theta, rot, int(interleaved), eps, out))
+        return Tensor(out[0]), Tensor(out[1])
+
+    def segment_attention(self, k, v, starts, scale=None):
+        """self = queries [T, Hq, dk], k and v [T, Hkv, dk], starts [segments + 1] row offsets: causal attention within each segment;
+        scale defaults to 1 / sqrt(dk)."""
+        return Tensor(lib().vh_segment_attention(self.h, k.h, v.h, starts.h, self.shape[-1] ** -0.5 if scale is None else scale))
+
+    def linear_cross_entropy(self, w, targets, ignore_index=-100):
+        """self.linear(w).cross_entropy(targets) without the logits in memory; rows whose target is ignore_index are left out of the mean."""
+        return Tensor(lib().vh_linear_cross_entropy(self.h, w.h, targets.h, ignore_index))
 
     def linear(self, w, b=None): return Tensor(lib().vh_linear(self.h, w.h, -1 if b is None else b.h))
 

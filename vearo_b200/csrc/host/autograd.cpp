@@ -81,12 +81,12 @@ void Tensor::write_f32(const float* data) const {
 // ---- tape ------------------------------------------------------------------------------------
 namespace {
 enum class Op { Add, Sub, Mul, Div, Matmul, Reshape, Transpose, Permute, Relu, Gelu, Softmax, LayerNorm, Embedding,
-                CrossEntropy, Sum, Mean, Conv2d, MaxPool2d, AvgPool2d, BatchNorm, FusedAttention, Linear, BnReluPool, PackRows, FusedAttentionPacked, Checkpoint, Leaf };
+                CrossEntropy, Sum, Mean, Conv2d, MaxPool2d, AvgPool2d, BatchNorm, FusedAttention, Linear, BnReluPool, PackRows, FusedAttentionPacked, NormRope, SegmentAttention, LinearCrossEntropy, Checkpoint, Leaf };
 struct Node {
   int id = 0; Op op = Op::Leaf;
   std::vector<int> inputs;
   std::vector<Tensor> saved;
-  i64 a0 = 0, a1 = 0, a2 = 0; float f0 = 0.0f;
+  i64 a0 = 0, a1 = 0, a2 = 0; float f0 = 0.0f, f1 = 0.0f;
   std::vector<i64> axes;
   Tensor extra;             // attention probabilities / cross-entropy row statistics
   Tensor leaf;              // for Leaf nodes: the tensor itself
@@ -265,6 +265,42 @@ Tensor Tensor::fused_attention_packed(i64 n_head, const Tensor* mask) const {
   Tensor out = Tensor::adopt(o_);
   Tensor probs; if (rec) probs = Tensor::adopt(p_);
   if (Node* n = record(Op::FusedAttentionPacked, ins, out)) { n->extra = probs; n->a0 = n_head; }
+  return out;
+}
+static void record_norm_rope(const Tensor& x, const Tensor& w, const Tensor& positions, float theta, int rot_dim, bool interleaved, float eps, Tensor& out) {
+  if (Node* n = record(Op::NormRope, {&x, &w, &positions}, out)) { n->a0 = rot_dim; n->a1 = interleaved; n->f0 = eps; n->f1 = theta; }
+}
+Tensor Tensor::norm_rope(const Tensor& weight, const Tensor& positions, float theta, int rot_dim, bool interleaved, float eps) const {
+  VB_OUT1(vb_qk_norm_rope(&d_, nullptr, &weight.d_, nullptr, &positions.d_, theta, rot_dim, interleaved, eps, &o_, nullptr), "qk_norm_rope");
+  record_norm_rope(*this, weight, positions, theta, rot_dim, interleaved, eps, out);
+  return out;
+}
+std::pair<Tensor, Tensor> Tensor::qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& positions, float theta, int rot_dim,
+                                               bool interleaved, float eps) {
+  vb_tensor q_, k_;
+  check(vb_qk_norm_rope(&q.d_, &k.d_, &wq.d_, &wk.d_, &positions.d_, theta, rot_dim, interleaved, eps, &q_, &k_), "qk_norm_rope");
+  std::pair<Tensor, Tensor> out{Tensor::adopt(q_), Tensor::adopt(k_)};
+  record_norm_rope(q, wq, positions, theta, rot_dim, interleaved, eps, out.first);
+  record_norm_rope(k, wk, positions, theta, rot_dim, interleaved, eps, out.second);
+  return out;
+}
+// saved behind the inputs: the output; extra: the rows' log-sum-exp
+Tensor Tensor::segment_attention(const Tensor& k, const Tensor& v, const Tensor& starts, float scale) const {
+  const bool rec = t_enabled && (requires_grad() || k.requires_grad() || v.requires_grad());
+  vb_tensor o_, l_;
+  check(vb_segment_attention(&d_, &k.d_, &v.d_, &starts.d_, scale, &o_, rec ? &l_ : nullptr), "segment_attention");
+  Tensor out = Tensor::adopt(o_), lse;
+  if (rec) lse = Tensor::adopt(l_);
+  if (Node* n = record(Op::SegmentAttention, {this, &k, &v, &starts}, out)) { n->f0 = scale; n->extra = lse; n->saved.push_back(Tensor::view_of(out, out.d_)); }
+  return out;
+}
+Tensor Tensor::linear_cross_entropy(const Tensor& weight, const Tensor& targets, i64 ignore_index) const {
+  const bool rec = t_enabled && (requires_grad() || weight.requires_grad());
+  vb_tensor o_, l_;
+  check(vb_linear_cross_entropy(&d_, &weight.d_, &targets.d_, ignore_index, &o_, rec ? &l_ : nullptr), "linear_cross_entropy");
+  Tensor out = Tensor::adopt(o_), lse;
+  if (rec) lse = Tensor::adopt(l_);
+  if (Node* n = record(Op::LinearCrossEntropy, {this, &weight, &targets}, out)) { n->a0 = ignore_index; n->extra = lse; }
   return out;
 }
 Tensor Tensor::pack_rows(const Tensor& a, const Tensor& b, const Tensor& c) {
@@ -478,6 +514,28 @@ void run_backward(const Tensor& y, const Tensor& seed, const NestedInput& nested
                                                  node.extra.defined() ? &node.extra.desc() : nullptr, &dqkv), "fused_attention_packed_backward");
         gin = {Tensor::adopt(dqkv)};
         if (sv.size() > 1) gin.push_back(Tensor());
+        break;
+      }
+      case Op::NormRope: {
+        vb_tensor gx, gw;
+        check(vb_qk_norm_rope_backward(&sv[0].desc(), nullptr, &sv[1].desc(), nullptr, &sv[2].desc(), node.f1, (int)node.a0, (int)node.a1, node.f0, &go.desc(), nullptr,
+                                       &gx, nullptr, &gw, nullptr), "qk_norm_rope_backward");
+        gin = {Tensor::adopt(gx), Tensor::adopt(gw), Tensor()};
+        break;
+      }
+      case Op::SegmentAttention: {
+        vb_tensor dq, dk, dv;
+        check(vb_segment_attention_backward(&sv[0].desc(), &sv[1].desc(), &sv[2].desc(), &sv[3].desc(), node.f0, &sv[4].desc(), &node.extra.desc(), &go.desc(), &dq, &dk, &dv),
+              "segment_attention_backward");
+        gin = {Tensor::adopt(dq), Tensor::adopt(dk), Tensor::adopt(dv), Tensor()};
+        break;
+      }
+      case Op::LinearCrossEntropy: {
+        const bool need_x = node.inputs[0] >= 0, need_w = node.inputs[1] >= 0;
+        vb_tensor gx, gw;
+        check(vb_linear_cross_entropy_backward(&sv[0].desc(), &sv[1].desc(), &sv[2].desc(), node.a0, &node.extra.desc(), &go.desc(), need_x ? &gx : nullptr, need_w ? &gw : nullptr),
+              "linear_cross_entropy_backward");
+        gin = {need_x ? Tensor::adopt(gx) : Tensor(), need_w ? Tensor::adopt(gw) : Tensor(), Tensor()};
         break;
       }
       case Op::PackRows: {      // row blocks of the gradient, as views

@@ -70,6 +70,15 @@ int vh_batchnorm(int x, int g, int b, int rm, int rv, int training, float mom, f
   VH_TRY(return put(at(x).batchnorm(at(g), at(b), at(rm), at(rv), training != 0, mom, eps)));
 }
 int vh_fused_attention(int q, int k, int v, int mask) { VH_TRY(return put(at(q).fused_attention(at(k), at(v), mask >= 0 ? &at(mask) : nullptr))); }
+int vh_norm_rope(int x, int w, int pos, float theta, int rot_dim, int interleaved, float eps) {
+  VH_TRY(return put(at(x).norm_rope(at(w), at(pos), theta, rot_dim, interleaved != 0, eps)));
+}
+int vh_qk_norm_rope(int q, int k, int wq, int wk, int pos, float theta, int rot_dim, int interleaved, float eps, int* out) {
+  VH_TRY(std::pair<Tensor, Tensor> r = Tensor::qk_norm_rope(at(q), at(k), at(wq), at(wk), at(pos), theta, rot_dim, interleaved != 0, eps);
+         out[0] = put(r.first); out[1] = put(r.second); return 0);
+}
+int vh_segment_attention(int q, int k, int v, int starts, float scale) { VH_TRY(return put(at(q).segment_attention(at(k), at(v), at(starts), scale))); }
+int vh_linear_cross_entropy(int x, int w, int t, int64_t ignore_index) { VH_TRY(return put(at(x).linear_cross_entropy(at(w), at(t), ignore_index))); }
 int vh_linear(int x, int w, int b) { VH_TRY(return put(at(x).linear(at(w), b >= 0 ? &at(b) : nullptr))); }
 int vh_linear_gelu(int x, int w, int b) { VH_TRY(return put(at(x).linear_gelu(at(w), b >= 0 ? &at(b) : nullptr))); }
 int vh_reshape(int a, const int64_t* shape, int rank) { VH_TRY(return put(at(a).reshape(std::vector<i64>(shape, shape + rank)))); }

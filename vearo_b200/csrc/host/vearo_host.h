@@ -10,6 +10,7 @@
 #include <memory>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 #include "../../../include/vearo_b200.h"
 
@@ -77,6 +78,15 @@ class Tensor {
   // a, b, c: views that lie one after another along dim 0 of one storage (same trailing shape); the view that spans the three.
   // Recorded on the tape: its gradient is handed back to a, b and c as row blocks.
   static Tensor pack_rows(const Tensor& a, const Tensor& b, const Tensor& c);
+  // self = one tensor of heads [T, H, dk] (queries or keys): RMS norm of every head and the rotary turn (vb_qk_norm_rope)
+  Tensor norm_rope(const Tensor& weight, const Tensor& positions, float theta, int rot_dim, bool interleaved, float eps) const;
+  // queries and keys in one launch (recorded as two nodes)
+  static std::pair<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Tensor& positions, float theta, int rot_dim,
+                                                bool interleaved, float eps);
+  // self = queries [T, Hq, dk]; causal attention within the segments that starts [n + 1] delimits (vb_segment_attention)
+  Tensor segment_attention(const Tensor& k, const Tensor& v, const Tensor& starts, float scale) const;
+  // self = x [.., D]: mean cross entropy of x.weight^T without the logits in memory (vb_linear_cross_entropy)
+  Tensor linear_cross_entropy(const Tensor& weight, const Tensor& targets, i64 ignore_index) const;
   Tensor linear(const Tensor& weight, const Tensor* bias) const;   // fused x.W^T + b
   Tensor linear_gelu(const Tensor& weight, const Tensor* bias) const;   // linear(...).gelu() with the activation formed in the GEMM's epilogue
   Tensor reshape(const std::vector<i64>& shape) const;
