@@ -31,6 +31,8 @@ using namespace tc;
 constexpr int kGroups = 4, kRowWarps = 4 * kGroups, kThreads = 32 * (2 + kRowWarps);      // warp 0: TMA, warp 1: MMA, the others: rows
 constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+__device__ __forceinline__ float2 lo2(const float4& v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi2(const float4& v) { return make_float2(v.z, v.w); }
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // ---- planes ------------------------------------------------------------------------------------------------------------------------
@@ -41,8 +43,8 @@ struct PrepareDev {
   PlanesDev in[4];
   int n, T, tiles, dk, hq;
   const float* starts; int n_seg; int* begin; int* end; int4* ranges; int* order; int* err;      // where the segment of each row begins and ends, and the ranges of a tile's rows
-  const float* o; i64 o_st, o_sh; bool o_vec; const float* lse;                     // for do: delta and the lse in base 2, padded to whole tiles
-  float* delta; float* lse2;
+  const float* o; i64 o_st, o_sh; bool o_vec; const float* lse;                     // for do: delta and 14 - lse in base 2, padded to whole tiles
+  float* delta; float* lift;
 };
 
 // The offset of the segment that row t is in (-1: none), as an index into the offsets.
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
       else { v[i].x = s[0]; if (c + 1 < p.dk) v[i].y = s[1]; if (c + 2 < p.dk) v[i].z = s[2]; if (c + 3 < p.dk) v[i].w = s[3]; }
     }
   }
-  if (p.delta && which == 3) {      // delta of the rows, and their lse in base 2 (a row of no segment: +infinity, so that every p is 0)
+  if (p.delta && which == 3) {      // delta of the rows, and 14 minus their lse in base 2 (a row of no segment: -infinity, so that every p is 0)
     const float* o = p.o + t0 * p.o_st + h * p.o_sh + c;
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
         float l = t < p.T ? p.lse[(i64)h * p.T + t] : -INFINITY;
         const bool dead = l == -INFINITY;
         if (d != d) l = d;             // (a gradient that is not finite: dv sees it through p)
-        p.lse2[at] = dead ? INFINITY : l * kL2e;
+        p.lift[at] = dead ? -INFINITY : 14.0f - l * kL2e;
         p.delta[at] = dead ? 0.0f : d;
       }
     }
@@ -299,10 +301,12 @@ __device__ __forceinline__ void load_cols(uint32_t taddr, float (&v)[W]) {
 }
 // the quarter of a row's columns as the left operand of product_cols: W / 2 columns of hi, W / 2 of lo
 template <int W>
-__device__ __forceinline__ void store_operand(uint32_t taddr, const float (&v)[W]) {
-  uint32_t r[W];
+__device__ __forceinline__ void split_operand(const float (&v)[W], uint32_t (&r)[W]) {
 #pragma unroll
   for (int j = 0; j < W / 2; ++j) split2_finite(v[2 * j], v[2 * j + 1], &r[j], &r[W / 2 + j]);
+}
+template <int W>
+__device__ __forceinline__ void store_operand(uint32_t taddr, const uint32_t (&r)[W]) {
   if constexpr (W == 32) tmem_st32(taddr, r); else tmem_st16(taddr, r);
 }
 // acc = acc * keep + part * f over this thread's quarter of an accumulator
@@ -376,12 +380,12 @@ __device__ __forceinline__ float split_weights(const float (&v)[W], float sc, fl
   return a.x + a.y;
 }
 template <int W>
-__device__ __forceinline__ void weights_of_cols(float (&v)[W], float sc, const float* lse2) {
-  const float2 s2 = make_float2(sc, sc), c14 = make_float2(14.0f, 14.0f), neg = make_float2(-1.0f, -1.0f);
+__device__ __forceinline__ void weights_of_cols(float (&v)[W], float sc, const float* lift) {
+  const float2 s2 = make_float2(sc, sc);
 #pragma unroll
   for (int i = 0; i < W; i += 4) {
-    const float4 l = *reinterpret_cast<const float4*>(lse2 + i);
-    const float2 a = fma2(make_float2(v[i], v[i + 1]), s2, fma2(lo2(l), neg, c14)), b = fma2(make_float2(v[i + 2], v[i + 3]), s2, fma2(hi2(l), neg, c14));
+    const float4 l = *reinterpret_cast<const float4*>(lift + i);
+    const float2 a = fma2(make_float2(v[i], v[i + 1]), s2, lo2(l)), b = fma2(make_float2(v[i + 2], v[i + 3]), s2, hi2(l));
     v[i] = exp2_fast(a.x); v[i + 1] = exp2_fast(a.y); v[i + 2] = exp2_fast(b.x); v[i + 3] = exp2_fast(b.y);
   }
 }
@@ -433,7 +437,7 @@ struct AttnParams {
   const int* order;                           // [2][tiles] tiles by the work they have as queries, and as keys, the most first
   const int4* ranges;                         // [tiles] smallest and largest begin, smallest and largest end of the tile's rows
   Side q, k, v, g;
-  const float* lse2; const float* delta;      // [hq][tiles * 128]
+  const float* lift; const float* delta;      // [hq][tiles * 128]: 14 - lse in base 2 (a weight comes with a factor of 2^14), delta
   float* out; float* lse;                     // forward
   float *dq, *dk_, *dv;                       // backward; with parts > 1 dk_ and dv are [parts][T, hk, dk], summed afterwards
   int parts;                                  // a key head's group of query heads is dealt to this many CTAs
@@ -441,12 +445,25 @@ struct AttnParams {
 };
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------------
+// What the row warps want of a tile besides its matrices, put into shared memory with it: a few of its factors, and for tiles whose columns
+// are queries their lift and delta (read from global memory where they are used they cost two trips to L2 a tile, 1900 of 5700 cycles).
+template <int N, int VECTORS> struct Notes { float4 f; float v[VECTORS][N]; };
+__device__ __forceinline__ void copy_note(float* dst, const float* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void expect_more(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 // The resident tile (Q, or K in the dV kernel) and a ring of planes, streamed in the order in which the products take them: half a tile
 // at a time, so that 128-wide heads too have a product's worth of planes in flight.
 template <int DP> struct StreamSmem {
   static constexpr int kPlane = plane_bytes<128, DP>(), kSlots = DP == 64 ? 10 : 5;
-  static constexpr int kBars = 1 + 2 * kSlots + 2 + 1 + 1;
-  static constexpr int kTotal = 1024 + kPlane * (2 + kSlots) + kBars * 8 + 64;
+  // (dV) Tile j's notes lie in slot j % kNotes.  Its planes are the stream's numbers 4 j - 2 and 4 j - 1, those of do 4 j + 4 and 4 j + 5, and the
+// last are released when P of tile j has been formed: the slot is filled again only after that, as the plane which comes with it has waited.
+  static constexpr int kNotes = DP == 64 ? 4 : 3, kNoteBytes = kNotes * (int)sizeof(Notes<128, 1>);
+  static_assert(4 * kNotes - 2 - kSlots >= 4, "a note is overwritten while it is read");
+  static constexpr int kBars = 1 + 2 * kSlots + 2 + 1 + 1 + kNotes;
+  static constexpr int kTotal = 1024 + kPlane * (2 + kSlots) + kNoteBytes + kBars * 8 + 64;
 };
 // One CTA an SM, sixteen row warps.  Scores have two buffers, so the next tile's are formed while the row warps are at this one's; a
 // weight is split into its halves where its exponential comes out, so that the special-function and the arithmetic pipes work at
@@ -637,8 +654,9 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
   using L = StreamSmem<DP>;
   constexpr int NS = L::kSlots, W = DP / kGroups, H = 128 / kGroups;
   uint8_t *sk = smem, *ring = smem + 2 * L::kPlane;
-  uint64_t* bars = (uint64_t*)(ring + NS * L::kPlane);
-  uint64_t *b_x = bars, *b_full = bars + 1, *b_free = b_full + NS, *b_s = b_free + NS, *b_p = b_s + 2, *b_o = b_p + 1;
+  Notes<128, 1>* notes = (Notes<128, 1>*)(ring + NS * L::kPlane);
+  uint64_t* bars = (uint64_t*)((uint8_t*)notes + L::kNoteBytes);
+  uint64_t *b_x = bars, *b_full = bars + 1, *b_note = b_full + NS, *b_free = b_note + L::kNotes, *b_s = b_free + NS, *b_p = b_s + 2, *b_o = b_p + 1;
   int* ints = (int*)(b_o + 1);
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
@@ -648,6 +666,7 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
   if (threadIdx.x == 0) {
     mbar_init(b_x, 1);
     for (int i = 0; i < NS; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_free[i], 1); }
+    for (int i = 0; i < L::kNotes; ++i) mbar_init(&b_note[i], 1);
     mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -668,17 +687,29 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
     if ((threadIdx.x & 31) == 0 && n > 0) {
       load_tile<128, DP>(sk, &maps.k, b_x, kt * 128, hk);
       uint32_t slot = 0, phase = 1;      // (the first round waits on the phase before the first: free)
-      auto fetch = [&](const CUtensorMap* map, int j) -> bool {      // lo, then hi: the order in which the products take them
+      const float sc0 = p.scale * kL2e * fabsf(p.k.inv[(i64)hk * p.tiles + kt]);
+      struct Place { int i, head, note; } q_at{0, h0, 0}, g_at{0, h0, 0};
+      auto fetch = [&](const CUtensorMap* map, Place& at, bool note) -> bool {      // lo, then hi: the order in which the products take them
         for (int pl = 1; pl >= 0; --pl) {
           if (!mbar_wait(&b_free[slot], phase, abort_flag)) return false;
-          load_plane<128, DP>(ring + slot * L::kPlane, map, &b_full[slot], (kt + j % per) * 128, h0 + j / per, pl);
+          load_plane<128, DP>(ring + slot * L::kPlane, map, &b_full[slot], (kt + at.i) * 128, at.head, pl);
           if (++slot == NS) { slot = 0; phase ^= 1; }
+          if (note && pl == 1) {
+            const i64 tile = (i64)at.head * p.tiles + kt + at.i;
+            Notes<128, 1>& to = notes[at.note];
+            expect_more(&b_note[at.note], 512);
+            copy_note(to.v[0], p.lift + tile * 128, 512, &b_note[at.note]);
+            to.f = make_float4(sc0 * fabsf(p.q.inv[tile]), fabsf(p.g.inv[tile]), 0.0f, 0.0f);
+            mbar_arrive(&b_note[at.note]);
+            if (++at.note == L::kNotes) at.note = 0;
+          }
         }
+        if (++at.i == per) { at.i = 0; ++at.head; }
         return true;
       };
-      bool ok = fetch(&maps.q, 0) && (n < 2 || fetch(&maps.q, 1));
-      for (int j = 0; j < n && ok; ++j) ok = fetch(&maps.g, j) && (j + 2 >= n || fetch(&maps.q, j + 2));
-      if (*abort_flag) let_land(bars, 1 + NS);
+      bool ok = fetch(&maps.q, q_at, true) && (n < 2 || fetch(&maps.q, q_at, true));
+      for (int j = 0; j < n && ok; ++j) ok = fetch(&maps.g, g_at, false) && (j + 2 >= n || fetch(&maps.q, q_at, true));
+      if (*abort_flag) let_land(bars, 1 + NS + L::kNotes);
     }
   } else if (warp == 1) {
     if (n > 0) {
@@ -720,26 +751,34 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
     const Seat at;
     const int t = kt * 128 + at.row;
     const int end = t < p.T ? p.end[t] : 0;
-    const float sc0 = p.scale * kL2e * fabsf(p.k.inv[(i64)hk * p.tiles + kt]);
     float acc[W], f_last = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
     bool ok = true;
+    int qt = kt, note = 0;
+    uint32_t note_phase = 0;
     for (int j = 0; j < n; ++j) {
-      const int qt = kt + j % per, c0 = qt * 128 + at.group * H;
-      const i64 tile = (i64)(h0 + j / per) * p.tiles + qt;
-      const float sc = sc0 * fabsf(p.q.inv[tile]), f_this = fabsf(p.g.inv[tile]);
+      const int c0 = qt * 128 + at.group * H;
+      if (!mbar_wait(&b_note[note], note_phase, abort_flag)) { ok = false; break; }
+      const float4 f = notes[note].f;
+      const float f_this = f.y;
       if (!mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      float v[H];
-      load_cols<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
-      weights_of_cols<H>(v, sc, p.lse2 + tile * 128 + at.group * H);
-      if (qt == kt || qt * 128 + 128 > e_min) keep_columns<H>(v, t - c0, end - 1 - c0, 0.0f);
+      uint32_t r[H];
+      {
+        float v[H];
+        load_cols<H>(t_s + (j & 1) * 128 + at.group * H + at.lane_off, v);
+        weights_of_cols<H>(v, f.x, notes[note].v[0] + at.group * H);
+        if (qt == kt || qt * 128 + 128 > e_min) keep_columns<H>(v, t - c0, end - 1 - c0, 0.0f);
+        split_operand<H>(v, r);
+      }
+      if (++note == L::kNotes) { note = 0; note_phase ^= 1; }
+      if (++qt == kt + per) qt = kt;
       if (j > 0) {
         if (!mbar_wait(b_o, (j - 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
       }
-      store_operand<H>(t_p + at.group * H + at.lane_off, v);
+      store_operand<H>(t_p + at.group * H + at.lane_off, r);
       if (j > 0) add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
       operand_written(b_p, at.lane);
       f_last = f_this;
@@ -766,19 +805,30 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
 //   S = X1 Y1^T, dP = X2 Y2^T, dS = p (dP - delta), result += dS Y1.
 // dS goes where S was; S has two buffers, so the next tile's S and dP are formed while dS Y1 runs.  Y1 is held from S to the last
 // product, so it has three buffers; X2 is kept in tensor memory, as the left operand of dP, to leave room for them.
+// 2^e with 2 |do| |v| 2^e below 2^14, over the weights' 2^14, and 2^-e
+struct DsScale { float to, back; };
+__device__ __forceinline__ DsScale ds_scale(float len, float vmax) {
+  const float b = 2.0f * len * vmax;
+  int e = b > 0.0f ? 13 - ((int)(__float_as_uint(b) >> 23) - 127) : 0;
+  e = e > 100 ? 100 : (e < -100 ? -100 : e);
+  return DsScale{__uint_as_float((uint32_t)(127 + e) << 23) * (1.0f / 16384.0f), __uint_as_float((uint32_t)(127 - e) << 23)};
+}
 template <int DP> struct GradSmem {
   static constexpr int N = DP == 64 ? 128 : 64;                       // 128-wide heads: 64 rows of Y at a time
   static constexpr int kTileX = 2 * plane_bytes<128, DP>(), kTileY = 2 * plane_bytes<N, DP>();
   static constexpr int kY1 = 3, kY2 = 2;
   static constexpr int kBars = 2 + 2 * kY1 + 2 * kY2 + 2 + 1 + 1 + 1;
-  static constexpr int kTotal = 1024 + kTileX + (kY1 + kY2) * kTileY + kBars * 8 + 64;
+  static constexpr int kNoteBytes = kY1 * (int)sizeof(Notes<N, 2>);     // (with the tile of Y1)
+  static constexpr int kTotal = 1024 + kTileX + (kY1 + kY2) * kTileY + kNoteBytes + kBars * 8 + 64;
+  static_assert(kTotal <= 227 * 1024, "shared memory");
 };
 template <int DP, bool DK>
 __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, const AttnParams& p, int block) {
   using L = GradSmem<DP>;
   constexpr int N = L::N, H = N / kGroups, W = DP / kGroups, N1 = L::kY1, N2 = L::kY2, R = 128 / N;
   uint8_t *x1 = smem, *y1 = x1 + L::kTileX, *y2 = y1 + N1 * L::kTileY;
-  uint64_t* bars = (uint64_t*)(y2 + N2 * L::kTileY);
+  Notes<N, 2>* notes = (Notes<N, 2>*)(y2 + N2 * L::kTileY);
+  uint64_t* bars = (uint64_t*)((uint8_t*)notes + L::kNoteBytes);
   uint64_t *b_x = bars, *b_y1full = bars + 1, *b_y2full = b_y1full + N1, *b_y1free = b_y2full + N2, *b_y2free = b_y1free + N1, *b_s = b_y2free + N2, *b_dp = b_s + 2,
            *b_ds = b_dp + 1, *b_o = b_ds + 1, *b_x2 = b_o + 1;
   int* ints = (int*)(b_x2 + 1);
@@ -826,16 +876,31 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
 
   if (warp == 0) {
     if ((threadIdx.x & 31) == 0 && n > 0) {
-      bool ok = true;
       load_tile<128, DP>(x1, map_x1, b_x, xt * 128, hx);
-      for (int j = 0; j < n && ok; ++j) {
-        const int hy = DK ? h0 + j / per : hk, y = (y0 + (DK ? j % per : j)) * N, s1 = j % N1, s2 = j % N2;
-        if (j >= N1) ok = mbar_wait(&b_y1free[s1], ((j / N1) - 1) & 1, abort_flag);
-        if (!ok) break;
+      const i64 x_at = (i64)hx * p.tiles + xt;
+      const float s_x = p.scale * kL2e * fabsf(DK ? p.k.inv[x_at] : p.q.inv[x_at]), fx2 = fabsf(DK ? p.v.inv[x_at] : p.g.inv[x_at]);
+      const DsScale row_scale = DK ? DsScale{} : ds_scale(p.g.len[x_at], vmax);
+      int hy = DK ? h0 : hk, i = 0, s1 = 0, s2 = 0;
+      uint32_t phase1 = 1, phase2 = 1;      // (the first round waits on the phase before the first: free)
+      for (int j = 0; j < n; ++j) {
+        const int y = (y0 + i) * N;
+        const i64 y_at = (i64)hy * p.tiles + y / 128;
+        // factors of S, of dP, of delta, of the product
+        const float q_inv = fabsf(DK ? p.q.inv[y_at] : p.k.inv[y_at]), g_inv = fabsf(DK ? p.g.inv[y_at] : p.v.inv[y_at]);
+        const DsScale ds = DK ? ds_scale(p.g.len[y_at], vmax) : row_scale;
+        if (!mbar_wait(&b_y1free[s1], phase1, abort_flag)) break;
+        notes[s1].f = make_float4(s_x * q_inv, g_inv * ds.to * fx2, ds.to, q_inv * ds.back);
+        if (DK) {
+          expect_more(&b_y1full[s1], 2 * N * 4);
+          copy_note(notes[s1].v[0], p.lift + y_at * 128 + y % 128, N * 4, &b_y1full[s1]);
+          copy_note(notes[s1].v[1], p.delta + y_at * 128 + y % 128, N * 4, &b_y1full[s1]);
+        }
         load_tile<N, DP>(y1 + s1 * L::kTileY, map_y1, &b_y1full[s1], y, hy);
-        if (j >= N2) ok = mbar_wait(&b_y2free[s2], ((j / N2) - 1) & 1, abort_flag);
-        if (!ok) break;
+        if (!mbar_wait(&b_y2free[s2], phase2, abort_flag)) break;
         load_tile<N, DP>(y2 + s2 * L::kTileY, map_y2, &b_y2full[s2], y, hy);
+        if (++s1 == N1) { s1 = 0; phase1 ^= 1; }
+        if (++s2 == N2) { s2 = 0; phase2 ^= 1; }
+        if (++i == per) { i = 0; ++hy; }
       }
       if (*abort_flag) let_land(bars, 1 + N1 + N2);
     }
@@ -844,11 +909,13 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
       const uint32_t leader = elect_leader();
       constexpr int kPX = plane_bytes<128, DP>(), kPY = plane_bytes<N, DP>();
       bool ok = warp_wait(b_x, 0, abort_flag);
+      uint32_t y1_in = 0, y1_phase = 0, y1_out = 0;
       auto scores = [&](int j) -> bool {      // (buffer j & 1 held dS of tile j - 2, which its product has read)
-        if (!warp_wait(&b_y1full[j % N1], (j / N1) & 1, abort_flag)) return false;
+        if (!warp_wait(&b_y1full[y1_in], y1_phase, abort_flag)) return false;
         if (j >= 2 && !warp_wait(b_o, j & 1, abort_flag)) return false;
         tc_fence_after();
-        const uint32_t d = t_s + (j & 1) * N, x = smem_u32(x1), y = smem_u32(y1 + (j % N1) * L::kTileY);
+        const uint32_t d = t_s + (j & 1) * N, x = smem_u32(x1), y = smem_u32(y1 + y1_in * L::kTileY);
+        if (++y1_in == N1) { y1_in = 0; y1_phase ^= 1; }
         rows_by_rows<N, DP>(leader, d, x + kPX, y, 0);
         rows_by_rows<N, DP>(leader, d, x, y + kPY, 1);
         rows_by_rows<N, DP>(leader, d, x, y, 1);
@@ -874,11 +941,12 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
         tc_fence_after();
         if (j + 1 < n) ok = other(j + 1);
         if (!ok) break;
-        const uint32_t ds = t_s + (j & 1) * N, y = smem_u32(y1 + (j % N1) * L::kTileY);
+        const uint32_t ds = t_s + (j & 1) * N, y = smem_u32(y1 + y1_out * L::kTileY);
         kept_by_cols<N, DP, true>(leader, t_o, ds, y, 0);
         kept_by_cols<N, DP, false>(leader, t_o, ds, y + kPY, 1);
         kept_by_cols<N, DP, false>(leader, t_o, ds, y, 1);
-        commit_by(leader, &b_y1free[j % N1]);
+        commit_by(leader, &b_y1free[y1_out]);
+        if (++y1_out == N1) y1_out = 0;
         commit_by(leader, b_o);
         if (j + 2 < n) ok = scores(j + 2);
       }
@@ -897,71 +965,57 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
       else tmem_st32(t_x2 + at.group * 32 + at.lane_off, reinterpret_cast<const uint32_t*>(w));
       operand_written(b_x2, at.lane);
     }
-    const i64 x_at = (i64)hx * p.tiles + xt;
-    const float s_x = p.scale * kL2e * fabsf(DK ? p.k.inv[x_at] : p.q.inv[x_at]);
-    // 2^e with 2 |do| |v| 2^e below 2^14, and its inverse
-    auto ds_scale = [&](float len, float* inverse) -> float {
-      const float b = 2.0f * len * vmax;
-      int e = b > 0.0f ? 13 - ((int)(__float_as_uint(b) >> 23) - 127) : 0;
-      e = e > 100 ? 100 : (e < -100 ? -100 : e);
-      *inverse = __uint_as_float((uint32_t)(127 - e) << 23);
-      return __uint_as_float((uint32_t)(127 + e) << 23);
-    };
-    float back, f_last = 0.0f, lse_row = 0.0f, delta_row = 0.0f, f2 = 0.0f, fx = DK ? fabsf(p.v.inv[x_at]) : 0.0f;
-    if (!DK) {
-      f2 = ds_scale(p.g.len[x_at], &back) * (1.0f / 16384.0f);      // (p carries 2^14)
-      fx = fabsf(p.g.inv[x_at]) * f2;
-      lse_row = 14.0f - p.lse2[x_at * 128 + at.row];
-      delta_row = -p.delta[x_at * 128 + at.row] * f2;
-    }
-    float acc[W];
+    float lift_row = 0.0f, delta_row = 0.0f;
+    if (!DK) { const i64 r = ((i64)hx * p.tiles + xt) * 128 + at.row; lift_row = p.lift[r]; delta_row = p.delta[r]; }
+    float acc[W], f_last = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
     bool ok = true;
+    int y = y0 * N, s1 = 0;
+    uint32_t phase1 = 0;
     for (int j = 0; j < n; ++j) {
-      const int hy = DK ? h0 + j / per : hk, y = (y0 + (DK ? j % per : j)) * N, c0 = y + at.group * H;
-      const i64 y_at = (i64)hy * p.tiles + y / 128, col = (i64)hy * p.tiles * 128 + c0;
-      const float sc = s_x * fabsf(DK ? p.q.inv[y_at] : p.k.inv[y_at]);
-      float f1, f_this;
-      if (DK) {
-        f2 = ds_scale(p.g.len[y_at], &back) * (1.0f / 16384.0f);
-        f1 = fabsf(p.g.inv[y_at]) * f2 * fx;
-        f_this = fabsf(p.q.inv[y_at]) * back;
-      } else {
-        f1 = fx * fabsf(p.v.inv[y_at]);
-        f_this = fabsf(p.k.inv[y_at]) * back;
-      }
+      const int c0 = y + at.group * H;
+      const bool crossed = DK ? y < xt * 128 + 128 || y + N > e_min : y + N > xt * 128 || y < e_max;
+      // (the slot is filled again only after the product of this tile, which waits for this tile's dS)
+      if (!mbar_wait(&b_y1full[s1], phase1, abort_flag)) { ok = false; break; }
+      const Notes<N, 2>& note = notes[s1];
+      const float4 f = note.f;
       if (!mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
       float v[H];
       load_cols<H>(t_s + (j & 1) * N + at.group * H + at.lane_off, v);
-      if (DK) weights_of_cols<H>(v, sc, p.lse2 + col);
-      else weights_of_row<H>(v, sc, lse_row);
-      const bool crossed = DK ? y < xt * 128 + 128 || y + N > e_min : y + N > xt * 128 || y < e_max;
+      if (DK) weights_of_cols<H>(v, f.x, note.v[0] + at.group * H);
+      else weights_of_row<H>(v, f.x, lift_row);
       if (!mbar_wait(b_dp, j & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
       {
         float d[H];
         load_cols<H>(t_dp + at.group * H + at.lane_off, d);
-        const float2 f12 = make_float2(f1, f1), f22 = make_float2(-f2, -f2);
-        float2 de = make_float2(delta_row, delta_row);
+        const float2 f1 = make_float2(f.y, f.y), f2 = make_float2(-f.z, -f.z);
+        float2 da = mul2(make_float2(delta_row, delta_row), f2), db = da;
 #pragma unroll
-        for (int i = 0; i < H; i += 2) {
-          if (DK) de = mul2(*reinterpret_cast<const float2*>(p.delta + col + i), f22);
-          const float2 x = mul2(make_float2(v[i], v[i + 1]), fma2(make_float2(d[i], d[i + 1]), f12, de));
-          v[i] = x.x; v[i + 1] = x.y;
+        for (int i = 0; i < H; i += 4) {
+          if (DK) { const float4 e = *reinterpret_cast<const float4*>(note.v[1] + at.group * H + i); da = mul2(lo2(e), f2); db = mul2(hi2(e), f2); }
+          const float2 a = mul2(make_float2(v[i], v[i + 1]), fma2(make_float2(d[i], d[i + 1]), f1, da));
+          const float2 b = mul2(make_float2(v[i + 2], v[i + 3]), fma2(make_float2(d[i + 2], d[i + 3]), f1, db));
+          v[i] = a.x; v[i + 1] = a.y; v[i + 2] = b.x; v[i + 3] = b.y;
         }
       }
       if (crossed) keep_columns<H>(v, (DK ? t : mine) - c0, (DK ? mine - 1 : t) - c0, 0.0f);
+      uint32_t r[H];
+      split_operand<H>(v, r);
       // (a quarter's dS lies within its own quarter of S)
-      store_operand<H>(t_s + (j & 1) * N + at.group * H + at.lane_off, v);
+      store_operand<H>(t_s + (j & 1) * N + at.group * H + at.lane_off, r);
       if (j > 0) {
         if (!mbar_wait(b_o, (j - 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
       }
       operand_written(b_ds, at.lane);
-      f_last = f_this;
+      f_last = f.w;
+      if (++s1 == N1) { s1 = 0; phase1 ^= 1; }
+      y += N;
+      if (DK && y == (y0 + per) * N) y = y0 * N;
     }
     if (ok && n > 0) {
       ok = mbar_wait(b_o, (n - 1) & 1, abort_flag);
@@ -990,12 +1044,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward(const __grid_constant_
   else if (b < 2 * keys) grad_v<DP>(smem, maps, p, b - keys);
   else grad_qk<DP, false>(smem, maps, p, b - 2 * keys);
 }
+__device__ __forceinline__ float plus(float a, float b) { return a + b; }
+__device__ __forceinline__ float4 plus(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 // the parts of dK and dV added in order
-__global__ void __launch_bounds__(256) k_add_parts(const float* __restrict__ a, const float* __restrict__ b, float* __restrict__ oa, float* __restrict__ ob, i64 n, int parts) {
+template <class V>
+__global__ void __launch_bounds__(256) k_add_parts(const V* __restrict__ a, const V* __restrict__ b, V* __restrict__ oa, V* __restrict__ ob, i64 n, int parts) {
   for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (i64)gridDim.x * 256) {
-    const float* src = i < n ? a + i : b + (i - n);
-    float s = src[0];
-    for (int k = 1; k < parts; ++k) s += src[(i64)k * n];
+    const V* src = i < n ? a + i : b + (i - n);
+    V s = src[0];
+    for (int k = 1; k < parts; ++k) s = plus(s, src[(i64)k * n]);
     if (i < n) oa[i] = s; else ob[i - n] = s;
   }
 }
@@ -1043,7 +1100,7 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
     inv[i] = take((size_t)heads[i] * tiles * 4); len[i] = take((size_t)heads[i] * tiles * 4); bad[i] = take((size_t)heads[i] * tiles * 16);
   }
   const size_t begin = take((size_t)s.T * 4), end = take((size_t)s.T * 4), ranges = take((size_t)tiles * sizeof(int4)), order = take((size_t)tiles * 8);
-  const size_t delta = o ? take((size_t)s.hq * tiles * 512) : 0, lse2 = o ? take((size_t)s.hq * tiles * 512) : 0;
+  const size_t delta = o ? take((size_t)s.hq * tiles * 512) : 0, lift = o ? take((size_t)s.hq * tiles * 512) : 0;
   VB_TRY(scratch_alloc(at, &w.hold.p));
   uint8_t* base = (uint8_t*)w.hold.p;
   PrepareDev& d = w.prep;
@@ -1058,10 +1115,10 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
   }
   d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.ranges = (int4*)(base + ranges); d.order = (int*)(base + order); d.err = ctx().d_err;
   if (o) { d.o = o->p; d.o_st = o->st; d.o_sh = o->sh; d.lse = lse;
-           d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lse2 = (float*)(base + lse2); }
+           d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lift = (float*)(base + lift); }
   AttnParams& p = w.p;
   p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.scale = s.scale;
-  p.begin = d.begin; p.end = d.end; p.ranges = d.ranges; p.order = d.order; p.lse2 = d.lse2; p.delta = d.delta; p.err = ctx().d_err;
+  p.begin = d.begin; p.end = d.end; p.ranges = d.ranges; p.order = d.order; p.lift = d.lift; p.delta = d.delta; p.err = ctx().d_err;
   ProfScope prof("segment_attn_prepare", 8.0 * (double)s.T * all * s.dk);
   if (dp == 64) k_prepare<64><<<dim3(tiles + 1, all), 256, 0, ctx().stream>>>(d);
   else k_prepare<128><<<dim3(tiles + 1, all), 256, 0, ctx().stream>>>(d);
@@ -1118,8 +1175,12 @@ int backward(Work& w, float* dq, float* dk, float* dv) {
   }
   VB_TRY(launch_early(k_backward<DP>, (unsigned)(p.tiles * (2 * p.hk * p.parts + p.hq)), kSmem, m, p));
   if (p.parts > 1) {
-    const i64 ctas = (2 * n + 1023) / 1024, cap = (i64)ctx().sm_count * 8;
-    k_add_parts<<<(unsigned)(ctas < cap ? ctas : cap), 256, 0, ctx().stream>>>(p.dk_, p.dv, dk, dv, n, p.parts);
+    const i64 cap = (i64)ctx().sm_count * 8;
+    const bool vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15) == 0;
+    const i64 m = vec ? n / 4 : n, ctas = (2 * m + 255) / 256;
+    const unsigned grid = (unsigned)(ctas < cap ? ctas : cap);
+    if (vec) k_add_parts<<<grid, 256, 0, ctx().stream>>>((const float4*)p.dk_, (const float4*)p.dv, (float4*)dk, (float4*)dv, m, p.parts);
+    else k_add_parts<<<grid, 256, 0, ctx().stream>>>((const float*)p.dk_, (const float*)p.dv, dk, dv, m, p.parts);
     VB_LAUNCH_CHECK();
   }
   return VB_OK;
