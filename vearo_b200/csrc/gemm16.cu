@@ -25,7 +25,7 @@ constexpr float kGradScale = 16384.0f;
 
 // ---- splitting ------------------------------------------------------------------------------------------------------------------
 struct SplitDev { const float* x; const int* keep; __half* planes; float* inv; i64 rows, cols, ld, plane, inv_ld; int cb, blocks; bool vec, by_row; };
-struct SplitJobs { SplitDev job[3]; };
+struct SplitJobs { SplitDev job[3]; TargetRows rows; int* err; };
 __global__ void __launch_bounds__(256) k_split16(const __grid_constant__ SplitJobs jobs) {
   __shared__ float red[8];
   int blk = blockIdx.x, which = 0;
@@ -34,6 +34,11 @@ __global__ void __launch_bounds__(256) k_split16(const __grid_constant__ SplitJo
   const int rb = blk / j.cb, cbi = blk - rb * j.cb;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const i64 c0 = (i64)cbi * 128 + lane * 4;
+  if (jobs.rows.targets && which == 0 && cbi == 0) {
+    const i64 r = (i64)rb * 128 + threadIdx.x;
+    if (threadIdx.x < 128 && r < j.rows) jobs.rows.out[r] = read_target(jobs.rows.targets[r], jobs.rows.ignore, jobs.rows.vocab, jobs.err);
+    if (rb == 0 && threadIdx.x < jobs.rows.n_zero) jobs.rows.zero[threadIdx.x] = 0;
+  }
   float4 v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {      // (a warp has whole rows of the block)
@@ -136,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (WHAT == Tile16::RowStats) wait_for_last_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.prob[0].tiles + p.prob[1].tiles;
   // the i-th tile of the CTA for a whole warp; false where there are no more (or a wait ran out)
@@ -433,6 +439,7 @@ int launch(const Params& p, int ctas) {
     VB_CUDA(cudaFuncSetAttribute(k_gemm16<WHAT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     ready = true;
   }
+  if (WHAT == Tile16::RowStats) return launch_early(k_gemm16<WHAT>, dim3(ctas), dim3(kThreads), kSmem, p);
   k_gemm16<WHAT><<<ctas, kThreads, kSmem, ctx().stream>>>(p);
   VB_LAUNCH_CHECK();
   return VB_OK;
@@ -448,8 +455,10 @@ Split16 split16_at(void* mem, i64 rows, i64 cols, bool by_row) {
   return s;
 }
 
-int launch_split16(const SplitJob* jobs, int n) {
+int launch_split16(const SplitJob* jobs, int n, const TargetRows* rows) {
   SplitJobs d{};
+  if (rows) d.rows = *rows;
+  d.err = ctx().d_err;
   double bytes = 0.0;
   i64 all = 0;
   for (int i = 0; i < n; ++i) {

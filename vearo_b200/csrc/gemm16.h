@@ -17,7 +17,9 @@ inline size_t split16_bytes(i64 rows, i64 cols, bool by_row = false) {
 Split16 split16_at(void* mem, i64 rows, i64 cols, bool by_row = false);                           // lays the pair out in memory of that size
 constexpr int kNoTarget = -(1 << 30);
 struct SplitJob { const float* x; Split16 to; const int* keep = nullptr; };                       // x: [rows, cols] contiguous; keep[row] == kNoTarget: read as 0
-int launch_split16(const SplitJob* jobs, int n);                                                  // n <= 3, one launch
+// Target columns given as floats, one a row of the first job: as integers to `out`.  `zero`: ints that the launch sets to 0.
+struct TargetRows { const float* targets; i64 ignore, vocab; int* out; int* zero; int n_zero; };
+int launch_split16(const SplitJob* jobs, int n, const TargetRows* rows = nullptr);                // n <= 3, one launch
 
 // What a product does with its tiles.
 enum class Tile16 {
@@ -42,7 +44,8 @@ struct Product16 {
   const float* lse;                              // [M]
   Split16 grad;                                  // [M, N]
 };
-// n <= 2 (Store), independent of one another, one launch; counter: an int on the device that is 0 when the launch begins
+// n <= 2 (Store), independent of one another, one launch; counter: an int on the device that is 0 when the launch begins.  The RowStats
+// kernel may start while the kernel ahead of it runs and waits for it by itself.
 int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter);
 
 }  // namespace vb

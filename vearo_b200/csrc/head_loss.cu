@@ -9,18 +9,12 @@
 // adds the piece to dx and writes its rows of dW.  Tensor-bound: 2 N V D and 6 N V D operations, three instructions each (gemm16.cu).
 #include "gemm16.h"
 #include "head_loss.h"
+#include "split16.cuh"
 
 namespace vb {
 namespace {
 
-// Target columns as integers.  Rows whose target is `ignore` are left out; a negative or too large one is reported and left out.
-__device__ __forceinline__ int read_target(float v, i64 ignore, i64 vocab, int* err) {
-  if (v == (float)ignore || (fabsf(v) < 1e9f && (i64)roundf(v) == ignore)) return kNoTarget;
-  if (!(v > -0.5f)) { atomicOr(err, ERRBIT_NEG_ID); return kNoTarget; }
-  if (!(roundf(v) < (float)vocab)) { atomicOr(err, ERRBIT_OOB_ID); return kNoTarget; }
-  return (int)roundf(v);
-}
-// One CTA: every row's target, the products' tile counters and, for the backward pass, coef = g / (rows with a target).
+// Backward, one CTA: every row's target, the products' tile counters and coef = g / (rows with a target).
 __global__ void __launch_bounds__(1024) k_targets(const float* __restrict__ targets, i64 n, i64 ignore, i64 vocab, int* __restrict__ out,
                                                   const float* __restrict__ g, float* __restrict__ coef, int* counters, int n_counters, int* err) {
   __shared__ int red[32];
@@ -31,7 +25,6 @@ __global__ void __launch_bounds__(1024) k_targets(const float* __restrict__ targ
     out[i] = t;
     live += t != kNoTarget;
   }
-  if (!coef) return;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) live += __shfl_xor_sync(0xffffffffu, live, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = live;
@@ -42,10 +35,13 @@ __global__ void __launch_bounds__(1024) k_targets(const float* __restrict__ targ
     *coef = *g / (float)(c > 0 ? c : 1);
   }
 }
-// lse and the row's loss from its pairs: 32 rows x 32 pair lanes a CTA, pairs joined in a fixed order
+// lse and the row's loss from its pairs: 32 rows x 32 pair lanes a CTA, pairs joined in a fixed order; the CTA that ends last takes the
+// mean over the rows, in a fixed order too.  (As a kernel of its own the mean cost 3 us of 28 at 512 x 256 x 8192.)
 __global__ void __launch_bounds__(1024) k_join_stats(const float2* __restrict__ stats, const float* __restrict__ target_value, const int* __restrict__ target,
-                                                     float* __restrict__ lse, float* __restrict__ nll, int n, int pairs) {
+                                                     float* __restrict__ lse, float* nll, float* __restrict__ loss, int* ticket, int n, int pairs) {
   __shared__ float sm[32][33], ss[32][33];
+  __shared__ bool last;
+  wait_for_last_kernel();
   const int row = blockIdx.x * 32 + threadIdx.x;
   float m = -INFINITY, s = 0.0f;
   if (row < n) {
@@ -70,23 +66,27 @@ __global__ void __launch_bounds__(1024) k_join_stats(const float2* __restrict__ 
     const float l = top + logf(s);
     lse[r] = l;
     nll[r] = target[r] == kNoTarget ? 0.0f : l - target_value[r];
+    __threadfence();
   }
-}
-__global__ void __launch_bounds__(1024) k_mean_loss(const float* __restrict__ nll, const int* __restrict__ target, i64 n, float* __restrict__ loss) {
-  __shared__ float red[32];
-  __shared__ int cnt[32];
-  float s = 0.0f;
-  int live = 0;
-  for (i64 i = threadIdx.x; i < n; i += 1024) { s += nll[i]; live += target[i] != kNoTarget; }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) { s += __shfl_xor_sync(0xffffffffu, s, o); live += __shfl_xor_sync(0xffffffffu, live, o); }
-  if ((threadIdx.x & 31) == 0) { red[threadIdx.x >> 5] = s; cnt[threadIdx.x >> 5] = live; }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    float t = 0.0f;
+  const int tid = threadIdx.y * 32 + threadIdx.x;
+  if (tid == 0) { last = atomicAdd(ticket, 1) == (int)gridDim.x - 1; __threadfence(); }
+  __syncthreads();
+  if (!last) return;
+  float* sums = &sm[0][0];
+  int* counts = (int*)&ss[0][0];
+  float t = 0.0f;
+  int live = 0;
+  for (int i = tid; i < n; i += 1024) { t += __ldcg(nll + i); live += target[i] != kNoTarget; }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { t += __shfl_xor_sync(0xffffffffu, t, o); live += __shfl_xor_sync(0xffffffffu, live, o); }
+  if (threadIdx.x == 0) { sums[threadIdx.y] = t; counts[threadIdx.y] = live; }
+  __syncthreads();
+  if (tid == 0) {
+    float all = 0.0f;
     int c = 0;
-    for (int i = 0; i < 32; ++i) { t += red[i]; c += cnt[i]; }
-    *loss = c > 0 ? t / (float)c : 0.0f;
+    for (int i = 0; i < 32; ++i) { all += sums[i]; c += counts[i]; }
+    *loss = c > 0 ? all / (float)c : 0.0f;
   }
 }
 
@@ -101,22 +101,17 @@ int launch_head_loss(const float* x, const float* w, const float* targets, i64 i
   VB_TRY(scratch_alloc(split16_bytes(n, d, true), &hx.p));
   VB_TRY(scratch_alloc(split16_bytes(v, d), &hw.p));
   VB_TRY(scratch_alloc((size_t)(pairs * n) * sizeof(float2), &hs.p));
-  VB_TRY(scratch_alloc((size_t)n * 12 + 4, &hr.p));
-  float* nll = (float*)hr.p; float* tv = nll + n; int* tgt = (int*)(tv + n); int* counter = tgt + n;
+  VB_TRY(scratch_alloc((size_t)n * 12 + 8, &hr.p));
+  float* nll = (float*)hr.p; float* tv = nll + n; int* tgt = (int*)(tv + n); int* counters = tgt + n;
   const Split16 sx = split16_at(hx.p, n, d, true), sw = split16_at(hw.p, v, d);
   const SplitJob jobs[2] = {{x, sx}, {w, sw}};
-  VB_TRY(launch_split16(jobs, 2));
-  k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, nullptr, nullptr, counter, 1, ctx().d_err);
-  VB_LAUNCH_CHECK();
+  const TargetRows rows{targets, ignore, v, tgt, counters, 2};
+  VB_TRY(launch_split16(jobs, 2, &rows));
   Product16 g{};
   g.a = Op16{sx, false}; g.b = Op16{sw, false}; g.M = n; g.N = v; g.K = d;
   g.target = tgt; g.stats = (float2*)hs.p; g.target_value = tv;
-  VB_TRY(launch_gemm16(Tile16::RowStats, &g, 1, counter));
-  k_join_stats<<<(unsigned)((n + 31) / 32), dim3(32, 32), 0, ctx().stream>>>((const float2*)hs.p, tv, tgt, lse, nll, (int)n, (int)pairs);
-  VB_LAUNCH_CHECK();
-  k_mean_loss<<<1, 1024, 0, ctx().stream>>>(nll, tgt, n, loss);
-  VB_LAUNCH_CHECK();
-  return VB_OK;
+  VB_TRY(launch_gemm16(Tile16::RowStats, &g, 1, counters));
+  return launch_early(k_join_stats, dim3((unsigned)((n + 31) / 32)), dim3(32, 32), 0, (const float2*)hs.p, tv, tgt, lse, nll, loss, counters + 1, (int)n, (int)pairs);
 }
 
 int launch_head_loss_backward(const float* x, const float* w, const float* targets, i64 ignore, const float* lse, const float* g, float* gx, float* gw,

@@ -394,8 +394,6 @@ __device__ __forceinline__ void keep_columns(float (&v)[W], int first, int last,
 #pragma unroll
   for (int i = 0; i < W; ++i) if (i < first || i > last) v[i] = other;
 }
-// The kernels are launched while k_prepare still runs (programmatic dependent launch): they set up, then wait for what it writes.
-__device__ __forceinline__ void wait_for_prepare() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
@@ -505,7 +503,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
-  wait_for_prepare();
+  wait_for_last_kernel();
   const int qt = p.order[blockIdx.x / p.hq];
   const int4 range = p.ranges[qt];
   const int b_min = range.x, b_max = range.y;
@@ -672,7 +670,7 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
-  wait_for_prepare();
+  wait_for_last_kernel();
   const int kt = p.order[p.tiles + block / p.parts / p.hk];
   const int4 range = p.ranges[kt];
   const int e_min = range.z, e_max = range.w;
@@ -849,7 +847,7 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
-  wait_for_prepare();
+  wait_for_last_kernel();
   const int xt = p.order[(DK ? p.tiles : 0) + rest / x_heads];
   const int4 range = p.ranges[xt];
   const int e_min = DK ? range.z : range.x, e_max = DK ? range.w : range.y;
@@ -1125,18 +1123,6 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
   VB_LAUNCH_CHECK();
   return VB_OK;
 }
-// a kernel that may start while the one ahead of it in the stream still runs
-template <class... P, class... A>
-int launch_early(void (*kernel)(P...), unsigned ctas, int smem, A... args) {
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(ctas); c.blockDim = dim3(kThreads); c.dynamicSmemBytes = (size_t)smem; c.stream = ctx().stream; c.attrs = &at; c.numAttrs = 1;
-  VB_CUDA(cudaLaunchKernelEx(&c, kernel, args...));
-  VB_LAUNCH_CHECK();
-  return VB_OK;
-}
 template <class K>
 int allow_smem(K kernel, int bytes) {
   VB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
@@ -1149,7 +1135,7 @@ int forward(Work& w) {
   VB_TRY(ready);
   CUtensorMap mq, mk, mv;
   VB_TRY(make_map(&mq, w.prep.in[0], w.p.T, DP, 128)); VB_TRY(make_map(&mk, w.prep.in[1], w.p.T, DP, 128)); VB_TRY(make_map(&mv, w.prep.in[2], w.p.T, DP, 128));
-  return launch_early(k_forward<DP>, (unsigned)w.p.hq * w.p.tiles, FwdCfg<DP>::kTotal, mq, mk, mv, w.p);
+  return launch_early(k_forward<DP>, dim3((unsigned)w.p.hq * w.p.tiles), dim3(kThreads), FwdCfg<DP>::kTotal, mq, mk, mv, w.p);
 }
 template <int DP>
 int backward(Work& w, float* dq, float* dk, float* dv) {
@@ -1173,7 +1159,7 @@ int backward(Work& w, float* dq, float* dk, float* dv) {
     VB_TRY(scratch_alloc((size_t)(2 * p.parts * n) * sizeof(float), &hold.p));
     p.dk_ = (float*)hold.p; p.dv = p.dk_ + p.parts * n;
   }
-  VB_TRY(launch_early(k_backward<DP>, (unsigned)(p.tiles * (2 * p.hk * p.parts + p.hq)), kSmem, m, p));
+  VB_TRY(launch_early(k_backward<DP>, dim3((unsigned)(p.tiles * (2 * p.hk * p.parts + p.hq))), dim3(kThreads), kSmem, m, p));
   if (p.parts > 1) {
     const i64 cap = (i64)ctx().sm_count * 8;
     const bool vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15) == 0;

@@ -13,6 +13,7 @@
 #pragma once
 #include <cuda_fp16.h>
 #include "common.h"
+#include "gemm16.h"
 #include "tc_util.cuh"
 
 namespace vb {
@@ -99,4 +100,26 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 }
 
 }  // namespace tc
+
+// A target column as an integer.  A row whose target is `ignore` is left out (kNoTarget); a negative or too large one is reported and left out.
+__device__ __forceinline__ int read_target(float v, i64 ignore, i64 vocab, int* err) {
+  if (v == (float)ignore || (fabsf(v) < 1e9f && (i64)roundf(v) == ignore)) return kNoTarget;
+  if (!(v > -0.5f)) { atomicOr(err, ERRBIT_NEG_ID); return kNoTarget; }
+  if (!(roundf(v) < (float)vocab)) { atomicOr(err, ERRBIT_OOB_ID); return kNoTarget; }
+  return (int)roundf(v);
+}
+// of a kernel launched by launch_early: nothing that the kernel ahead of it in the stream writes is touched before this
+__device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// a launch that may begin while the kernel ahead of it in the stream still runs
+template <class... P, class... A>
+int launch_early(void (*kernel)(P...), dim3 ctas, dim3 threads, int smem, A... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = ctas; c.blockDim = threads; c.dynamicSmemBytes = (size_t)smem; c.stream = ctx().stream; c.attrs = &at; c.numAttrs = 1;
+  VB_CUDA(cudaLaunchKernelEx(&c, kernel, args...));
+  VB_LAUNCH_CHECK();
+  return VB_OK;
+}
 }  // namespace vb
