@@ -66,7 +66,8 @@ int rope_checks(const vb_tensor* q, const vb_tensor* k, const vb_tensor* wq, con
   VB_CHECK(std::isfinite(theta) && theta > 0.0f && std::isfinite(eps) && eps >= 0.0f, "theta must be positive and eps not negative");
   if (dk > 2 * kRopeMaxPairs) return set_error(VB_ERR_UNSUPPORTED, "vb_qk_norm_rope: head sizes up to 512");
   if (T > 0x7fffffff || q->dims[1] + (k ? k->dims[1] : 0) > 65536) return set_error(VB_ERR_UNSUPPORTED, "vb_qk_norm_rope: at most 2^31 - 1 tokens and 65536 heads");
-  for (int j = 0; j < rot_dim / 2; ++j) tab->rev[j] = std::exp(-2.0 * j / rot_dim * std::log((double)theta)) / 6.283185307179586476925286766559;
+  const double step = rot_dim > 0 ? -2.0 / rot_dim * std::log((double)theta) : 0.0;
+  for (int j = 0; j < rot_dim / 2; ++j) tab->rev[j] = std::exp(j * step) / 6.283185307179586476925286766559;
   return VB_OK;
 }
 

@@ -7,17 +7,19 @@
 //
 // HBM-bound: reads each head once and writes it once (backward: reads x and g, writes dx).  Eight lanes own a head, each lane
 // "units" of eight components that hold both members of its pairs (two runs of four, rot/2 apart, or eight neighbours), so the
-// turn needs no exchange and the norm three shuffles; loads and stores are 16 bytes.  A CTA takes a few tokens and computes
-// their cosines and sines once, for all heads.  The angle is formed in turns: position times frequency / 2 pi in 64 bits (the
+// turn needs no exchange and the norm three shuffles; loads and stores are 16 bytes.  A warp takes a token, or 4 HEADS heads of one,
+// queries and keys in one row: it asks for all of them, forms the token's cosines and sines in shared memory while they are on their way,
+// and meets no other warp (CTAs that shared the cosines of a few tokens stood at their barriers: backward at 8192 x 16 heads of 64, 26 us of kernel then, 21 now; its bytes at the rate of a copy: 15).  The angle is formed in turns: position times frequency / 2 pi in 64 bits (the
 // frequencies are 64-bit host values in the kernel's parameters), the fraction of a quarter turn in 32, so far positions lose
 // nothing.  Head sizes, rotated widths or addresses that do not fit the 16-byte units take a scalar kernel, one warp per head.
 #include "common.h"
 #include "qk_norm_rope.h"
+#include "split16.cuh"
 
 namespace vb {
 namespace {
 
-constexpr int kThreads = 256, kLanes = 8, kGroups = kThreads / kLanes;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kLanes = 8, kGroups = kThreads / kLanes;
 
 // cosine and sine of `pos` turns-per-position `rev`, argument reduced to an eighth of a turn before it is rounded to 32 bits
 __device__ __forceinline__ float2 turn_of(double pos, double rev) {
@@ -64,133 +66,74 @@ __device__ __forceinline__ void turn_unit(float4& x, float4& y, const float2* cs
 }
 __device__ __forceinline__ float dot4(float4 a, float4 b) { return a.x * b.x + a.y * b.y + a.z * b.z + a.w * b.w; }
 __device__ __forceinline__ float4 mul4(float4 a, float4 b) { return make_float4(a.x * b.x, a.y * b.y, a.z * b.z, a.w * b.w); }
+__device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
 __device__ __forceinline__ float4 scale4(float4 a, float s) { return make_float4(a.x * s, a.y * s, a.z * s, a.w * s); }
 
-__device__ __forceinline__ void fill_turns(float2* cs, const RopeTable& tab, const float* pos, i64 t0, int nt, int half) {
-  for (int i = threadIdx.x; i < nt * half; i += blockDim.x) {
-    const int t = i / half;
-    cs[i] = turn_of((double)pos[t0 + t], tab.rev[i - t * half]);
-  }
+// cosines and sines of a token, by one warp into its own strip
+__device__ __forceinline__ void fill_turns(float2* cs, const RopeTable& tab, float pos, int half) {
+  for (int j = threadIdx.x & 31; j < half; j += 32) cs[j] = turn_of((double)pos, tab.rev[j]);
+}
+// Head hh of token t where the queries' heads are counted first.
+struct HeadAt { const float* x; int h; bool is_q; };
+__device__ __forceinline__ HeadAt head_at(const HeadView& q, const HeadView& k, i64 t, int hh) {
+  HeadAt a;
+  a.is_q = hh < q.heads;
+  a.h = a.is_q ? hh : hh - q.heads;
+  a.x = a.is_q ? q.p + t * q.st + a.h * q.sh : k.p + t * k.st + a.h * k.sh;
+  return a;
 }
 
-// the heads of one of the two tensors for the CTA's tokens, forward
-template <int UPL, bool INTER>
-__device__ __forceinline__ void forward_heads(const HeadView& x, const float* __restrict__ w, float* __restrict__ out, const float2* cs,
-                                              i64 t0, int nt, int dk, int rot, float eps) {
-  const int lane = threadIdx.x & (kLanes - 1), group = threadIdx.x / kLanes;
-  const int half = rot / 2;
-  float4 wa[UPL], wb[UPL];
-  int oa[UPL], ob[UPL];
-#pragma unroll
-  for (int i = 0; i < UPL; ++i) {
-    const int u = lane + i * kLanes;
-    unit_at<INTER>(u, rot, oa[i], ob[i]);
-    wa[i] = wb[i] = make_float4(0, 0, 0, 0);
-    if (8 * u < dk) { wa[i] = *reinterpret_cast<const float4*>(w + oa[i]); wb[i] = *reinterpret_cast<const float4*>(w + ob[i]); }
-  }
-  const float rdk = 1.0f / (float)dk;
-  const int rows = nt * x.heads;
-  for (int r0 = 0; r0 < rows; r0 += kGroups) {      // (whole groups stay together: the shuffles below name every lane)
-    const int r = r0 + group;
-    const bool live = r < rows;
-    const int t = live ? r / x.heads : 0, h = live ? r - t * x.heads : 0;
-    const float* p = x.p + (t0 + t) * x.st + h * x.sh;
-    float4 a[UPL], b[UPL];
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < UPL; ++i) {
-      a[i] = b[i] = make_float4(0, 0, 0, 0);
-      if (live && 8 * (lane + i * kLanes) < dk) { a[i] = *reinterpret_cast<const float4*>(p + oa[i]); b[i] = *reinterpret_cast<const float4*>(p + ob[i]); }
-      ss += dot4(a[i], a[i]) + dot4(b[i], b[i]);
-    }
-    const float inv = 1.0f / sqrtf(group_sum(ss) * rdk + eps);
-    float* o = out + ((t0 + t) * x.heads + h) * (i64)dk;
-#pragma unroll
-    for (int i = 0; i < UPL; ++i) {
-      const int u = lane + i * kLanes;
-      if (!live || 8 * u >= dk) continue;
-      float4 ya = mul4(scale4(a[i], inv), wa[i]), yb = mul4(scale4(b[i], inv), wb[i]);
-      if (8 * u < rot) turn_unit<INTER>(ya, yb, cs + t * half, u, 1.0f);
-      *reinterpret_cast<float4*>(o + oa[i]) = ya;
-      *reinterpret_cast<float4*>(o + ob[i]) = yb;
-    }
-  }
-}
-template <int UPL, bool INTER>
-__global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ RopeTable tab, HeadView q, HeadView k, const float* __restrict__ wq,
+template <int UPL, bool INTER, int HEADS>
+__global__ void __launch_bounds__(kThreads, 4) k_norm_rope(const __grid_constant__ RopeTable tab, HeadView q, HeadView k, const float* __restrict__ wq,
                                                         const float* __restrict__ wk, const float* __restrict__ pos, float* __restrict__ oq,
-                                                        float* __restrict__ ok, i64 tokens, int per_cta, int dk, int rot, float eps) {
-  extern __shared__ float2 cs[];
-  const i64 t0 = (i64)blockIdx.x * per_cta;
-  const int nt = (int)(tokens - t0 < per_cta ? tokens - t0 : per_cta);
-  fill_turns(cs, tab, pos, t0, nt, rot / 2);
-  __syncthreads();
-  forward_heads<UPL, INTER>(q, wq, oq, cs, t0, nt, dk, rot, eps);
-  if (k.p) forward_heads<UPL, INTER>(k, wk, ok, cs, t0, nt, dk, rot, eps);
-}
-
-// ... backward; acc: this lane's sums of g' x-hat over the heads it has seen
-template <int UPL, bool INTER>
-__device__ __forceinline__ void backward_heads(const HeadView& x, const HeadView& g, const float* __restrict__ w, float* __restrict__ gx,
-                                               const float2* cs, i64 t0, int nt, int dk, int rot, float eps, float4 (&acc)[2 * UPL]) {
-  const int lane = threadIdx.x & (kLanes - 1), group = threadIdx.x / kLanes;
-  const int half = rot / 2;
-  const float rdk = 1.0f / (float)dk;
-  const int rows = nt * x.heads;
-  for (int r0 = 0; r0 < rows; r0 += kGroups) {
-    const int r = r0 + group;
-    const bool live = r < rows;
-    const int t = live ? r / x.heads : 0, h = live ? r - t * x.heads : 0;
-    const float* px = x.p + (t0 + t) * x.st + h * x.sh;
-    const float* pg = g.p + (t0 + t) * g.st + h * g.sh;
-    float4 a[UPL], b[UPL], ga[UPL], gb[UPL];
-    float ss = 0.0f;
+                                                        float* __restrict__ ok, i64 tokens, int dk, int rot, float eps) {
+  extern __shared__ float2 turns[];
+  const int lane = threadIdx.x & (kLanes - 1), wid = threadIdx.x >> 5, h0 = blockIdx.y * 4 * HEADS + ((threadIdx.x & 31) >> 3);
+  const i64 t = (i64)blockIdx.x * kWarps + wid;
+  if (t >= tokens) return;
+  const int heads = q.heads + (k.p ? k.heads : 0), half = rot / 2;
+  float4 a[HEADS][UPL], b[HEADS][UPL];
+#pragma unroll
+  for (int n = 0; n < HEADS; ++n) {
+    const HeadAt at = head_at(q, k, t, h0 + 4 * n);
 #pragma unroll
     for (int i = 0; i < UPL; ++i) {
       const int u = lane + i * kLanes;
       int oa, ob;
       unit_at<INTER>(u, rot, oa, ob);
-      a[i] = b[i] = ga[i] = gb[i] = make_float4(0, 0, 0, 0);
-      if (live && 8 * u < dk) {
-        a[i] = *reinterpret_cast<const float4*>(px + oa); b[i] = *reinterpret_cast<const float4*>(px + ob);
-        ga[i] = *reinterpret_cast<const float4*>(pg + oa); gb[i] = *reinterpret_cast<const float4*>(pg + ob);
-      }
-      ss += dot4(a[i], a[i]) + dot4(b[i], b[i]);
+      a[n][i] = b[n][i] = make_float4(0, 0, 0, 0);
+      if (h0 + 4 * n < heads && 8 * u < dk) { a[n][i] = *reinterpret_cast<const float4*>(at.x + oa); b[n][i] = *reinterpret_cast<const float4*>(at.x + ob); }
     }
+  }
+  float2* cs = turns + wid * half;
+  fill_turns(cs, tab, pos[t], half);
+  __syncwarp();
+  const float rdk = 1.0f / (float)dk;
+#pragma unroll
+  for (int n = 0; n < HEADS; ++n) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < UPL; ++i) ss += dot4(a[n][i], a[n][i]) + dot4(b[n][i], b[n][i]);
     const float inv = 1.0f / sqrtf(group_sum(ss) * rdk + eps);
-    float c = 0.0f;
+    if (h0 + 4 * n >= heads) continue;
+    const HeadAt at = head_at(q, k, t, h0 + 4 * n);
+    const float* w = at.is_q ? wq : wk;
+    float* o = (at.is_q ? oq + (t * q.heads + at.h) * (i64)dk : ok + (t * k.heads + at.h) * (i64)dk);
 #pragma unroll
     for (int i = 0; i < UPL; ++i) {
       const int u = lane + i * kLanes;
       if (8 * u >= dk) continue;
-      if (8 * u < rot) turn_unit<INTER>(ga[i], gb[i], cs + t * half, u, -1.0f);
-      a[i] = scale4(a[i], inv); b[i] = scale4(b[i], inv);      // x-hat
-      const float4 pa = mul4(ga[i], a[i]), pb = mul4(gb[i], b[i]);
-      if (live) {
-        acc[2 * i].x += pa.x; acc[2 * i].y += pa.y; acc[2 * i].z += pa.z; acc[2 * i].w += pa.w;
-        acc[2 * i + 1].x += pb.x; acc[2 * i + 1].y += pb.y; acc[2 * i + 1].z += pb.z; acc[2 * i + 1].w += pb.w;
-      }
       int oa, ob;
       unit_at<INTER>(u, rot, oa, ob);
-      ga[i] = mul4(ga[i], *reinterpret_cast<const float4*>(w + oa)); gb[i] = mul4(gb[i], *reinterpret_cast<const float4*>(w + ob));
-      c += dot4(ga[i], a[i]) + dot4(gb[i], b[i]);
+      float4 ya = mul4(scale4(a[n][i], inv), *reinterpret_cast<const float4*>(w + oa)), yb = mul4(scale4(b[n][i], inv), *reinterpret_cast<const float4*>(w + ob));
+      if (8 * u < rot) turn_unit<INTER>(ya, yb, cs, u, 1.0f);
+      *reinterpret_cast<float4*>(o + oa) = ya;
+      *reinterpret_cast<float4*>(o + ob) = yb;
     }
-    c = group_sum(c) * rdk;
-    float* o = gx + ((t0 + t) * x.heads + h) * (i64)dk;
-#pragma unroll
-    for (int i = 0; i < UPL; ++i) {
-      const int u = lane + i * kLanes;
-      if (!live || 8 * u >= dk) continue;
-      int oa, ob;
-      unit_at<INTER>(u, rot, oa, ob);
-      float4 ra, rb;
-      ra.x = (ga[i].x - a[i].x * c) * inv; ra.y = (ga[i].y - a[i].y * c) * inv; ra.z = (ga[i].z - a[i].z * c) * inv; ra.w = (ga[i].w - a[i].w * c) * inv;
-      rb.x = (gb[i].x - b[i].x * c) * inv; rb.y = (gb[i].y - b[i].y * c) * inv; rb.z = (gb[i].z - b[i].z * c) * inv; rb.w = (gb[i].w - b[i].w * c) * inv;
-      *reinterpret_cast<float4*>(o + oa) = ra;
-      *reinterpret_cast<float4*>(o + ob) = rb;
-    }
+    __syncwarp(0xffu << (threadIdx.x & 24));
   }
 }
+
 // the CTA's sums for one weight: lanes of equal position in all groups, added in group order
 template <int UPL, bool INTER>
 __device__ __forceinline__ void store_weight_sums(const float4 (&acc)[2 * UPL], float* part, float* sm, int dk, int rot) {
@@ -213,28 +156,88 @@ __device__ __forceinline__ void store_weight_sums(const float4 (&acc)[2 * UPL], 
     }
   }
 }
-template <int UPL, bool INTER>
-__global__ void __launch_bounds__(kThreads) k_norm_rope_bwd(const __grid_constant__ RopeTable tab, HeadView q, HeadView k, HeadView gq, HeadView gk,
+template <int UPL, bool INTER, int HEADS>
+__global__ void __launch_bounds__(kThreads, UPL == 1 ? 3 : UPL == 2 ? 2 : 1) k_norm_rope_bwd(const __grid_constant__ RopeTable tab, HeadView q, HeadView k, HeadView gq, HeadView gk,
                                                             const float* __restrict__ wq, const float* __restrict__ wk, const float* __restrict__ pos,
                                                             float* __restrict__ dq, float* __restrict__ dkeys, float* __restrict__ part,
-                                                            i64 tokens, int per_cta, int dk, int rot, float eps) {
-  extern __shared__ float2 cs[];
+                                                            i64 tokens, int dk, int rot, float eps) {
+  extern __shared__ float2 turns[];
   __shared__ __align__(16) float sums[kGroups * 64];
-  float4 accq[2 * UPL], acck[2 * UPL];
+  const int lane = threadIdx.x & (kLanes - 1), wid = threadIdx.x >> 5, h0 = blockIdx.y * 4 * HEADS + ((threadIdx.x & 31) >> 3);
+  const int heads = q.heads + (k.p ? k.heads : 0), half = rot / 2;
+  float2* cs = turns + wid * half;
+  const float rdk = 1.0f / (float)dk;
+  float4 accq[2 * UPL], acck[2 * UPL];      // this lane's sums of g' x-hat over the heads it has seen
 #pragma unroll
   for (int i = 0; i < 2 * UPL; ++i) accq[i] = acck[i] = make_float4(0, 0, 0, 0);
-  for (i64 t0 = (i64)blockIdx.x * per_cta; t0 < tokens; t0 += (i64)gridDim.x * per_cta) {
-    const int nt = (int)(tokens - t0 < per_cta ? tokens - t0 : per_cta);
-    __syncthreads();
-    fill_turns(cs, tab, pos, t0, nt, rot / 2);
-    __syncthreads();
-    backward_heads<UPL, INTER>(q, gq, wq, dq, cs, t0, nt, dk, rot, eps, accq);
-    if (k.p) backward_heads<UPL, INTER>(k, gk, wk, dkeys, cs, t0, nt, dk, rot, eps, acck);
+  for (i64 t = (i64)blockIdx.x * kWarps + wid; t < tokens; t += (i64)gridDim.x * kWarps) {
+    float4 a[HEADS][UPL], b[HEADS][UPL], ga[HEADS][UPL], gb[HEADS][UPL];
+#pragma unroll
+    for (int n = 0; n < HEADS; ++n) {
+      const float *px = head_at(q, k, t, h0 + 4 * n).x, *pg = head_at(gq, gk, t, h0 + 4 * n).x;
+#pragma unroll
+      for (int i = 0; i < UPL; ++i) {
+        const int u = lane + i * kLanes;
+        int oa, ob;
+        unit_at<INTER>(u, rot, oa, ob);
+        a[n][i] = b[n][i] = ga[n][i] = gb[n][i] = make_float4(0, 0, 0, 0);
+        if (h0 + 4 * n < heads && 8 * u < dk) {
+          a[n][i] = *reinterpret_cast<const float4*>(px + oa); b[n][i] = *reinterpret_cast<const float4*>(px + ob);
+          ga[n][i] = *reinterpret_cast<const float4*>(pg + oa); gb[n][i] = *reinterpret_cast<const float4*>(pg + ob);
+        }
+      }
+    }
+    __syncwarp();      // (the last token's cosines have been read)
+    fill_turns(cs, tab, pos[t], half);
+    __syncwarp();
+#pragma unroll
+    for (int n = 0; n < HEADS; ++n) {
+      const bool live = h0 + 4 * n < heads;      // (a head that is not there is all zeros: it adds nothing)
+      const HeadAt at = head_at(q, k, t, live ? h0 + 4 * n : 0);
+      const float* w = at.is_q ? wq : wk;
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < UPL; ++i) ss += dot4(a[n][i], a[n][i]) + dot4(b[n][i], b[n][i]);
+      const float inv = 1.0f / sqrtf(group_sum(ss) * rdk + eps);
+      float c = 0.0f;
+#pragma unroll
+      for (int i = 0; i < UPL; ++i) {
+        const int u = lane + i * kLanes;
+        if (8 * u >= dk) continue;
+        float4 &xa = a[n][i], &xb = b[n][i], &ya = ga[n][i], &yb = gb[n][i];
+        if (8 * u < rot) turn_unit<INTER>(ya, yb, cs, u, -1.0f);
+        xa = scale4(xa, inv); xb = scale4(xb, inv);      // x-hat
+        const float4 pa = mul4(ya, xa), pb = mul4(yb, xb);
+        if (live) {
+          if (at.is_q) { accq[2 * i] = add4(accq[2 * i], pa); accq[2 * i + 1] = add4(accq[2 * i + 1], pb); }
+          else { acck[2 * i] = add4(acck[2 * i], pa); acck[2 * i + 1] = add4(acck[2 * i + 1], pb); }
+        }
+        int oa, ob;
+        unit_at<INTER>(u, rot, oa, ob);
+        ya = mul4(ya, *reinterpret_cast<const float4*>(w + oa)); yb = mul4(yb, *reinterpret_cast<const float4*>(w + ob));
+        c += dot4(ya, xa) + dot4(yb, xb);
+      }
+      c = group_sum(c) * rdk;
+      if (live) {
+        float* o = at.is_q ? dq + (t * q.heads + at.h) * (i64)dk : dkeys + (t * k.heads + at.h) * (i64)dk;
+#pragma unroll
+        for (int i = 0; i < UPL; ++i) {
+          const int u = lane + i * kLanes;
+          if (8 * u >= dk) continue;
+          int oa, ob;
+          unit_at<INTER>(u, rot, oa, ob);
+          *reinterpret_cast<float4*>(o + oa) = scale4(add4(ga[n][i], scale4(a[n][i], -c)), inv);
+          *reinterpret_cast<float4*>(o + ob) = scale4(add4(gb[n][i], scale4(b[n][i], -c)), inv);
+        }
+      }
+      __syncwarp();
+    }
   }
   // partial sums: one row of [dk] (queries) and, where there are keys, one more behind it per CTA
   const int width = k.p ? 2 * dk : dk;
-  store_weight_sums<UPL, INTER>(accq, part + (i64)blockIdx.x * width, sums, dk, rot);
-  if (k.p) store_weight_sums<UPL, INTER>(acck, part + (i64)blockIdx.x * width + dk, sums, dk, rot);
+  part += ((i64)blockIdx.y * gridDim.x + blockIdx.x) * width;
+  store_weight_sums<UPL, INTER>(accq, part, sums, dk, rot);
+  if (k.p) store_weight_sums<UPL, INTER>(acck, part + dk, sums, dk, rot);
 }
 
 // ---- any head size, rotated width and alignment: one warp per head, components in 32-bit accesses -----------------------------
@@ -338,6 +341,7 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope_bwd_any(const __grid_con
 __global__ void __launch_bounds__(1024) k_weight_sums(const float* __restrict__ part, float* __restrict__ gwq, float* __restrict__ gwk, int dk,
                                                       int width, int ctas) {
   __shared__ float sm[32][33];
+  wait_for_last_kernel();
   const int c = (int)blockIdx.x * 32 + threadIdx.x;
   float s = 0.0f;
   if (c < width) for (int i = threadIdx.y; i < ctas; i += 32) s += part[(i64)i * width + c];
@@ -354,14 +358,6 @@ __global__ void __launch_bounds__(1024) k_weight_sums(const float* __restrict__ 
 bool aligned16(const HeadView& v) { return !v.p || ((reinterpret_cast<uintptr_t>(v.p) & 15) == 0 && v.st % 4 == 0 && v.sh % 4 == 0); }
 bool aligned16(const float* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// tokens a CTA takes: enough heads for every group of lanes, at most 8 KB of cosines and sines
-int tokens_per_cta(int heads, int rot) {
-  int n = (2 * kGroups + heads - 1) / heads;
-  const int cap = rot > 0 ? 2048 / rot : 64;
-  if (n > cap) n = cap;
-  return n < 1 ? 1 : n;
-}
-
 }  // namespace
 
 int launch_norm_rope(const RopeTable& tab, const HeadView& q, const HeadView& k, const float* wq, const float* wk, const float* pos,
@@ -369,16 +365,18 @@ int launch_norm_rope(const RopeTable& tab, const HeadView& q, const HeadView& k,
   const int heads = q.heads + (k.p ? k.heads : 0);
   ProfScope prof("norm_rope", 8.0 * (double)tokens * heads * dk);
   if (dk % 8 == 0 && dk <= 256 && rot % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(wq) && (!wk || aligned16(wk))) {
-    const int per = tokens_per_cta(heads, rot);
-    const i64 ctas = (tokens + per - 1) / per;
-    const size_t smem = (size_t)per * (rot / 2) * sizeof(float2);
-#define GO(U, I) k_norm_rope<U, I><<<(unsigned)ctas, kThreads, smem, ctx().stream>>>(tab, q, k, wq, wk, pos, oq, ok, tokens, per, dk, rot, eps)
+    const size_t smem = (size_t)kWarps * (rot / 2) * sizeof(float2);
+    // heads a group of lanes: as many as keep 128 bytes of a lane on their way, one where a warp's four groups hold all heads at once
+#define GO(U, I, H) k_norm_rope<U, I, H><<<dim3((unsigned)((tokens + kWarps - 1) / kWarps), (unsigned)((heads + 4 * H - 1) / (4 * H))), kThreads, smem, ctx().stream>>>( \
+    tab, q, k, wq, wk, pos, oq, ok, tokens, dk, rot, eps)
+#define GO_BY(U, I, H) do { if (H > 1 && heads <= 4) GO(U, I, 1); else GO(U, I, H); } while (0)
     switch ((dk + 63) / 64) {
-      case 1: if (inter) GO(1, true); else GO(1, false); break;
-      case 2: if (inter) GO(2, true); else GO(2, false); break;
-      case 3: if (inter) GO(3, true); else GO(3, false); break;
-      default: if (inter) GO(4, true); else GO(4, false); break;
+      case 1: if (inter) GO_BY(1, true, 4); else GO_BY(1, false, 4); break;
+      case 2: if (inter) GO_BY(2, true, 2); else GO_BY(2, false, 2); break;
+      case 3: if (inter) GO(3, true, 1); else GO(3, false, 1); break;
+      default: if (inter) GO(4, true, 1); else GO(4, false, 1); break;
     }
+#undef GO_BY
 #undef GO
   } else {
     i64 ctas = (tokens * heads + kThreads / 32 - 1) / (kThreads / 32), cap = (i64)ctx().sm_count * 8;
@@ -397,18 +395,24 @@ int launch_norm_rope_backward(const RopeTable& tab, const HeadView& q, const Hea
   {
     ProfScope prof("norm_rope_bwd", 12.0 * (double)tokens * heads * dk);
     if (dk % 8 == 0 && dk <= 256 && rot % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(gq) && aligned16(gk) && aligned16(wq) && (!wk || aligned16(wk))) {
-      const int per = tokens_per_cta(heads, rot);
-      const i64 want = (tokens + per - 1) / per, cap = (i64)ctx().sm_count * 4;
-      ctas = (int)(want < cap ? want : cap);
-      const size_t smem = (size_t)per * (rot / 2) * sizeof(float2);
-      VB_TRY(scratch_alloc((size_t)ctas * width * sizeof(float), &hold.p));
-#define GO(U, I) k_norm_rope_bwd<U, I><<<(unsigned)ctas, kThreads, smem, ctx().stream>>>(tab, q, k, gq, gk, wq, wk, pos, dq, dkeys, (float*)hold.p, tokens, per, dk, rot, eps)
+      const size_t smem = (size_t)kWarps * (rot / 2) * sizeof(float2);
+      const i64 want = (tokens + kWarps - 1) / kWarps;
+#define GO(U, I, H) do { \
+    const unsigned rows = (unsigned)((heads + 4 * H - 1) / (4 * H)); \
+    const i64 cap = (i64)ctx().sm_count * (U == 1 ? 3 : U == 2 ? 2 : 1) / rows > 0 ? (i64)ctx().sm_count * (U == 1 ? 3 : U == 2 ? 2 : 1) / rows : 1; \
+    const unsigned cols = (unsigned)(want < cap ? want : cap); \
+    ctas = (int)(rows * cols); \
+    VB_TRY(scratch_alloc((size_t)ctas * width * sizeof(float), &hold.p)); \
+    k_norm_rope_bwd<U, I, H><<<dim3(cols, rows), kThreads, smem, ctx().stream>>>(tab, q, k, gq, gk, wq, wk, pos, dq, dkeys, (float*)hold.p, tokens, dk, rot, eps); \
+  } while (0)
+#define GO_BY(U, I, H) do { if (H > 1 && heads <= 4) GO(U, I, 1); else GO(U, I, H); } while (0)
       switch ((dk + 63) / 64) {
-        case 1: if (inter) GO(1, true); else GO(1, false); break;
-        case 2: if (inter) GO(2, true); else GO(2, false); break;
-        case 3: if (inter) GO(3, true); else GO(3, false); break;
-        default: if (inter) GO(4, true); else GO(4, false); break;
+        case 1: if (inter) GO_BY(1, true, 2); else GO_BY(1, false, 2); break;
+        case 2: if (inter) GO(2, true, 1); else GO(2, false, 1); break;
+        case 3: if (inter) GO(3, true, 1); else GO(3, false, 1); break;
+        default: if (inter) GO(4, true, 1); else GO(4, false, 1); break;
       }
+#undef GO_BY
 #undef GO
     } else {
       const i64 want = (tokens * heads + kThreads / 32 - 1) / (kThreads / 32), cap = (i64)ctx().sm_count * 4;
@@ -419,9 +423,7 @@ int launch_norm_rope_backward(const RopeTable& tab, const HeadView& q, const Hea
     }
     VB_LAUNCH_CHECK();
   }
-  k_weight_sums<<<(unsigned)((width + 31) / 32), dim3(32, 32), 0, ctx().stream>>>((const float*)hold.p, gwq, gwk, dk, width, ctas);
-  VB_LAUNCH_CHECK();
-  return VB_OK;
+  return launch_early(k_weight_sums, dim3((unsigned)((width + 31) / 32)), dim3(32, 32), 0, (const float*)hold.p, gwq, gwk, dk, width, ctas);
 }
 
 }  // namespace vb
