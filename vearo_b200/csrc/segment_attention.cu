@@ -48,27 +48,27 @@ struct PrepareDev {
 };
 
 // The offset of the segment that row t is in (-1: none), as an index into the offsets.
-__device__ __forceinline__ int segment_of(const PrepareDev& p, int t) {
+__device__ __forceinline__ int segment_of(const PrepareDev& p, const float* starts, int t) {
   int lo = 0, hi = p.n_seg + 1;          // offsets [0, lo) are <= t
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (roundf(p.starts[mid]) <= (float)t) lo = mid + 1; else hi = mid;
+    if (roundf(starts[mid]) <= (float)t) lo = mid + 1; else hi = mid;
   }
   return lo > 0 && lo <= p.n_seg ? lo - 1 : -1;
 }
 // Where the segment of row t begins and ends (rows of no segment: an empty range).  Offsets that decrease or leave [0, T] are
 // reported; whatever they are, every range stays inside [0, T].
-__device__ __forceinline__ int2 find_segment(const PrepareDev& p, int t) {
+__device__ __forceinline__ int2 find_segment(const PrepareDev& p, const float* starts, int t) {
   for (int i = t; i <= p.n_seg; i += p.tiles * 128) {
-    const float s = p.starts[i];
+    const float s = starts[i];
     if (!(s > -0.5f)) atomicOr(p.err, ERRBIT_NEG_ID);
-    else if (!(s < (float)p.T + 0.5f) || (i > 0 && !(p.starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
+    else if (!(s < (float)p.T + 0.5f) || (i > 0 && !(starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
   }
   if (t >= p.T) return make_int2(p.T, 0);
   int b = p.T, e = 0;
-  const int s = segment_of(p, t);
+  const int s = segment_of(p, starts, t);
   if (s >= 0) {
-    const float fb = roundf(p.starts[s]), fe = roundf(p.starts[s + 1]);
+    const float fb = roundf(starts[s]), fe = roundf(starts[s + 1]);
     b = fb > 0.0f ? (int)fb : 0;
     e = fe < (float)p.T ? (int)fe : p.T;
     if (!(b <= t && t < e)) { b = p.T; e = 0; }
@@ -78,52 +78,81 @@ __device__ __forceinline__ int2 find_segment(const PrepareDev& p, int t) {
 }
 
 // Tiles in the order of the work that their rows have ahead of them (which = 0: as queries, how far back their segment begins; 1: as keys,
-// how far on it ends), the most first: a sort by count into 1024 classes.
-__device__ void plan_order(const PrepareDev& p, int which, int* classes) {
+// how far on it ends), the most first: a sort by count into 1024 classes, four a thread.  (Tiles of a class come in any order: it
+// decides when a tile is worked on, not how.)
+constexpr int kClasses = 1024;
+__device__ void plan_order(const PrepareDev& p, const float* starts, int which, int* classes, int* warp_sums) {
   int* order = p.order + which * p.tiles;
-  for (int i = threadIdx.x; i < 1024; i += 256) classes[i] = 0;
+  *reinterpret_cast<int4*>(classes + threadIdx.x * 4) = make_int4(0, 0, 0, 0);
   __syncthreads();
   auto class_of = [&](int tile) -> int {
-    const int t = which == 0 ? tile * 128 : min(p.T - 1, tile * 128 + 127), s = segment_of(p, t);
+    const int t = which == 0 ? tile * 128 : min(p.T - 1, tile * 128 + 127), s = segment_of(p, starts, t);
     int n = 0;
-    if (s >= 0) n = which == 0 ? tile - (int)fmaxf(roundf(p.starts[s]), 0.0f) / 128 : ((int)fminf(roundf(p.starts[s + 1]), (float)p.T) - 1) / 128 - tile;
-    return 1023 - max(0, min(n, 1023));
+    if (s >= 0) n = which == 0 ? tile - (int)fmaxf(roundf(starts[s]), 0.0f) / 128 : ((int)fminf(roundf(starts[s + 1]), (float)p.T) - 1) / 128 - tile;
+    return kClasses - 1 - max(0, min(n, kClasses - 1));
   };
   for (int i = threadIdx.x; i < p.tiles; i += 256) atomicAdd(&classes[class_of(i)], 1);
   __syncthreads();
-  if (threadIdx.x < 32) {                // counts into places: 32 classes a lane
-    int sum = 0;
-    for (int i = 0; i < 32; ++i) { const int c = classes[threadIdx.x * 32 + i]; classes[threadIdx.x * 32 + i] = sum; sum += c; }
-    int before = sum;
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;      // counts into places
+  const int4 n = *reinterpret_cast<int4*>(classes + threadIdx.x * 4);
+  int before = n.x + n.y + n.z + n.w;
+  const int mine = before;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if ((int)threadIdx.x >= o) before += x; }
-    before -= sum;
-    for (int i = 0; i < 32; ++i) classes[threadIdx.x * 32 + i] += before;
-  }
+  for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
+  if (lane == 31) warp_sums[wid] = before;
+  __syncthreads();
+  before -= mine;
+  for (int i = 0; i < wid; ++i) before += warp_sums[i];
+  *reinterpret_cast<int4*>(classes + threadIdx.x * 4) = make_int4(before, before + n.x, before + n.x + n.y, before + n.x + n.y + n.z);
   __syncthreads();
   for (int i = threadIdx.x; i < p.tiles; i += 256) order[atomicAdd(&classes[class_of(i)], 1)] = i;
-  __syncthreads();
 }
 
+// A CTA turns 128 rows of a head into planes.  The first head's CTAs find their rows' segments as well, and one or two CTAs more plan the
+// order of the tiles.  All that a CTA wants of global memory is asked for before the first of it is used, and the offsets are searched
+// in shared memory where they fit: with few tiles the kernel is as long as its longest chain of waits (1531 tokens, 6 + 2 heads of 80, for the
+// gradient: 23.6 us with the offsets searched and delta formed a load at a time).
 template <int DP>
-__global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
+__global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p) {
   constexpr int kLanes = DP / 4, kRows = 256 / kLanes, kPasses = 128 / kRows;      // lanes of a row, rows of a pass
-  __shared__ float red[8];
+  __shared__ float red[8], row_delta[128], offsets[1024];
   __shared__ uint32_t bad[4];
   __shared__ int4 range[4];
-  __shared__ int classes[1024];
+  __shared__ __align__(16) int classes[kClasses];
   const int tile = blockIdx.x;
-  if (tile == p.tiles) {                 // one CTA more than there are tiles plans their order
-    if (blockIdx.y == 0) { plan_order(p, 0, classes); if (p.delta) plan_order(p, 1, classes); }
-    return;
-  }
+  const bool plans = tile == p.tiles;
+  if (plans && blockIdx.y > (p.delta ? 1 : 0)) return;
   int h = blockIdx.y, which = 0;
   while (h >= p.in[which].heads) h -= p.in[which++].heads;
   const PlanesDev& x = p.in[which];
+  const int c = (threadIdx.x % kLanes) * 4, r0 = threadIdx.x / kLanes;
+  float4 v[kPasses];
+  const bool mine = c < p.dk;
+  const i64 t0 = (i64)tile * 128 + r0;
+  const float* src = x.x + t0 * x.st + h * x.sh + c;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    v[i] = make_float4(0, 0, 0, 0);
+    if (mine && t0 + i * kRows < p.T) {
+      const float* s = src + i * kRows * x.st;
+      if (x.vec) v[i] = __ldcs(reinterpret_cast<const float4*>(s));
+      else { v[i].x = s[0]; if (c + 1 < p.dk) v[i].y = s[1]; if (c + 2 < p.dk) v[i].z = s[2]; if (c + 3 < p.dk) v[i].w = s[3]; }
+    }
+  }
+  const bool with_delta = p.delta && which == 3;
+  float lse = -INFINITY;
+  if (with_delta && threadIdx.x < 128 && tile * 128 + (int)threadIdx.x < p.T) lse = p.lse[(i64)h * p.T + tile * 128 + threadIdx.x];
   if (threadIdx.x < 4) bad[threadIdx.x] = 0;
-  if (blockIdx.y == 0) {                 // the rows' segments and the range of their ends
-    if (threadIdx.x < 128) {
-      const int2 s = find_segment(p, tile * 128 + threadIdx.x);
+  if (plans || blockIdx.y == 0) {
+    const float* starts = p.starts;
+    if (p.n_seg < 1024) {
+      for (int i = threadIdx.x; i <= p.n_seg; i += 256) offsets[i] = p.starts[i];
+      starts = offsets;
+    }
+    __syncthreads();
+    if (plans) { plan_order(p, starts, blockIdx.y, classes, (int*)red); return; }
+    if (threadIdx.x < 128) {             // the rows' segments and the range of their ends
+      const int2 s = find_segment(p, starts, tile * 128 + threadIdx.x);
       const int4 r = make_int4(__reduce_min_sync(0xffffffffu, s.x), __reduce_max_sync(0xffffffffu, s.x), __reduce_min_sync(0xffffffffu, s.y), __reduce_max_sync(0xffffffffu, s.y));
       if ((threadIdx.x & 31) == 0) range[threadIdx.x >> 5] = r;
     }
@@ -134,45 +163,29 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
       p.ranges[tile] = r;
     }
   } else __syncthreads();
-  const int c = (threadIdx.x % kLanes) * 4, r0 = threadIdx.x / kLanes;
-  float4 v[kPasses];
-  const bool mine = c < p.dk;
-  const i64 t0 = (i64)tile * 128 + r0;
-  const float* src = x.x + t0 * x.st + h * x.sh + c;
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) {      // all loads before the first use
-    v[i] = make_float4(0, 0, 0, 0);
-    if (mine && t0 + i * kRows < p.T) {
-      const float* s = src + i * kRows * x.st;
-      if (x.vec) v[i] = __ldcs(reinterpret_cast<const float4*>(s));
-      else { v[i].x = s[0]; if (c + 1 < p.dk) v[i].y = s[1]; if (c + 2 < p.dk) v[i].z = s[2]; if (c + 3 < p.dk) v[i].w = s[3]; }
-    }
-  }
-  if (p.delta && which == 3) {      // delta of the rows, and 14 minus their lse in base 2 (a row of no segment: -infinity, so that every p is 0)
+  if (with_delta) {      // delta of the rows
     const float* o = p.o + t0 * p.o_st + h * p.o_sh + c;
+    constexpr int kBatch = DP == 64 ? 4 : 8;
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const i64 t = t0 + i * kRows;
-      float d = 0.0f;
-      if (mine && t < p.T) {
-        const float* oo = o + i * kRows * p.o_st;
-        if (p.o_vec) { const float4 y = *reinterpret_cast<const float4*>(oo); d = v[i].x * y.x; d = fmaf(v[i].y, y.y, d); d = fmaf(v[i].z, y.z, d); d = fmaf(v[i].w, y.w, d); }
-        else {
-          d = v[i].x * oo[0];
-          if (c + 1 < p.dk) d = fmaf(v[i].y, oo[1], d);
-          if (c + 2 < p.dk) d = fmaf(v[i].z, oo[2], d);
-          if (c + 3 < p.dk) d = fmaf(v[i].w, oo[3], d);
+    for (int i0 = 0; i0 < kPasses; i0 += kBatch) {
+      float4 y[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        y[i] = make_float4(0, 0, 0, 0);
+        if (mine && t0 + (i0 + i) * kRows < p.T) {
+          const float* s = o + (i0 + i) * kRows * p.o_st;
+          if (p.o_vec) y[i] = *reinterpret_cast<const float4*>(s);
+          else { y[i].x = s[0]; if (c + 1 < p.dk) y[i].y = s[1]; if (c + 2 < p.dk) y[i].z = s[2]; if (c + 3 < p.dk) y[i].w = s[3]; }
         }
       }
 #pragma unroll
-      for (int k = kLanes / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
-      if (c == 0) {
-        const i64 at = ((i64)h * p.tiles + tile) * 128 + i * kRows + r0;
-        float l = t < p.T ? p.lse[(i64)h * p.T + t] : -INFINITY;
-        const bool dead = l == -INFINITY;
-        if (d != d) l = d;             // (a gradient that is not finite: dv sees it through p)
-        p.lift[at] = dead ? -INFINITY : 14.0f - l * kL2e;
-        p.delta[at] = dead ? 0.0f : d;
+      for (int i = 0; i < kBatch; ++i) {
+        const float4 g = v[i0 + i];
+        float d = g.x * y[i].x;
+        d = fmaf(g.y, y[i].y, d); d = fmaf(g.z, y[i].z, d); d = fmaf(g.w, y[i].w, d);
+#pragma unroll
+        for (int k = kLanes / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
+        if (c == 0) row_delta[(i0 + i) * kRows + r0] = d;
       }
     }
   }
@@ -200,6 +213,14 @@ __global__ void __launch_bounds__(256) k_prepare(PrepareDev p) {
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) red[wid] = m;
   __syncthreads();
+  if (with_delta && threadIdx.x < 128) {      // and 14 minus their lse in base 2 (a row of no segment: -infinity, so that every p is 0)
+    const float d = row_delta[threadIdx.x];
+    const bool dead = lse == -INFINITY;
+    if (d != d) lse = d;                      // (a gradient that is not finite: dv sees it through p)
+    const i64 at = ((i64)h * p.tiles + tile) * 128 + threadIdx.x;
+    p.lift[at] = dead ? -INFINITY : 14.0f - lse * kL2e;
+    p.delta[at] = dead ? 0.0f : d;
+  }
   m = red[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) m = fmaxf(m, red[i]);
