@@ -277,19 +277,21 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + pl * plane_bytes<ROWS, DP>() + c * ROWS * 128, map, bar, c * 64, row, head, pl);
 }
-// D[128, N] (+)= A[128, DP] B[N, DP]^T for one plane of each, K-major tiles in shared memory; or A in tensor memory (DP / 2 columns)
+// D[128, N] (+)= A[128, DP] B[N, DP]^T for one plane of each, K-major tiles in shared memory; or A in tensor memory (DP / 2 columns).
+// The first 16 `steps` components alone: beyond the head size the planes are 0.
 template <int N, int DP>
-__device__ __forceinline__ void rows_by_rows(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t on) {
+__device__ __forceinline__ void rows_by_rows(uint32_t leader, int steps, uint32_t d, uint32_t a, uint32_t b, uint32_t on) {
   const uint64_t da = desc16(a, 0), db = desc16(b, 0);
 #pragma unroll
   for (int k = 0; k < DP / 16; ++k, on = 1)
-    mma_f16(leader, d, da + (((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4), db + (((k >> 2) * N * 128 + (k & 3) * 32) >> 4), idesc16(128, N, 0, 0), on);
+    if (k < steps) mma_f16(leader, d, da + (((k >> 2) * 128 * 128 + (k & 3) * 32) >> 4), db + (((k >> 2) * N * 128 + (k & 3) * 32) >> 4), idesc16(128, N, 0, 0), on);
 }
 template <int N, int DP>
-__device__ __forceinline__ void kept_by_rows(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t on) {
+__device__ __forceinline__ void kept_by_rows(uint32_t leader, int steps, uint32_t d, uint32_t a, uint32_t b, uint32_t on) {
   const uint64_t db = desc16(b, 0);
 #pragma unroll
-  for (int k = 0; k < DP / 16; ++k, on = 1) mma_f16_ta(leader, d, a + k * 8, db + (((k >> 2) * N * 128 + (k & 3) * 32) >> 4), idesc16(128, N, 0, 0), on);
+  for (int k = 0; k < DP / 16; ++k, on = 1)
+    if (k < steps) mma_f16_ta(leader, d, a + k * 8, db + (((k >> 2) * N * 128 + (k & 3) * 32) >> 4), idesc16(128, N, 0, 0), on);
 }
 // D[128, DP] (+)= A[128, K] B[K, DP], A in tensor memory (per quarter of the columns: K / 8 columns of hi, then of lo), B a plane of K rows
 template <int K, int DP, bool LO>
@@ -451,6 +453,7 @@ struct Seat {
 struct Side { const __half* planes; const float* inv; const float* len; const uint32_t* bad; };
 struct AttnParams {
   int T, tiles, hq, hk, dk;
+  int steps;                                  // of 16 components in a head
   float scale;
   const int* begin; const int* end;
   const int* order;                           // [2][tiles] tiles by the work they have as queries, and as keys, the most first
@@ -562,11 +565,11 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       auto scores = [&](int j) -> bool {
         const uint32_t d = t_s + (j & 1) * 128;
         if (!next()) return false;
-        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 0);
+        rows_by_rows<128, DP>(leader, p.steps, d, x_hi, r0 + slot * L::kPlane, 0);
         release();
         if (!next()) return false;
-        rows_by_rows<128, DP>(leader, d, x_lo, r0 + slot * L::kPlane, 1);
-        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 1);
+        rows_by_rows<128, DP>(leader, p.steps, d, x_lo, r0 + slot * L::kPlane, 1);
+        rows_by_rows<128, DP>(leader, p.steps, d, x_hi, r0 + slot * L::kPlane, 1);
         release();
         commit_by(leader, &b_s[j & 1]);
         return true;
@@ -741,11 +744,11 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
       auto scores = [&](int j) -> bool {
         const uint32_t d = t_s + (j & 1) * 128;
         if (!next()) return false;
-        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 0);
+        rows_by_rows<128, DP>(leader, p.steps, d, x_hi, r0 + slot * L::kPlane, 0);
         release();
         if (!next()) return false;
-        rows_by_rows<128, DP>(leader, d, x_lo, r0 + slot * L::kPlane, 1);
-        rows_by_rows<128, DP>(leader, d, x_hi, r0 + slot * L::kPlane, 1);
+        rows_by_rows<128, DP>(leader, p.steps, d, x_lo, r0 + slot * L::kPlane, 1);
+        rows_by_rows<128, DP>(leader, p.steps, d, x_hi, r0 + slot * L::kPlane, 1);
         release();
         commit_by(leader, &b_s[j & 1]);
         return true;
@@ -935,9 +938,9 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
         tc_fence_after();
         const uint32_t d = t_s + (j & 1) * N, x = smem_u32(x1), y = smem_u32(y1 + y1_in * L::kTileY);
         if (++y1_in == N1) { y1_in = 0; y1_phase ^= 1; }
-        rows_by_rows<N, DP>(leader, d, x + kPX, y, 0);
-        rows_by_rows<N, DP>(leader, d, x, y + kPY, 1);
-        rows_by_rows<N, DP>(leader, d, x, y, 1);
+        rows_by_rows<N, DP>(leader, p.steps, d, x + kPX, y, 0);
+        rows_by_rows<N, DP>(leader, p.steps, d, x, y + kPY, 1);
+        rows_by_rows<N, DP>(leader, p.steps, d, x, y, 1);
         commit_by(leader, &b_s[j & 1]);
         return true;
       };
@@ -945,9 +948,9 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
         if (!warp_wait(&b_y2full[j % N2], (j / N2) & 1, abort_flag)) return false;
         tc_fence_after();
         const uint32_t y = smem_u32(y2 + (j % N2) * L::kTileY);
-        kept_by_rows<N, DP>(leader, t_dp, t_x2 + DP / 2, y, 0);
-        kept_by_rows<N, DP>(leader, t_dp, t_x2, y + kPY, 1);
-        kept_by_rows<N, DP>(leader, t_dp, t_x2, y, 1);
+        kept_by_rows<N, DP>(leader, p.steps, t_dp, t_x2 + DP / 2, y, 0);
+        kept_by_rows<N, DP>(leader, p.steps, t_dp, t_x2, y + kPY, 1);
+        kept_by_rows<N, DP>(leader, p.steps, t_dp, t_x2, y, 1);
         commit_by(leader, &b_y2free[j % N2]);
         commit_by(leader, b_dp);
         return true;
@@ -1068,6 +1071,7 @@ __device__ __forceinline__ float4 plus(float4 a, float4 b) { return make_float4(
 // the parts of dK and dV added in order
 template <class V>
 __global__ void __launch_bounds__(256) k_add_parts(const V* __restrict__ a, const V* __restrict__ b, V* __restrict__ oa, V* __restrict__ ob, i64 n, int parts) {
+  wait_for_last_kernel();
   for (i64 i = (i64)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (i64)gridDim.x * 256) {
     const V* src = i < n ? a + i : b + (i - n);
     V s = src[0];
@@ -1136,7 +1140,7 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
   if (o) { d.o = o->p; d.o_st = o->st; d.o_sh = o->sh; d.lse = lse;
            d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lift = (float*)(base + lift); }
   AttnParams& p = w.p;
-  p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.scale = s.scale;
+  p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.steps = (s.dk + 15) / 16; p.scale = s.scale;
   p.begin = d.begin; p.end = d.end; p.ranges = d.ranges; p.order = d.order; p.lift = d.lift; p.delta = d.delta; p.err = ctx().d_err;
   ProfScope prof("segment_attn_prepare", 8.0 * (double)s.T * all * s.dk);
   if (dp == 64) k_prepare<64><<<dim3(tiles + 1, all), 256, 0, ctx().stream>>>(d);
@@ -1185,10 +1189,9 @@ int backward(Work& w, float* dq, float* dk, float* dv) {
     const i64 cap = (i64)ctx().sm_count * 8;
     const bool vec = n % 4 == 0 && ((reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15) == 0;
     const i64 m = vec ? n / 4 : n, ctas = (2 * m + 255) / 256;
-    const unsigned grid = (unsigned)(ctas < cap ? ctas : cap);
-    if (vec) k_add_parts<<<grid, 256, 0, ctx().stream>>>((const float4*)p.dk_, (const float4*)p.dv, (float4*)dk, (float4*)dv, m, p.parts);
-    else k_add_parts<<<grid, 256, 0, ctx().stream>>>((const float*)p.dk_, (const float*)p.dv, dk, dv, m, p.parts);
-    VB_LAUNCH_CHECK();
+    const dim3 grid((unsigned)(ctas < cap ? ctas : cap));
+    if (vec) return launch_early(k_add_parts<float4>, grid, dim3(256), 0, (const float4*)p.dk_, (const float4*)p.dv, (float4*)dk, (float4*)dv, m, p.parts);
+    return launch_early(k_add_parts<float>, grid, dim3(256), 0, (const float*)p.dk_, (const float*)p.dv, dk, dv, m, p.parts);
   }
   return VB_OK;
 }
