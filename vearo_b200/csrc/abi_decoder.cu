@@ -18,19 +18,18 @@ struct OnDevice {
   OnDevice() { if (ctx().ready && cudaGetDevice(&before) == cudaSuccess && before != ctx().device) cudaSetDevice(ctx().device); }
   ~OnDevice() { if (ctx().ready && before >= 0 && before != ctx().device) cudaSetDevice(before); }
 };
-// Outputs of a call that may still fail: what has been allocated is given back unless done() is reached.
+// Outputs of a call that may still fail: the caller's descriptors are written by done(), after the last look at the inputs' (which may be
+// the same descriptors); without it what has been allocated is given back.
 struct Outputs {
-  vb_tensor* t[6] = {};
+  vb_tensor fresh[6], *to[6];
   int n = 0;
   int add(vb_tensor* out, int rank, const i64* dims, float** p) {
-    vb_tensor fresh;
-    VB_TRY(new_output(&fresh, rank, dims));
-    *out = fresh;
-    t[n++] = out;
-    return slot_ptr(out->slot, p);
+    VB_TRY(new_output(&fresh[n], rank, dims));
+    to[n] = out;
+    return slot_ptr(fresh[n++].slot, p);
   }
-  void done() { n = 0; }
-  ~Outputs() { for (int i = 0; i < n; ++i) { slot_release(t[i]->slot, nullptr); t[i]->slot = 0; } }
+  void done() { for (int i = 0; i < n; ++i) *to[i] = fresh[i]; n = 0; }
+  ~Outputs() { for (int i = 0; i < n; ++i) slot_release(fresh[i].slot, nullptr); }
 };
 // The arena hands scratch and outputs of one call to the next, which a replay of a captured call would not know of.
 int common_checks(const char* who) {
