@@ -156,3 +156,34 @@ def test_refusals_leave_no_slot_behind(vb):
         assert L.vb_segment_attention_backward(q.ref, k.ref, v.ref, s.ref, 1.0, *[r(i) for i in a], *[C.byref(x) for x in o]) == 1
     assert L.vb_segment_attention_backward(q.ref, k.ref, v.ref, s.ref, 1.0, q.ref, lse.ref, q.ref, C.byref(o[0]), None, C.byref(o[2])) == 1
     assert vb.memory_stats()["live_slots"] == before
+
+
+@pytest.mark.parametrize("fill", [1e30, -3e-30, np.nan])
+def test_rows_of_no_segment_may_hold_anything(vb, fill):
+    """Rows before the first segment and behind the last share tiles, and so exponents, with rows that have one."""
+    T, starts = 300, [9, 140, 270]
+    q, k, v, g = rnd(50, T, 2, 64), rnd(51, T, 1, 64), rnd(52, T, 1, 64), rnd(53, T, 2, 64)
+    for x in (q, k, v, g):
+        x[:9], x[270:] = 0, 0
+    want = run(vb, q, k, v, starts, 0.125, g)
+    for x in (q, k, v, g):
+        x[:9], x[270:] = fill, fill
+    for a, b in zip(run(vb, q, k, v, starts, 0.125, g), want):
+        assert (a == b).all()
+
+
+def test_gradients_may_go_to_the_descriptors_of_the_inputs(vb):
+    """Outputs are written to the descriptors after the last look at the inputs, whichever descriptors they are."""
+    T = 60
+    q, k, v, g = rnd(54, T, 4, 16), rnd(55, T, 1, 16), rnd(56, T, 1, 16), rnd(57, T, 4, 16)
+    want = run(vb, q, k, v, [0, 25, T], 0.25, g)
+    D = [Dev(vb, a) for a in (q, k, v, [0, 25, T], want[0], want[1], g)]
+    d = [vb.VbTensor.from_buffer_copy(x.desc) for x in D[:4]]
+    at = [C.byref(x) for x in d]
+    vb.vb_check(vb.lib().vb_segment_attention_backward(*at, 0.25, D[4].ref, D[5].ref, D[6].ref, at[1], at[3], at[0]))
+    for x, b in zip((d[1], d[3], d[0]), want[2:]):
+        assert x.shape == b.shape
+        a = np.empty(b.shape, np.float32)
+        vb.vb_check(vb.lib().vb_read(x.slot, 0, a.ctypes.data_as(vb.c_f32p), a.size))
+        vb.lib().vb_release(x.slot, None)
+        assert (a == b).all()

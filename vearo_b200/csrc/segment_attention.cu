@@ -112,7 +112,7 @@ __device__ void plan_order(const PrepareDev& p, const float* starts, int which, 
 // order of the tiles.  All that a CTA wants of global memory is asked for before the first of it is used, and the offsets are searched
 // in shared memory where they fit: with few tiles the kernel is as long as its longest chain of waits (1531 tokens, 6 + 2 heads of 80, for the
 // gradient: 23.6 us with the offsets searched and delta formed a load at a time).
-template <int DP>
+template <int DP, bool GRAD>
 __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p) {
   constexpr int kLanes = DP / 4, kRows = 256 / kLanes, kPasses = 128 / kRows;      // lanes of a row, rows of a pass
   __shared__ float red[8], row_delta[128], offsets[1024];
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   __shared__ __align__(16) int classes[kClasses];
   const int tile = blockIdx.x;
   const bool plans = tile == p.tiles;
-  if (plans && blockIdx.y > (p.delta ? 1 : 0)) return;
+  if (plans && blockIdx.y > (GRAD ? 1 : 0)) return;
   int h = blockIdx.y, which = 0;
   while (h >= p.in[which].heads) h -= p.in[which++].heads;
   const PlanesDev& x = p.in[which];
@@ -129,17 +129,20 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   float4 v[kPasses];
   const bool mine = c < p.dk;
   const i64 t0 = (i64)tile * 128 + r0;
+  // Rows before the first segment and behind the last may hold anything: they are not read, and as zeros do not reach the tile's exponent.
+  const float first = roundf(p.starts[0]), behind = roundf(p.starts[p.n_seg]);
+  const int live0 = first > 0.0f ? (int)fminf(first, (float)p.T) : 0, live1 = behind < (float)p.T ? (int)fmaxf(behind, 0.0f) : p.T;
   const float* src = x.x + t0 * x.st + h * x.sh + c;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     v[i] = make_float4(0, 0, 0, 0);
-    if (mine && t0 + i * kRows < p.T) {
+    if (mine && t0 + i * kRows >= live0 && t0 + i * kRows < live1) {
       const float* s = src + i * kRows * x.st;
       if (x.vec) v[i] = __ldcs(reinterpret_cast<const float4*>(s));
       else { v[i].x = s[0]; if (c + 1 < p.dk) v[i].y = s[1]; if (c + 2 < p.dk) v[i].z = s[2]; if (c + 3 < p.dk) v[i].w = s[3]; }
     }
   }
-  const bool with_delta = p.delta && which == 3;
+  const bool with_delta = GRAD && which == 3;
   float lse = -INFINITY;
   if (with_delta && threadIdx.x < 128 && tile * 128 + (int)threadIdx.x < p.T) lse = p.lse[(i64)h * p.T + tile * 128 + threadIdx.x];
   if (threadIdx.x < 4) bad[threadIdx.x] = 0;
@@ -1143,8 +1146,10 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
   p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.steps = (s.dk + 15) / 16; p.scale = s.scale;
   p.begin = d.begin; p.end = d.end; p.ranges = d.ranges; p.order = d.order; p.lift = d.lift; p.delta = d.delta; p.err = ctx().d_err;
   ProfScope prof("segment_attn_prepare", 8.0 * (double)s.T * all * s.dk);
-  if (dp == 64) k_prepare<64><<<dim3(tiles + 1, all), 256, 0, ctx().stream>>>(d);
-  else k_prepare<128><<<dim3(tiles + 1, all), 256, 0, ctx().stream>>>(d);
+  const dim3 grid(tiles + 1, all);
+  if (dp == 64) { if (o) k_prepare<64, true><<<grid, 256, 0, ctx().stream>>>(d); else k_prepare<64, false><<<grid, 256, 0, ctx().stream>>>(d); }
+  else if (o) k_prepare<128, true><<<grid, 256, 0, ctx().stream>>>(d);
+  else k_prepare<128, false><<<grid, 256, 0, ctx().stream>>>(d);
   VB_LAUNCH_CHECK();
   return VB_OK;
 }
