@@ -228,3 +228,20 @@ def test_the_same_bits_twice(vb):
         return [loss, lse] + outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *D, -100, Dev(vb, lse), one, n=2)
     for a, b in zip(run(), run()):
         assert (a == b).all()
+
+
+@pytest.mark.parametrize("n,d,v", [(2, 40, 20000), (1, 129, 9001), (70, 260, 5000), (5000, 64, 10), (3000, 33, 70)])
+def test_long_sums_of_few_tiles(vb, n, d, v):
+    """dx sums over the vocabulary and dW over the rows: with few rows, or few classes, they are formed in parts."""
+    x, w = rnd(40, n, d), rnd(41, v, d, scale=2.0 / np.sqrt(d))
+    t = np.random.default_rng(42).integers(0, v, n).astype(np.float32)
+    (lse, loss, gx, gw), (e_lse, e_loss, egx, egw) = truth(x, w, t, -100, 1.5)
+    D = [Dev(vb, a) for a in (x, w, t)]
+    got_loss, got_lse = outputs(vb, vb.lib().vb_linear_cross_entropy, *D, -100, n=2)
+    assert (np.abs(got_lse - lse) <= e_lse).all() and abs(got_loss[0] - loss) <= e_loss
+    rest = (*D, -100, Dev(vb, got_lse), Dev(vb, np.array([1.5], np.float32)))
+    got = outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *rest, n=2)
+    vb.check_errors()
+    assert (np.abs(got[0] - gx) <= egx).all() and (np.abs(got[1] - gw) <= egw).all()
+    for a, b in zip(got, outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *rest, n=2)):
+        assert (a == b).all()

@@ -90,10 +90,20 @@ struct OperandDev { CUtensorMap map; const float* inv; i64 inv_ld; int mn, by_ro
 struct ProblemDev {
   OperandDev a, b;
   CUtensorMap out_map;                       // Store: f32, where `by_copy`; LossGrad: the planes
-  int M, N, K, tiles_m, tiles;
+  int M, N, K, tiles_m, tiles;               // tiles: of all parts
+  int parts, part_k;                         // Store: the sum over k in parts of part_k steps, each a tile of its own in plane `part` of the result
   float* out; i64 ldo; int add, by_copy;
   const float* alpha; float alpha_host;
 };
+// A tile of a problem: rows, columns, steps of k, part.
+struct TileAt { int tm, tn, k0, k1, part; };
+__device__ __forceinline__ TileAt tile_at(const ProblemDev& q, int t) {
+  TileAt a;
+  a.part = t % q.parts; t /= q.parts;
+  a.tm = t % q.tiles_m; a.tn = t / q.tiles_m;
+  a.k0 = a.part * q.part_k; a.k1 = min(q.K, a.k0 + q.part_k);
+  return a;
+}
 struct Params {
   ProblemDev prob[2];
   const int* target; int col0; float2* stats; float* target_value; const float* lse;
@@ -165,9 +175,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
         if (t >= tiles) break;
         next = next_tile(p.counter);
         const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
-        const int lt = t < p.prob[0].tiles ? t : t - p.prob[0].tiles;
-        const int m0 = (lt % q.tiles_m) * kBM, n0 = (lt / q.tiles_m) * kBN;
-        for (int k0 = 0; k0 < q.K; k0 += kBK, ++it) {
+        const TileAt at = tile_at(q, t < p.prob[0].tiles ? t : t - p.prob[0].tiles);
+        const int m0 = at.tm * kBM, n0 = at.tn * kBN;
+        for (int k0 = at.k0; k0 < at.k1; k0 += kBK, ++it) {
           const int st = it % kStages;
           if (it >= kStages && !mbar_wait(&bars[B_EMPTY + st], ((it / kStages) - 1) & 1, abort_flag)) { ok = false; break; }
           uint64_t* full = &bars[B_FULL + st];
@@ -200,12 +210,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
       const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
       const uint32_t idesc = idesc16(kBM, kBN, q.a.mn, q.b.mn);
       const uint64_t step_a = (q.a.mn ? 2048 : 32) >> 4, step_b = (q.b.mn ? 2048 : 32) >> 4;
-      for (int k0 = 0; k0 < q.K && ok; k0 += 2 * kBK, ++run) {
+      const TileAt at = tile_at(q, t < p.prob[0].tiles ? t : t - p.prob[0].tiles);
+      for (int k0 = at.k0; k0 < at.k1 && ok; k0 += 2 * kBK, ++run) {
         const int acc = run & 1;
         if (run >= 2 && !warp_wait(&bars[B_RUNFREE + acc], ((run >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
         const uint32_t d = tmem + acc * kBN;
         uint32_t on = 0;
-        for (int k = k0; k < q.K && k < k0 + 2 * kBK; k += kBK, ++it) {
+        for (int k = k0; k < at.k1 && k < k0 + 2 * kBK; k += kBK, ++it) {
           const int st = it % kStages;
           if (!warp_wait(&bars[B_FULL + st], (it / kStages) & 1, abort_flag)) { ok = false; break; }
           tc_fence_after();
@@ -234,8 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
     int t;
     for (uint32_t i = 0; ok && take(i, &t); ++i) {
       const ProblemDev& q = t < p.prob[0].tiles ? p.prob[0] : p.prob[1];
-      const int lt = t < p.prob[0].tiles ? t : t - p.prob[0].tiles;
-      const int tm = lt % q.tiles_m, tn = lt / q.tiles_m;
+      const TileAt at = tile_at(q, t < p.prob[0].tiles ? t : t - p.prob[0].tiles);
+      const int tm = at.tm, tn = at.tn;
       const int m = tm * kBM + row, n0 = tn * kBN + half * 128;
       int target = kNoTarget;
       float off = 0.0f;
@@ -254,9 +265,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
         if (q.b.inv) s *= q.b.mn ? q.b.inv[(i64)kb * q.b.inv_ld + nb] : q.b.inv[(i64)nb * q.b.inv_ld + kb];
         return s;
       };
-      float s = scale_of(0);
-      for (int kb = 0; kb * 128 < q.K; ++kb, ++run) {
-        const float s_next = (kb + 1) * 128 < q.K ? scale_of(kb + 1) : 0.0f;
+      float s = scale_of(at.k0 / 128);
+      for (int kb = at.k0 / 128; kb * 128 < at.k1; ++kb, ++run) {
+        const float s_next = (kb + 1) * 128 < at.k1 ? scale_of(kb + 1) : 0.0f;
         if (!mbar_wait(&bars[B_RUN + (run & 1)], (run >> 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const uint32_t src = tmem + (run & 1) * kBN + half * 128 + ((uint32_t)(quarter * 32) << 16);
@@ -296,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
             fence_async_smem();
             __syncwarp();
             if (lane == 0 && col < q.N && mrow < q.M) {
-              if (q.add) add_block(&q.out_map, stg, col, mrow, 0); else store_block(&q.out_map, stg, col, mrow, 0);
+              if (q.add) add_block(&q.out_map, stg, col, mrow, 0); else store_block(&q.out_map, stg, col, mrow, at.part);
               commit_blocks();
             }
           } else {
@@ -420,16 +431,33 @@ int make_operand(const Op16& o, int box_mn, OperandDev* d) {
   return VB_OK;
 }
 
-// map of a result for the epilogue's 32 x 32 blocks: f32 rows of `ld` (128-byte swizzle), or the two planes of halves (64-byte swizzle)
-int make_result(CUtensorMap* map, void* base, i64 cols, i64 rows, i64 ld, i64 plane, bool half) {
+// map of a result for the epilogue's 32 x 32 blocks: f32 rows of `ld` (128-byte swizzle), a plane a part, or the two planes of halves (64-byte swizzle)
+int make_result(CUtensorMap* map, void* base, i64 cols, i64 rows, i64 ld, i64 plane, int planes, bool half) {
   const cuuint64_t size = half ? 2 : 4;
-  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, half ? 2u : 1u}, strides[2] = {(cuuint64_t)ld * size, (cuuint64_t)(half ? plane : ld * rows) * size};
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes}, strides[2] = {(cuuint64_t)ld * size, (cuuint64_t)plane * size};
   cuuint32_t box[3] = {32, 32, 1}, estr[3] = {1, 1, 1};
   CUresult r = encode_fn()(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, base, dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, half ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(VB_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
   return VB_OK;
+}
+
+// the parts of a product added in order
+__global__ void __launch_bounds__(256) k_join_parts(const float* __restrict__ part, i64 part_ld, i64 part_step, int parts, float* __restrict__ out, i64 ldo, int M, int N, bool add) {
+  const int n = blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  for (i64 m = blockIdx.y; m < M; m += gridDim.y) {
+    const float* p = part + m * part_ld + n;
+    float s = add ? out[m * ldo + n] : 0.0f;
+    int i = 0;
+    for (; i + 4 <= parts; i += 4) {
+      const float a = p[i * part_step], b = p[(i + 1) * part_step], c = p[(i + 2) * part_step], d = p[(i + 3) * part_step];
+      s = (((s + a) + b) + c) + d;
+    }
+    for (; i < parts; ++i) s += p[i * part_step];
+    out[m * ldo + n] = s;
+  }
 }
 
 template <Tile16 WHAT>
@@ -481,19 +509,44 @@ int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter) {
   Params p{};
   p.counter = counter;
   double flops = 0.0;
+  i64 work = 0;                    // runs of 128 k, and three for a tile's epilogue
+  for (int i = 0; i < n; ++i) {
+    const Product16& g = products[i];
+    const i64 tm = (g.M + kBM - 1) / kBM, tn = (g.N + kBN - 1) / kBN;
+    if (g.M > 0x7fffff00 || g.N > 0x7fffff00 || g.K > 0x7fffff00 || tm * tn > 0x3fffffff) return set_error(VB_ERR_UNSUPPORTED, "product too large");
+    work += tm * tn * ((g.K + 127) / 128 + 3);
+  }
+  Temp hold[2];
   for (int i = 0; i < n; ++i) {
     const Product16& g = products[i];
     ProblemDev& q = p.prob[i];
-    const i64 tm = (g.M + kBM - 1) / kBM, tn = (g.N + kBN - 1) / kBN;
-    if (g.M > 0x7fffff00 || g.N > 0x7fffff00 || g.K > 0x7fffff00 || tm * tn > 0x3fffffff) return set_error(VB_ERR_UNSUPPORTED, "product too large");
-    q.M = (int)g.M; q.N = (int)g.N; q.K = (int)g.K; q.tiles_m = (int)tm; q.tiles = (int)(tm * tn);
+    const i64 tm = (g.M + kBM - 1) / kBM, tn = (g.N + kBN - 1) / kBN, runs = (g.K + 127) / 128;
+    q.M = (int)g.M; q.N = (int)g.N; q.K = (int)g.K; q.tiles_m = (int)tm;
+    // A tile whose sum is longer than an SM's share of the launch is formed in parts of that length, eight runs at least (2 rows, width 880,
+    // 45893 columns: dx is four tiles of 359 runs, 1158 us a gradient pass in one part, PARTS_US in PARTS_N).
+    q.parts = 1;
+    q.part_k = (int)(runs * 128);
+    if (what == Tile16::Store) {
+      const i64 share = work / ctx().sm_count > 8 ? work / ctx().sm_count : 8;
+      if (runs > share + share / 2) {
+        const i64 parts = (runs + share - 1) / share, part_runs = (runs + parts - 1) / parts;
+        q.parts = (int)((runs + part_runs - 1) / part_runs);
+        q.part_k = (int)(part_runs * 128);
+      }
+    }
+    q.tiles = (int)(tm * tn * q.parts);
     VB_TRY(make_operand(g.a, kBM, &q.a));
     VB_TRY(make_operand(g.b, kBN, &q.b));
     q.out = g.out; q.ldo = g.ldo; q.add = g.add; q.alpha = g.alpha; q.alpha_host = g.alpha_host;
     // (the copy engine stores rows that begin on 16 bytes)
     q.by_copy = what == Tile16::Store && g.ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-    if (q.by_copy) VB_TRY(make_result(&q.out_map, g.out, g.N, g.M, g.ldo, 0, false));
-    if (what == Tile16::LossGrad) VB_TRY(make_result(&q.out_map, g.grad.planes, g.N, g.M, g.grad.ld, g.grad.plane, true));
+    if (q.parts > 1) {
+      const i64 ld = (g.N + 3) / 4 * 4;
+      VB_TRY(scratch_alloc((size_t)(q.parts * g.M * ld) * sizeof(float), &hold[i].p));
+      q.by_copy = 1; q.add = 0;
+      VB_TRY(make_result(&q.out_map, hold[i].p, g.N, g.M, ld, g.M * ld, q.parts, false));
+    } else if (q.by_copy) VB_TRY(make_result(&q.out_map, g.out, g.N, g.M, g.ldo, g.ldo * g.M, 1, false));
+    if (what == Tile16::LossGrad) VB_TRY(make_result(&q.out_map, g.grad.planes, g.N, g.M, g.grad.ld, g.grad.plane, 2, true));
     flops += 2.0 * (double)g.M * (double)g.N * (double)g.K;
   }
   p.target = products[0].target; p.col0 = (int)products[0].col0; p.stats = products[0].stats; p.target_value = products[0].target_value; p.lse = products[0].lse;
@@ -503,10 +556,19 @@ int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter) {
   ProfScope prof("gemm16", flops);
   const int ctas = tiles < ctx().sm_count ? tiles : ctx().sm_count;
   switch (what) {
-    case Tile16::Store: return launch<Tile16::Store>(p, ctas);
-    case Tile16::RowStats: return launch<Tile16::RowStats>(p, ctas);
-    default: return launch<Tile16::LossGrad>(p, ctas);
+    case Tile16::Store: VB_TRY(launch<Tile16::Store>(p, ctas)); break;
+    case Tile16::RowStats: VB_TRY(launch<Tile16::RowStats>(p, ctas)); break;
+    default: VB_TRY(launch<Tile16::LossGrad>(p, ctas));
   }
+  for (int i = 0; i < n; ++i) {
+    const Product16& g = products[i];
+    if (p.prob[i].parts == 1) continue;
+    const i64 ld = (g.N + 3) / 4 * 4;
+    k_join_parts<<<dim3((unsigned)((g.N + 255) / 256), (unsigned)(g.M < 4096 ? g.M : 4096)), 256, 0, ctx().stream>>>((const float*)hold[i].p, ld, g.M * ld, p.prob[i].parts, g.out, g.ldo,
+                                                                                                                   (int)g.M, (int)g.N, g.add);
+    VB_LAUNCH_CHECK();
+  }
+  return VB_OK;
 }
 
 }  // namespace vb
