@@ -245,3 +245,35 @@ def test_long_sums_of_few_tiles(vb, n, d, v):
     assert (np.abs(got[0] - gx) <= egx).all() and (np.abs(got[1] - gw) <= egw).all()
     for a, b in zip(got, outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *rest, n=2)):
         assert (a == b).all()
+
+
+@pytest.mark.parametrize("n,d,v", [(1, 4, 1), (2, 2048, 70), (4, 128, 64), (5, 132, 65), (8, 1024, 3000), (9, 260, 129), (16, 2048, 500), (16, 64, 20011), (17, 64, 700), (12, 2052, 100),
+                                   (40, 512, 900), (150, 96, 64), (3, 516, 40000)])
+def test_few_rows(vb, n, d, v):
+    """Up to 16 rows, or few blocks of logits: W is read in 32 bits, once a pass.  A row that is left out may hold anything."""
+    x, w = rnd(50, n, d), rnd(51, v, d, scale=2.0 / np.sqrt(d))
+    t = np.random.default_rng(52).integers(0, v, n).astype(np.float32)
+    if n > 2:
+        t[1] = -7
+    (lse, loss, gx, gw), (e_lse, e_loss, egx, egw) = truth(x, w, t, -7, -0.3)
+    x0 = x.copy()
+    if n > 2:
+        x[1] = np.nan
+    D = [Dev(vb, a) for a in (x, w, t)]
+    live = t != -7
+    got_loss, got_lse = outputs(vb, vb.lib().vb_linear_cross_entropy, *D, -7, n=2)
+    assert (np.abs(got_lse - lse) <= e_lse)[live].all() and abs(got_loss[0] - loss) <= e_loss
+    rest = (*D, -7, Dev(vb, got_lse), Dev(vb, np.array([-0.3], np.float32)))
+    got = outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *rest, n=2)
+    vb.check_errors()
+    assert (np.abs(got[0] - gx) <= egx).all() and (np.abs(got[1] - gw) <= egw).all()
+    assert (got[0][~live] == 0).all() and np.isfinite(x0).all()
+    L = vb.lib()
+    for i, want in ((0, got[0]), (1, got[1])):      # one gradient alone, the same bits
+        o = vb.VbTensor()
+        args = [a.ref if isinstance(a, Dev) else a for a in rest]
+        vb.vb_check(L.vb_linear_cross_entropy_backward(*args, C.byref(o) if i == 0 else None, C.byref(o) if i == 1 else None))
+        a = np.empty(o.shape, np.float32)
+        vb.vb_check(L.vb_read(o.slot, 0, a.ctypes.data_as(vb.c_f32p), a.size))
+        L.vb_release(o.slot, None)
+        assert (a == want).all()
