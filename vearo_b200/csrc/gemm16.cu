@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
         for (int c = 0; c < 128; c += 32) {
           uint32_t v[32];
           tmem_ld32(src + c, v);
-          tmem_wait_ld();
+          wait_for_cols<32>(v);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), s2, make_float2(acc[c + e], acc[c + e + 1]));

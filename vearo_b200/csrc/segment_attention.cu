@@ -273,12 +273,16 @@ __device__ __forceinline__ void load_plane(uint8_t* dst, const CUtensorMap* map,
   for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + c * ROWS * 128, map, bar, c * 64, row, head, pl);
 }
 template <int ROWS, int DP>
-__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int head) {
-  mbar_arrive_expect_tx(bar, 2 * plane_bytes<ROWS, DP>());
+__device__ __forceinline__ void copy_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int head) {
 #pragma unroll
   for (int pl = 0; pl < 2; ++pl)
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c) tma_load_4d(dst + pl * plane_bytes<ROWS, DP>() + c * ROWS * 128, map, bar, c * 64, row, head, pl);
+}
+template <int ROWS, int DP>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int row, int head) {
+  mbar_arrive_expect_tx(bar, 2 * plane_bytes<ROWS, DP>());
+  copy_tile<ROWS, DP>(dst, map, bar, row, head);
 }
 // D[128, N] (+)= A[128, DP] B[N, DP]^T for one plane of each, K-major tiles in shared memory; or A in tensor memory (DP / 2 columns).
 // The first 16 `steps` components alone: beyond the head size the planes are 0.
@@ -323,7 +327,7 @@ template <int W>
 __device__ __forceinline__ void load_cols(uint32_t taddr, float (&v)[W]) {
   static_assert(W == 16 || W == 32, "one load");
   if constexpr (W == 32) tmem_ld32(taddr, reinterpret_cast<uint32_t*>(v)); else tmem_ld16(taddr, reinterpret_cast<uint32_t*>(v));
-  tmem_wait_ld();
+  wait_for_cols<W>(reinterpret_cast<uint32_t*>(v));
 }
 // the quarter of a row's columns as the left operand of product_cols: W / 2 columns of hi, W / 2 of lo
 template <int W>
@@ -528,32 +532,38 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();      // (the copies below come before the other warps have seen the barriers)
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   wait_for_last_kernel();
   const int qt = p.order[blockIdx.x / p.hq];
   const int4 range = p.ranges[qt];
   const int b_min = range.x, b_max = range.y;
+  const int kb0 = b_min < p.T ? b_min / 128 : qt + 1, n = qt + 1 - kb0;      // key tiles (none: no row of the tile has a segment)
+  // the producer's place in the ring, and its first copies, under way while the rest of the CTA sets up
+  uint32_t in_slot = 0, in_phase = 1;      // (the first round waits on the phase before the first: free)
+  auto fetch = [&](const CUtensorMap* map, int j) -> bool {      // lo, then hi: the order in which the products take them
+    for (int pl = 1; pl >= 0; --pl) {
+      if (!mbar_wait(&b_free[in_slot], in_phase, abort_flag)) return false;
+      load_plane<128, DP>(ring + in_slot * L::kPlane, map, &b_full[in_slot], (kb0 + j) * 128, hk, pl);
+      if (++in_slot == NS) { in_slot = 0; in_phase ^= 1; }
+    }
+    return true;
+  };
+  bool fetched = true;
+  if (threadIdx.x == 0 && n > 0) {
+    load_tile<128, DP>(sq, &map_q, b_x, qt * 128, h);
+    fetched = fetch(&map_k, 0) && (n < 2 || fetch(&map_k, 1));
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t t_s = tmem, t_p = tmem + 256, t_o = tmem + 384, o_step = (NB - 1) * DP;      // (from one accumulator to the next)
-  const int kb0 = b_min < p.T ? b_min / 128 : qt + 1, n = qt + 1 - kb0;      // key tiles (none: no row of the tile has a segment)
 
   if (warp == 0) {
-    if ((threadIdx.x & 31) == 0 && n > 0) {
-      load_tile<128, DP>(sq, &map_q, b_x, qt * 128, h);
-      uint32_t slot = 0, phase = 1;      // (the first round waits on the phase before the first: free)
-      auto fetch = [&](const CUtensorMap* map, int j) -> bool {      // lo, then hi: the order in which the products take them
-        for (int pl = 1; pl >= 0; --pl) {
-          if (!mbar_wait(&b_free[slot], phase, abort_flag)) return false;
-          load_plane<128, DP>(ring + slot * L::kPlane, map, &b_full[slot], (kb0 + j) * 128, hk, pl);
-          if (++slot == NS) { slot = 0; phase ^= 1; }
-        }
-        return true;
-      };
-      bool ok = fetch(&map_k, 0) && (n < 2 || fetch(&map_k, 1));
+    if (threadIdx.x == 0 && n > 0) {
+      bool ok = fetched;
       for (int j = 0; j < n && ok; ++j) ok = fetch(&map_v, j) && (j + 2 >= n || fetch(&map_k, j + 2));
       if (*abort_flag) let_land(bars, 1 + NS);
     }
@@ -695,45 +705,55 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
     mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();      // (the copies below come before the other warps have seen the barriers)
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   wait_for_last_kernel();
   const int kt = p.order[p.tiles + block / p.parts / p.hk];
   const int4 range = p.ranges[kt];
   const int e_min = range.z, e_max = range.w;
+  const int per = e_max > 0 ? (e_max - 1) / 128 - kt + 1 : 0, n = per * heads;
+  // the producer's place in the ring and in the stream, and its first copies, under way while the rest of the CTA sets up
+  uint32_t in_slot = 0, in_phase = 1;      // (the first round waits on the phase before the first: free)
+  struct Place { int i, head, note; } q_at{0, h0, 0}, g_at{0, h0, 0};
+  auto fetch = [&](const CUtensorMap* map, Place& at) -> bool {      // lo, then hi: the order in which the products take them
+    for (int pl = 1; pl >= 0; --pl) {
+      if (!mbar_wait(&b_free[in_slot], in_phase, abort_flag)) return false;
+      load_plane<128, DP>(ring + in_slot * L::kPlane, map, &b_full[in_slot], (kt + at.i) * 128, at.head, pl);
+      if (++in_slot == NS) { in_slot = 0; in_phase ^= 1; }
+    }
+    return true;
+  };
+  auto on = [&](Place& at) { if (++at.i == per) { at.i = 0; ++at.head; } };
+  auto note_q = [&]() {                    // (its slot is free: the planes have waited for later products than the slot's last)
+    const i64 tile = (i64)q_at.head * p.tiles + kt + q_at.i;
+    Notes<128, 1>& to = notes[q_at.note];
+    uint64_t* bar = &b_note[q_at.note];
+    expect_more(bar, 512);
+    copy_note(to.v[0], p.lift + tile * 128, 512, bar);
+    to.f = make_float4(p.scale * kL2e * fabsf(p.k.inv[(i64)hk * p.tiles + kt]) * fabsf(p.q.inv[tile]), fabsf(p.g.inv[tile]), 0.0f, 0.0f);
+    mbar_arrive(bar);
+    if (++q_at.note == L::kNotes) q_at.note = 0;
+    on(q_at);
+  };
+  auto fetch_q = [&]() -> bool { if (!fetch(&maps.q, q_at)) return false; note_q(); return true; };
+  auto fetch_g = [&]() -> bool { const bool r = fetch(&maps.g, g_at); on(g_at); return r; };
+  bool fetched = true;
+  if (threadIdx.x == 0 && n > 0) {
+    load_tile<128, DP>(sk, &maps.k, b_x, kt * 128, hk);
+    fetched = fetch(&maps.q, q_at);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const uint32_t t_s = tmem, t_p = tmem + 256, t_o = tmem + 384;
-  const int per = e_max > 0 ? (e_max - 1) / 128 - kt + 1 : 0, n = per * heads;
 
   if (warp == 0) {
-    if ((threadIdx.x & 31) == 0 && n > 0) {
-      load_tile<128, DP>(sk, &maps.k, b_x, kt * 128, hk);
-      uint32_t slot = 0, phase = 1;      // (the first round waits on the phase before the first: free)
-      const float sc0 = p.scale * kL2e * fabsf(p.k.inv[(i64)hk * p.tiles + kt]);
-      struct Place { int i, head, note; } q_at{0, h0, 0}, g_at{0, h0, 0};
-      auto fetch = [&](const CUtensorMap* map, Place& at, bool note) -> bool {      // lo, then hi: the order in which the products take them
-        for (int pl = 1; pl >= 0; --pl) {
-          if (!mbar_wait(&b_free[slot], phase, abort_flag)) return false;
-          load_plane<128, DP>(ring + slot * L::kPlane, map, &b_full[slot], (kt + at.i) * 128, at.head, pl);
-          if (++slot == NS) { slot = 0; phase ^= 1; }
-          if (note && pl == 1) {
-            const i64 tile = (i64)at.head * p.tiles + kt + at.i;
-            Notes<128, 1>& to = notes[at.note];
-            expect_more(&b_note[at.note], 512);
-            copy_note(to.v[0], p.lift + tile * 128, 512, &b_note[at.note]);
-            to.f = make_float4(sc0 * fabsf(p.q.inv[tile]), fabsf(p.g.inv[tile]), 0.0f, 0.0f);
-            mbar_arrive(&b_note[at.note]);
-            if (++at.note == L::kNotes) at.note = 0;
-          }
-        }
-        if (++at.i == per) { at.i = 0; ++at.head; }
-        return true;
-      };
-      bool ok = fetch(&maps.q, q_at, true) && (n < 2 || fetch(&maps.q, q_at, true));
-      for (int j = 0; j < n && ok; ++j) ok = fetch(&maps.g, g_at, false) && (j + 2 >= n || fetch(&maps.q, q_at, true));
+    if (threadIdx.x == 0 && n > 0) {
+      note_q();
+      bool ok = fetched && (n < 2 || fetch_q());
+      for (int j = 0; j < n && ok; ++j) ok = fetch_g() && (j + 2 >= n || fetch_q());
       if (*abort_flag) let_land(bars, 1 + NS + L::kNotes);
     }
   } else if (warp == 1) {
@@ -859,7 +879,6 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
   int* ints = (int*)(b_x2 + 1);
   uint32_t* tmem_slot = (uint32_t*)ints + 2;
   volatile int* abort_flag = ints + 3;
-  float* vmax_slot = (float*)ints + 4;
 
   const int warp = threadIdx.x >> 5;
   const int part = DK ? block % p.parts : 0, rest = DK ? block / p.parts : block, x_heads = DK ? p.hk : p.hq;
@@ -870,62 +889,87 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     for (int i = 0; i < N2; ++i) { mbar_init(&b_y2full[i], 1); mbar_init(&b_y2free[i], 1); }
     mbar_init(b_dp, 1); mbar_init(b_ds, kRowWarps); mbar_init(b_o, 1);
     *abort_flag = 0;
-    *vmax_slot = 0.0f;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async_smem();      // (the copies below come before the other warps have seen the barriers)
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   wait_for_last_kernel();
   const int xt = p.order[(DK ? p.tiles : 0) + rest / x_heads];
   const int4 range = p.ranges[xt];
   const int e_min = DK ? range.z : range.x, e_max = DK ? range.w : range.y;
-  __syncthreads();                 // (vmax_slot is 0)
-  {   // longest value row of the head: the scale of dS has to hold |do| |v| twice
-    float m = 0.0f;
-    for (int i = threadIdx.x; i < p.tiles; i += kThreads) m = fmaxf(m, p.v.len[(i64)hk * p.tiles + i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) atomicMax((int*)vmax_slot, __float_as_int(m));      // (not negative: ordered like its bits)
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t t_s = tmem, t_dp = tmem + 2 * N, t_x2 = tmem + 3 * N, t_o = t_x2 + DP;      // (DP columns of X2: hi, lo)
-  const float vmax = *vmax_slot;
   // tiles of Y, in steps of N rows
   int y0, per;
   if (DK) { y0 = xt * R; per = e_max > 0 ? (e_max - 1) / N - y0 + 1 : 0; }
   else { const int last = xt * 128 + 127 < p.T ? xt * 128 + 127 : p.T - 1; y0 = e_min / N; per = e_min < p.T ? last / N - y0 + 1 : 0; }
   const int n = per * heads;
   const CUtensorMap *map_x1 = DK ? &maps.k : &maps.q, *map_y1 = DK ? &maps.qn : &maps.kn, *map_y2 = DK ? &maps.gn : &maps.vn;
+  const i64 x_at = (i64)hx * p.tiles + xt;
+  // The producer: copies of tile (hy, i) into slots s1 and s2, then what goes with it.  The first two tiles are under way while the rest of
+  // the CTA sets up.
+  struct Place { int hy, i; } tile_in{DK ? h0 : hk, 0}, note_in = tile_in;
+  auto on = [&](Place& at) { if (++at.i == per) { at.i = 0; ++at.hy; } };
+  int s1 = 0, s2 = 0, note_s1 = 0;
+  auto copy_y1 = [&]() {                   // (the note's arrival completes the barrier's count)
+    const int y = (y0 + tile_in.i) * N;
+    expect_more(&b_y1full[s1], L::kTileY + (DK ? 2 * N * 4 : 0));
+    copy_tile<N, DP>(y1 + s1 * L::kTileY, map_y1, &b_y1full[s1], y, tile_in.hy);
+    if (DK) {
+      const i64 r = (i64)tile_in.hy * p.tiles * 128 + y;
+      copy_note(notes[s1].v[0], p.lift + r, N * 4, &b_y1full[s1]);
+      copy_note(notes[s1].v[1], p.delta + r, N * 4, &b_y1full[s1]);
+    }
+    if (++s1 == N1) s1 = 0;
+  };
+  auto copy_y2 = [&]() {
+    load_tile<N, DP>(y2 + s2 * L::kTileY, map_y2, &b_y2full[s2], (y0 + tile_in.i) * N, tile_in.hy);
+    if (++s2 == N2) s2 = 0;
+    on(tile_in);
+  };
+  auto write_note = [&]() {                // factors of S, of dP; of what dS is scaled by; of the product
+    const i64 y_at = (i64)note_in.hy * p.tiles + (y0 + note_in.i) * N / 128;
+    const float s_x = p.scale * kL2e * fabsf(DK ? p.k.inv[x_at] : p.q.inv[x_at]), fx2 = fabsf(DK ? p.v.inv[x_at] : p.g.inv[x_at]);
+    const float a = fabsf(DK ? p.q.inv[y_at] : p.k.inv[y_at]), b = fabsf(DK ? p.g.inv[y_at] : p.v.inv[y_at]);
+    notes[note_s1].f = make_float4(s_x * a, b * fx2, DK ? p.g.len[y_at] : 0.0f, a);
+    mbar_arrive(&b_y1full[note_s1]);
+    if (++note_s1 == N1) note_s1 = 0;
+    on(note_in);
+  };
+  const Seat at;
+  uint4 x2[DP / 16];                       // row warps: half a row of X2, hi from groups 0 and 1, lo from 2 and 3
+  float vmax = 0.0f;                       // longest value row of the head: the scale of dS has to hold |do| |v| twice
+  if (threadIdx.x == 0 && n > 0) {
+    load_tile<128, DP>(x1, map_x1, b_x, xt * 128, hx);
+    copy_y1(); copy_y2();
+    if (n > 1) { copy_y1(); copy_y2(); }
+  } else if (warp >= 2) {
+    const Side& side = DK ? p.v : p.g;
+    const int t = xt * 128 + at.row;
+    const uint4* src = reinterpret_cast<const uint4*>(side.planes + ((i64)(at.group >> 1) * x_heads * p.T + (i64)hx * p.T + t) * DP) + (at.group & 1) * (DP / 16);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) x2[i] = t < p.T ? src[i] : make_uint4(0, 0, 0, 0);
+    for (int i = at.lane; i < p.tiles; i += 32) vmax = fmaxf(vmax, p.v.len[(i64)hk * p.tiles + i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t t_s = tmem, t_dp = tmem + 2 * N, t_x2 = tmem + 3 * N, t_o = t_x2 + DP;      // (DP columns of X2: hi, lo)
 
   if (warp == 0) {
-    if ((threadIdx.x & 31) == 0 && n > 0) {
-      load_tile<128, DP>(x1, map_x1, b_x, xt * 128, hx);
-      const i64 x_at = (i64)hx * p.tiles + xt;
-      const float s_x = p.scale * kL2e * fabsf(DK ? p.k.inv[x_at] : p.q.inv[x_at]), fx2 = fabsf(DK ? p.v.inv[x_at] : p.g.inv[x_at]);
-      const DsScale row_scale = DK ? DsScale{} : ds_scale(p.g.len[x_at], vmax);
-      int hy = DK ? h0 : hk, i = 0, s1 = 0, s2 = 0;
-      uint32_t phase1 = 1, phase2 = 1;      // (the first round waits on the phase before the first: free)
-      for (int j = 0; j < n; ++j) {
-        const int y = (y0 + i) * N;
-        const i64 y_at = (i64)hy * p.tiles + y / 128;
-        // factors of S, of dP, of delta, of the product
-        const float q_inv = fabsf(DK ? p.q.inv[y_at] : p.k.inv[y_at]), g_inv = fabsf(DK ? p.g.inv[y_at] : p.v.inv[y_at]);
-        const DsScale ds = DK ? ds_scale(p.g.len[y_at], vmax) : row_scale;
+    if (threadIdx.x == 0 && n > 0) {
+      write_note();
+      if (n > 1) write_note();
+      uint32_t phase1 = 1, phase2 = 0;     // (the third slot of Y1 is free, the first of Y2 when its product has been formed)
+      for (int j = 2; j < n; ++j) {
         if (!mbar_wait(&b_y1free[s1], phase1, abort_flag)) break;
-        notes[s1].f = make_float4(s_x * q_inv, g_inv * ds.to * fx2, ds.to, q_inv * ds.back);
-        if (DK) {
-          expect_more(&b_y1full[s1], 2 * N * 4);
-          copy_note(notes[s1].v[0], p.lift + y_at * 128 + y % 128, N * 4, &b_y1full[s1]);
-          copy_note(notes[s1].v[1], p.delta + y_at * 128 + y % 128, N * 4, &b_y1full[s1]);
-        }
-        load_tile<N, DP>(y1 + s1 * L::kTileY, map_y1, &b_y1full[s1], y, hy);
+        copy_y1();
+        if (s1 == 0) phase1 ^= 1;
+        write_note();
         if (!mbar_wait(&b_y2free[s2], phase2, abort_flag)) break;
-        load_tile<N, DP>(y2 + s2 * L::kTileY, map_y2, &b_y2full[s2], y, hy);
-        if (++s1 == N1) { s1 = 0; phase1 ^= 1; }
-        if (++s2 == N2) { s2 = 0; phase2 ^= 1; }
-        if (++i == per) { i = 0; ++hy; }
+        copy_y2();
+        if (s2 == 0) phase2 ^= 1;
       }
       if (*abort_flag) let_land(bars, 1 + N1 + N2);
     }
@@ -977,46 +1021,44 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
       }
     }
   } else {
-    const Seat at;
     const int t = xt * 128 + at.row;
     const int mine = DK ? (t < p.T ? p.end[t] : 0) : (t < p.T ? p.begin[t] : p.T);
-    {   // X2 into tensor memory: hi from groups 0 and 1, lo from 2 and 3, half a row each
-      uint4 w[DP / 16];
-      const Side& x2 = DK ? p.v : p.g;
-      const uint4* src = reinterpret_cast<const uint4*>(x2.planes + ((i64)(at.group >> 1) * x_heads * p.T + (i64)hx * p.T + t) * DP) + (at.group & 1) * (DP / 16);
-#pragma unroll
-      for (int i = 0; i < DP / 16; ++i) w[i] = t < p.T ? src[i] : make_uint4(0, 0, 0, 0);
-      if constexpr (DP == 64) tmem_st16(t_x2 + at.group * 16 + at.lane_off, reinterpret_cast<const uint32_t*>(w));
-      else tmem_st32(t_x2 + at.group * 32 + at.lane_off, reinterpret_cast<const uint32_t*>(w));
-      operand_written(b_x2, at.lane);
-    }
+    if constexpr (DP == 64) tmem_st16(t_x2 + at.group * 16 + at.lane_off, reinterpret_cast<const uint32_t*>(x2));
+    else tmem_st32(t_x2 + at.group * 32 + at.lane_off, reinterpret_cast<const uint32_t*>(x2));
+    operand_written(b_x2, at.lane);
+    // (addresses of this thread's quarters as sums of their own: taken apart at every use, one build read S of groups 1 to 3 fifteen columns off)
+    const uint32_t my_s = t_s + at.group * H + at.lane_off, my_dp = my_s + 2 * N, my_o = t_o + at.group * W + at.lane_off;
+    DsScale ds{};
+    if (!DK) ds = ds_scale(p.g.len[x_at], vmax);
     float lift_row = 0.0f, delta_row = 0.0f;
     if (!DK) { const i64 r = ((i64)hx * p.tiles + xt) * 128 + at.row; lift_row = p.lift[r]; delta_row = p.delta[r]; }
     float acc[W], f_last = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
     bool ok = true;
-    int y = y0 * N, s1 = 0;
-    uint32_t phase1 = 0;
+    int y = y0 * N, slot = 0;
+    uint32_t phase = 0;
     for (int j = 0; j < n; ++j) {
       const int c0 = y + at.group * H;
       const bool crossed = DK ? y < xt * 128 + 128 || y + N > e_min : y + N > xt * 128 || y < e_max;
       // (the slot is filled again only after the product of this tile, which waits for this tile's dS)
-      if (!mbar_wait(&b_y1full[s1], phase1, abort_flag)) { ok = false; break; }
-      const Notes<N, 2>& note = notes[s1];
+      if (!mbar_wait(&b_y1full[slot], phase, abort_flag)) { ok = false; break; }
+      const Notes<N, 2>& note = notes[slot];
       const float4 f = note.f;
+      if (DK) ds = ds_scale(f.z, vmax);
       if (!mbar_wait(&b_s[j & 1], (j >> 1) & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
       float v[H];
-      load_cols<H>(t_s + (j & 1) * N + at.group * H + at.lane_off, v);
+      load_cols<H>(my_s + (j & 1) * N, v);
       if (DK) weights_of_cols<H>(v, f.x, note.v[0] + at.group * H);
       else weights_of_row<H>(v, f.x, lift_row);
       if (!mbar_wait(b_dp, j & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
       {
         float d[H];
-        load_cols<H>(t_dp + at.group * H + at.lane_off, d);
-        const float2 f1 = make_float2(f.y, f.y), f2 = make_float2(-f.z, -f.z);
+        load_cols<H>(my_dp, d);
+        const float f_dp = f.y * ds.to;
+        const float2 f1 = make_float2(f_dp, f_dp), f2 = make_float2(-ds.to, -ds.to);
         float2 da = mul2(make_float2(delta_row, delta_row), f2), db = da;
 #pragma unroll
         for (int i = 0; i < H; i += 4) {
@@ -1030,15 +1072,15 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
       uint32_t r[H];
       split_operand<H>(v, r);
       // (a quarter's dS lies within its own quarter of S)
-      store_operand<H>(t_s + (j & 1) * N + at.group * H + at.lane_off, r);
+      store_operand<H>(my_s + (j & 1) * N, r);
       if (j > 0) {
         if (!mbar_wait(b_o, (j - 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
-        add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
+        add_part<W>(my_o, acc, f_last);
       }
       operand_written(b_ds, at.lane);
-      f_last = f.w;
-      if (++s1 == N1) { s1 = 0; phase1 ^= 1; }
+      f_last = f.w * ds.back;
+      if (++slot == N1) { slot = 0; phase ^= 1; }
       y += N;
       if (DK && y == (y0 + per) * N) y = y0 * N;
     }
@@ -1046,7 +1088,7 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
       ok = mbar_wait(b_o, (n - 1) & 1, abort_flag);
       if (ok) {
         tc_fence_after();
-        add_part<W>(t_o + at.group * W + at.lane_off, acc, f_last);
+        add_part<W>(my_o, acc, f_last);
       }
     }
     const int row0 = xt * 128 + at.quarter * 32;
