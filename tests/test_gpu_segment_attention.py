@@ -187,3 +187,14 @@ def test_gradients_may_go_to_the_descriptors_of_the_inputs(vb):
         vb.vb_check(vb.lib().vb_read(x.slot, 0, a.ctypes.data_as(vb.c_f32p), a.size))
         vb.lib().vb_release(x.slot, None)
         assert (a == b).all()
+
+
+@pytest.mark.parametrize("hq,hk,dk", [(4, 2, 64), (6, 1, 64), (6, 1, 96), (4, 4, 40)])
+def test_several_heads_of_a_group_in_one_block(vb, hq, hk, dk):
+    """Enough tiles that a key head's gradient is not dealt out to a block for each query head, or to fewer than all."""
+    T, starts = 3300, [0, 3, 350, 351, 900, 1200, 1200, 1800, 2303, 2305, 3000, 3290]
+    q, k, v, g = rnd(60, T, hq, dk, scale=1.3), rnd(61, T, hk, dk, scale=1.3), rnd(62, T, hk, dk), rnd(63, T, hq, dk, scale=0.01)
+    scale = 1.0 / np.sqrt(dk)
+    got = run(vb, q, k, v, starts, scale, g)
+    vb.check_errors()
+    check(got, *segment_attention(q, k, v, starts, scale, g, err=True))

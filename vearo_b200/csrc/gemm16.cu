@@ -8,7 +8,9 @@
 // = 64 k values of a 128 x 256 tile, both planes: 96 KB, two stages.  A run of k is one accumulator of 256 tensor-memory columns, two of them
 // in flight, so the adding warps work on one while the next is formed; a tile's epilogue hides under the next tile's first
 // runs the same way.  Both operands may lie K-major or MN-major in memory: half precision takes either through the same
-// 128-byte swizzle, so no operand is ever laid out twice.
+// 128-byte swizzle, so no operand is ever laid out twice.  Tensor-bound under the power limit: 8192 x 50304 x 768 (RowStats) 1258 us, 503 TFLOP/s
+// useful, 1510 issued at 1.53 GHz; dx and dW of 4097 rows, 1024 x 25152 columns (Store) 989 us, 427 useful.  k_split16 is HBM-bound: 4097 x 1024 and
+// 50304 x 1024 in 81 us, 5.5 TB/s read and written.
 #include "gemm16.h"
 #include "split16.cuh"
 
@@ -522,8 +524,8 @@ int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter) {
     ProblemDev& q = p.prob[i];
     const i64 tm = (g.M + kBM - 1) / kBM, tn = (g.N + kBN - 1) / kBN, runs = (g.K + 127) / 128;
     q.M = (int)g.M; q.N = (int)g.N; q.K = (int)g.K; q.tiles_m = (int)tm;
-    // A tile whose sum is longer than an SM's share of the launch is formed in parts of that length, eight runs at least (2 rows, width 880,
-    // 45893 columns: dx is four tiles of 359 runs, 1158 us a gradient pass in one part, PARTS_US in PARTS_N).
+    // A tile whose sum is longer than an SM's share of the launch is formed in parts of that length, eight runs at least (few rows, width 1024,
+    // 50304 columns: dx is four tiles of 393 runs; with 64 rows, forward and gradients 1259 us in one part, 450 so).
     q.parts = 1;
     q.part_k = (int)(runs * 128);
     if (what == Tile16::Store) {

@@ -6,7 +6,9 @@
 // Forward: one product whose tiles leave (max, sum of exp) for each row and 128 columns, 8 bytes where the logits would be 512, and
 // the target's logit; a second kernel joins the pairs of a row.  Backward: pieces of the vocabulary; a piece's logits are formed
 // again and leave the tensor core as dz in half-precision planes (the operand of the two products that follow), and one launch
-// adds the piece to dx and writes its rows of dW.  Tensor-bound: 2 N V D and 6 N V D operations, three instructions each (gemm16.cu).
+// adds the piece to dx and writes its rows of dW.  Tensor-bound: 2 N V D and 6 N V D operations, three instructions each (gemm16.cu):
+// 8192 rows, 768 x 50304: 1.39 to 1.56 ms forward, as the power limit has it; 4097 rows, 1024 x 50304, with the gradients 4.6 to 4.9 ms.
+// Up to 16 rows it is bound by the bytes of W and takes them in 32 bits (below).
 #include "gemm16.h"
 #include "head_loss.h"
 #include "split16.cuh"

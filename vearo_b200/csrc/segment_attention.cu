@@ -21,6 +21,13 @@
 //   k_backward  dV: S^T = K Q^T, P^T from the saved lse, dV += P^T dO, over the query heads of the group (no atomics)
 //               dQ: S = Q K^T, dP = dO V^T, dQ += dS K;  dK: the same with the roles of rows and columns exchanged
 // Every wait is bounded; when one runs out the CTA raises the device error word, frees its tensor memory and returns.
+//
+// Bound by the tensor cores where texts are long (16384 tokens, 8 + 2 heads of 128: k_forward 1067 us, 517 TFLOP/s useful, 1550 issued, at the
+// 1.53 GHz that the power limit leaves), by what a CTA does before its first tile and after its last where they are short: about 10 of 23
+// thousand cycles for four tiles (4096 tokens in 9 texts, 16 + 4 heads of 64: k_forward 55 us, k_backward 172; 8 texts of 1024, 12 heads: 73), and by
+// the chain of tiles of the longest text where there are fewer CTAs than SMs (1357 of 1531 tokens, 6 + 2 heads of 80: 35 and 66 us).
+// 128 x 128 tiles and one CTA an SM: two streamed operands, four planes each, fill shared memory, and scores in two buffers with what
+// follows from them tensor memory; two smaller CTAs an SM, and one that takes tiles from a counter, measured no better.
 #include "segment_attention.h"
 #include "split16.cuh"
 
@@ -111,7 +118,8 @@ __device__ void plan_order(const PrepareDev& p, const float* starts, int which, 
 // A CTA turns 128 rows of a head into planes.  The first head's CTAs find their rows' segments as well, and one or two CTAs more plan the
 // order of the tiles.  All that a CTA wants of global memory is asked for before the first of it is used, and the offsets are searched
 // in shared memory where they fit: with few tiles the kernel is as long as its longest chain of waits (1531 tokens, 6 + 2 heads of 80, for the
-// gradient: 23.6 us with the offsets searched and delta formed a load at a time).
+// gradient: 23.6 us with the offsets searched and delta formed a load at a time, 12.6 so).  HBM-bound with many: 8192 rows of 36 heads of 64 in
+// 25 us, 6 TB/s read and written.
 template <int DP, bool GRAD>
 __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p) {
   constexpr int kLanes = DP / 4, kRows = 256 / kLanes, kPasses = 128 / kRows;      // lanes of a row, rows of a pass
@@ -1219,11 +1227,13 @@ int backward(Work& w, float* dq, float* dk, float* dv) {
   AttnParams& p = w.p;
   VB_TRY(make_map(&m.q, in[0], p.T, DP, 128)); VB_TRY(make_map(&m.k, in[1], p.T, DP, 128)); VB_TRY(make_map(&m.g, in[3], p.T, DP, 128));
   VB_TRY(make_map(&m.qn, in[0], p.T, DP, N)); VB_TRY(make_map(&m.kn, in[1], p.T, DP, N)); VB_TRY(make_map(&m.vn, in[2], p.T, DP, N)); VB_TRY(make_map(&m.gn, in[3], p.T, DP, N));
-  // A CTA that walks the query heads of a whole group is the longest of the launch: where dK and dV have fewer than four CTAs for
-  // every SM the group is dealt to several, whose sums are added afterwards.
+  // A CTA that walks the query heads of a whole group is the longest of the launch, and dealing the group to several costs their parts' sums and
+  // more CTAs.  So it is dealt out until a CTA's heads are no more than an SM's share of the launch: 3 tiles' worth for every query head.
+  // Gradient, group in one CTA / dealt to as many as make four for every SM / by this rule: 4096 tokens in 9 texts, 16 + 4 heads of 64 131 / 176 / 131 us;
+  // 1531 in 3, 6 + 2 of 80 113 / 63 / 63; 1024 in one, 16 + 2 of 64 122 / 53 / 45; 8192 in 4, 16 + 4 of 128 884 / 1000 / 889.
   const int group = p.hq / p.hk;
   p.parts = 1;
-  for (int d = 2; d <= group && (i64)p.tiles * p.hk * p.parts < 4 * ctx().sm_count; ++d) if (group % d == 0) p.parts = d;
+  for (int d = 2; d <= group && (i64)group * ctx().sm_count > 3 * (i64)p.tiles * p.hq * p.parts; ++d) if (group % d == 0) p.parts = d;
   const i64 n = (i64)p.T * p.hk * p.dk;
   Temp hold;
   p.dq = dq; p.dk_ = dk; p.dv = dv;
