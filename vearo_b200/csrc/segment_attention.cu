@@ -49,7 +49,7 @@ struct PlanesDev { const float* x; i64 st, sh; __half* planes; float* inv; float
 struct PrepareDev {
   PlanesDev in[4];
   int n, T, tiles, dk, hq;
-  const float* starts; int n_seg; int* begin; int* end; int4* ranges; int* order; int* err;      // where the segment of each row begins and ends, and the ranges of a tile's rows
+  const float* starts; int n_seg; int* begin; int* end; int4* plan; int* err;      // where the segment of each row begins and ends, and the tiles' order with their rows' ranges
   const float* o; i64 o_st, o_sh; bool o_vec; const float* lse;                     // for do: delta and 14 - lse in base 2, padded to whole tiles
   float* delta; float* lift;
 };
@@ -63,56 +63,76 @@ __device__ __forceinline__ int segment_of(const PrepareDev& p, const float* star
   }
   return lo > 0 && lo <= p.n_seg ? lo - 1 : -1;
 }
-// Where the segment of row t begins and ends (rows of no segment: an empty range).  Offsets that decrease or leave [0, T] are
-// reported; whatever they are, every range stays inside [0, T].
-__device__ __forceinline__ int2 find_segment(const PrepareDev& p, const float* starts, int t) {
+// Where the segment of row t begins and ends (rows of no segment: (T, 0)); whatever the offsets are, inside [0, T].
+__device__ __forceinline__ int2 segment_at(const PrepareDev& p, const float* starts, int t) {
+  const int s = segment_of(p, starts, t);
+  if (s < 0) return make_int2(p.T, 0);
+  const float fb = roundf(starts[s]), fe = roundf(starts[s + 1]);
+  const int b = fb > 0.0f ? (int)fb : 0, e = fe < (float)p.T ? (int)fe : p.T;
+  return b <= t && t < e ? make_int2(b, e) : make_int2(p.T, 0);
+}
+// A row's segment.  Offsets that decrease or leave [0, T] are reported.
+__device__ __forceinline__ void find_segment(const PrepareDev& p, const float* starts, int t) {
   for (int i = t; i <= p.n_seg; i += p.tiles * 128) {
     const float s = starts[i];
     if (!(s > -0.5f)) atomicOr(p.err, ERRBIT_NEG_ID);
     else if (!(s < (float)p.T + 0.5f) || (i > 0 && !(starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
   }
-  if (t >= p.T) return make_int2(p.T, 0);
-  int b = p.T, e = 0;
-  const int s = segment_of(p, starts, t);
-  if (s >= 0) {
-    const float fb = roundf(starts[s]), fe = roundf(starts[s + 1]);
-    b = fb > 0.0f ? (int)fb : 0;
-    e = fe < (float)p.T ? (int)fe : p.T;
-    if (!(b <= t && t < e)) { b = p.T; e = 0; }
-  }
-  p.begin[t] = b; p.end[t] = e;
-  return make_int2(b, e);
+  if (t >= p.T) return;
+  const int2 r = segment_at(p, starts, t);
+  p.begin[t] = r.x; p.end[t] = r.y;
+}
+// rows [x, y) are those with a segment
+__device__ __forceinline__ int2 live_rows(const PrepareDev& p, const float* starts) {
+  const float first = roundf(starts[0]), behind = roundf(starts[p.n_seg]);
+  return make_int2(first > 0.0f ? (int)fminf(first, (float)p.T) : 0, behind < (float)p.T ? (int)fmaxf(behind, 0.0f) : p.T);
 }
 
-// Tiles in the order of the work that their rows have ahead of them (which = 0: as queries, how far back their segment begins; 1: as keys,
-// how far on it ends), the most first: a sort by count into 1024 classes, four a thread.  (Tiles of a class come in any order: it
-// decides when a tile is worked on, not how.)
+// What the other kernels want to know of a tile, in the order in which they take the tiles: (tile, smallest and largest begin of its rows' segments) for
+// tiles of queries (which = 0), (tile, smallest and largest end) for tiles of keys (1); a row of no segment counts as (T, 0).  The order is by the
+// work that the rows have ahead of them, the most first: a sort by count into 1024 classes, four a thread.  (Tiles of a class come in any
+// order: it decides when a tile is worked on, not how.)
 constexpr int kClasses = 1024;
-__device__ void plan_order(const PrepareDev& p, const float* starts, int which, int* classes, int* warp_sums) {
-  int* order = p.order + which * p.tiles;
+__device__ void plan_tiles(const PrepareDev& p, const float* starts, int which, int* classes, int* warp_sums) {
+  int4* plan = p.plan + which * p.tiles;
   *reinterpret_cast<int4*>(classes + threadIdx.x * 4) = make_int4(0, 0, 0, 0);
-  __syncthreads();
-  auto class_of = [&](int tile) -> int {
-    const int t = which == 0 ? tile * 128 : min(p.T - 1, tile * 128 + 127), s = segment_of(p, starts, t);
-    int n = 0;
-    if (s >= 0) n = which == 0 ? tile - (int)fmaxf(roundf(starts[s]), 0.0f) / 128 : ((int)fminf(roundf(starts[s + 1]), (float)p.T) - 1) / 128 - tile;
-    return kClasses - 1 - max(0, min(n, kClasses - 1));
+  const int2 live = live_rows(p, starts);
+  auto look = [&](int tile) -> int4 {      // and its class
+    const int first = max(tile * 128, live.x), last = min(tile * 128 + 127, live.y - 1);
+    int2 a = make_int2(p.T, 0), b = a;
+    if (first <= last) { a = segment_at(p, starts, first); b = segment_at(p, starts, last); }
+    const bool dead = first > tile * 128 || last < tile * 128 + 127;
+    int4 r;
+    int n;
+    if (which == 0) { r = make_int4(tile, min(a.x, b.x), dead ? p.T : max(a.x, b.x), 0); n = r.y < p.T ? tile - r.y / 128 : 0; }
+    else { r = make_int4(tile, dead ? 0 : min(a.y, b.y), max(a.y, b.y), 0); n = r.z > 0 ? (r.z - 1) / 128 - tile : 0; }
+    r.w = kClasses - 1 - max(0, min(n, kClasses - 1));
+    return r;
   };
-  for (int i = threadIdx.x; i < p.tiles; i += 256) atomicAdd(&classes[class_of(i)], 1);
+  __syncthreads();
+  int4 mine = make_int4(0, 0, 0, 0);       // (a thread's first tile is looked at once)
+  for (int i = threadIdx.x; i < p.tiles; i += 256) {
+    const int4 r = look(i);
+    if (i == (int)threadIdx.x) mine = r;
+    atomicAdd(&classes[r.w], 1);
+  }
   __syncthreads();
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;      // counts into places
   const int4 n = *reinterpret_cast<int4*>(classes + threadIdx.x * 4);
   int before = n.x + n.y + n.z + n.w;
-  const int mine = before;
+  const int all = before;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const int x = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += x; }
   if (lane == 31) warp_sums[wid] = before;
   __syncthreads();
-  before -= mine;
+  before -= all;
   for (int i = 0; i < wid; ++i) before += warp_sums[i];
   *reinterpret_cast<int4*>(classes + threadIdx.x * 4) = make_int4(before, before + n.x, before + n.x + n.y, before + n.x + n.y + n.z);
   __syncthreads();
-  for (int i = threadIdx.x; i < p.tiles; i += 256) order[atomicAdd(&classes[class_of(i)], 1)] = i;
+  for (int i = threadIdx.x; i < p.tiles; i += 256) {
+    const int4 r = i == (int)threadIdx.x ? mine : look(i);
+    plan[atomicAdd(&classes[r.w], 1)] = r;
+  }
 }
 
 // A CTA turns 128 rows of a head into planes.  The first head's CTAs find their rows' segments as well, and one or two CTAs more plan the
@@ -125,7 +145,6 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   constexpr int kLanes = DP / 4, kRows = 256 / kLanes, kPasses = 128 / kRows;      // lanes of a row, rows of a pass
   __shared__ float red[8], row_delta[128], offsets[1024];
   __shared__ uint32_t bad[4];
-  __shared__ int4 range[4];
   __shared__ __align__(16) int classes[kClasses];
   const int tile = blockIdx.x;
   const bool plans = tile == p.tiles;
@@ -138,13 +157,12 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   const bool mine = c < p.dk;
   const i64 t0 = (i64)tile * 128 + r0;
   // Rows before the first segment and behind the last may hold anything: they are not read, and as zeros do not reach the tile's exponent.
-  const float first = roundf(p.starts[0]), behind = roundf(p.starts[p.n_seg]);
-  const int live0 = first > 0.0f ? (int)fminf(first, (float)p.T) : 0, live1 = behind < (float)p.T ? (int)fmaxf(behind, 0.0f) : p.T;
+  const int2 live = live_rows(p, p.starts);
   const float* src = x.x + t0 * x.st + h * x.sh + c;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     v[i] = make_float4(0, 0, 0, 0);
-    if (mine && t0 + i * kRows >= live0 && t0 + i * kRows < live1) {
+    if (mine && t0 + i * kRows >= live.x && t0 + i * kRows < live.y) {
       const float* s = src + i * kRows * x.st;
       if (x.vec) v[i] = __ldcs(reinterpret_cast<const float4*>(s));
       else { v[i].x = s[0]; if (c + 1 < p.dk) v[i].y = s[1]; if (c + 2 < p.dk) v[i].z = s[2]; if (c + 3 < p.dk) v[i].w = s[3]; }
@@ -161,18 +179,8 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
       starts = offsets;
     }
     __syncthreads();
-    if (plans) { plan_order(p, starts, blockIdx.y, classes, (int*)red); return; }
-    if (threadIdx.x < 128) {             // the rows' segments and the range of their ends
-      const int2 s = find_segment(p, starts, tile * 128 + threadIdx.x);
-      const int4 r = make_int4(__reduce_min_sync(0xffffffffu, s.x), __reduce_max_sync(0xffffffffu, s.x), __reduce_min_sync(0xffffffffu, s.y), __reduce_max_sync(0xffffffffu, s.y));
-      if ((threadIdx.x & 31) == 0) range[threadIdx.x >> 5] = r;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int4 r = range[0];
-      for (int i = 1; i < 4; ++i) { r.x = min(r.x, range[i].x); r.y = max(r.y, range[i].y); r.z = min(r.z, range[i].z); r.w = max(r.w, range[i].w); }
-      p.ranges[tile] = r;
-    }
+    if (plans) { plan_tiles(p, starts, blockIdx.y, classes, (int*)red); return; }
+    if (threadIdx.x < 128) find_segment(p, starts, tile * 128 + threadIdx.x);
   } else __syncthreads();
   if (with_delta) {      // delta of the rows
     const float* o = p.o + t0 * p.o_st + h * p.o_sh + c;
@@ -471,8 +479,7 @@ struct AttnParams {
   int steps;                                  // of 16 components in a head
   float scale;
   const int* begin; const int* end;
-  const int* order;                           // [2][tiles] tiles by the work they have as queries, and as keys, the most first
-  const int4* ranges;                         // [tiles] smallest and largest begin, smallest and largest end of the tile's rows
+  const int4* plan;                           // [2][tiles] (plan_tiles)
   Side q, k, v, g;
   const float* lift; const float* delta;      // [hq][tiles * 128]: 14 - lse in base 2 (a weight comes with a factor of 2^14), delta
   float* out; float* lse;                     // forward
@@ -534,19 +541,17 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
   const int warp = threadIdx.x >> 5;
   const int h = blockIdx.x % p.hq, hk = h / (p.hq / p.hk);
   if (warp == 0) { prefetch_map(&map_q); prefetch_map(&map_k); prefetch_map(&map_v); }
-  if (threadIdx.x == 0) {
-    mbar_init(b_x, 1);
-    for (int i = 0; i < NS; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_free[i], 1); }
-    mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
-    *abort_flag = 0;
+  if (warp == 0) {
+    for (int i = threadIdx.x; i < L::kBars; i += 32) mbar_init(&bars[i], &bars[i] == b_p ? kRowWarps : 1);
+    if (threadIdx.x == 0) *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();      // (the copies below come before the other warps have seen the barriers)
+    __syncwarp();
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   wait_for_last_kernel();
-  const int qt = p.order[blockIdx.x / p.hq];
-  const int4 range = p.ranges[qt];
-  const int b_min = range.x, b_max = range.y;
+  const int4 tile = p.plan[blockIdx.x / p.hq];
+  const int qt = tile.x, b_min = tile.y, b_max = tile.z;
   const int kb0 = b_min < p.T ? b_min / 128 : qt + 1, n = qt + 1 - kb0;      // key tiles (none: no row of the tile has a segment)
   // the producer's place in the ring, and its first copies, under way while the rest of the CTA sets up
   uint32_t in_slot = 0, in_phase = 1;      // (the first round waits on the phase before the first: free)
@@ -706,20 +711,17 @@ __device__ __forceinline__ void grad_v(uint8_t* smem, const BwdMaps& maps, const
 
   const int warp = threadIdx.x >> 5;
   const int part = block % p.parts, hk = block / p.parts % p.hk, heads = p.hq / p.hk / p.parts, h0 = (hk * p.parts + part) * heads;
-  if (threadIdx.x == 0) {
-    mbar_init(b_x, 1);
-    for (int i = 0; i < NS; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_free[i], 1); }
-    for (int i = 0; i < L::kNotes; ++i) mbar_init(&b_note[i], 1);
-    mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1); mbar_init(b_p, kRowWarps); mbar_init(b_o, 1);
-    *abort_flag = 0;
+  if (warp == 0) {
+    for (int i = threadIdx.x; i < L::kBars; i += 32) mbar_init(&bars[i], &bars[i] == b_p ? kRowWarps : 1);
+    if (threadIdx.x == 0) *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();      // (the copies below come before the other warps have seen the barriers)
+    __syncwarp();
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   wait_for_last_kernel();
-  const int kt = p.order[p.tiles + block / p.parts / p.hk];
-  const int4 range = p.ranges[kt];
-  const int e_min = range.z, e_max = range.w;
+  const int4 planned = p.plan[p.tiles + block / p.parts / p.hk];
+  const int kt = planned.x, e_min = planned.y, e_max = planned.z;
   const int per = e_max > 0 ? (e_max - 1) / 128 - kt + 1 : 0, n = per * heads;
   // the producer's place in the ring and in the stream, and its first copies, under way while the rest of the CTA sets up
   uint32_t in_slot = 0, in_phase = 1;      // (the first round waits on the phase before the first: free)
@@ -891,20 +893,17 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
   const int warp = threadIdx.x >> 5;
   const int part = DK ? block % p.parts : 0, rest = DK ? block / p.parts : block, x_heads = DK ? p.hk : p.hq;
   const int hx = rest % x_heads, hk = DK ? hx : hx / (p.hq / p.hk), heads = DK ? p.hq / p.hk / p.parts : 1, h0 = DK ? (hk * p.parts + part) * heads : hx;
-  if (threadIdx.x == 0) {
-    mbar_init(b_x, 1); mbar_init(b_x2, kRowWarps); mbar_init(&b_s[0], 1); mbar_init(&b_s[1], 1);
-    for (int i = 0; i < N1; ++i) { mbar_init(&b_y1full[i], 1); mbar_init(&b_y1free[i], 1); }
-    for (int i = 0; i < N2; ++i) { mbar_init(&b_y2full[i], 1); mbar_init(&b_y2free[i], 1); }
-    mbar_init(b_dp, 1); mbar_init(b_ds, kRowWarps); mbar_init(b_o, 1);
-    *abort_flag = 0;
+  if (warp == 0) {
+    for (int i = threadIdx.x; i < L::kBars; i += 32) mbar_init(&bars[i], &bars[i] == b_x2 || &bars[i] == b_ds ? kRowWarps : 1);
+    if (threadIdx.x == 0) *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async_smem();      // (the copies below come before the other warps have seen the barriers)
+    __syncwarp();
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   wait_for_last_kernel();
-  const int xt = p.order[(DK ? p.tiles : 0) + rest / x_heads];
-  const int4 range = p.ranges[xt];
-  const int e_min = DK ? range.z : range.x, e_max = DK ? range.w : range.y;
+  const int4 planned = p.plan[(DK ? p.tiles : 0) + rest / x_heads];
+  const int xt = planned.x, e_min = planned.y, e_max = planned.z;      // (DK: of the ends, else of the begins)
   // tiles of Y, in steps of N rows
   int y0, per;
   if (DK) { y0 = xt * R; per = e_max > 0 ? (e_max - 1) / N - y0 + 1 : 0; }
@@ -1175,7 +1174,7 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
     planes[i] = take((size_t)2 * heads[i] * s.T * dp * 2);
     inv[i] = take((size_t)heads[i] * tiles * 4); len[i] = take((size_t)heads[i] * tiles * 4); bad[i] = take((size_t)heads[i] * tiles * 16);
   }
-  const size_t begin = take((size_t)s.T * 4), end = take((size_t)s.T * 4), ranges = take((size_t)tiles * sizeof(int4)), order = take((size_t)tiles * 8);
+  const size_t begin = take((size_t)s.T * 4), end = take((size_t)s.T * 4), plan = take((size_t)tiles * 2 * sizeof(int4));
   const size_t delta = o ? take((size_t)s.hq * tiles * 512) : 0, lift = o ? take((size_t)s.hq * tiles * 512) : 0;
   VB_TRY(scratch_alloc(at, &w.hold.p));
   uint8_t* base = (uint8_t*)w.hold.p;
@@ -1189,12 +1188,12 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
     *sides[i] = Side{d.in[i].planes, d.in[i].inv, d.in[i].len, d.in[i].bad};
     all += heads[i];
   }
-  d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.ranges = (int4*)(base + ranges); d.order = (int*)(base + order); d.err = ctx().d_err;
+  d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.plan = (int4*)(base + plan); d.err = ctx().d_err;
   if (o) { d.o = o->p; d.o_st = o->st; d.o_sh = o->sh; d.lse = lse;
            d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lift = (float*)(base + lift); }
   AttnParams& p = w.p;
   p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.steps = (s.dk + 15) / 16; p.scale = s.scale;
-  p.begin = d.begin; p.end = d.end; p.ranges = d.ranges; p.order = d.order; p.lift = d.lift; p.delta = d.delta; p.err = ctx().d_err;
+  p.begin = d.begin; p.end = d.end; p.plan = d.plan; p.lift = d.lift; p.delta = d.delta; p.err = ctx().d_err;
   ProfScope prof("segment_attn_prepare", 8.0 * (double)s.T * all * s.dk);
   const dim3 grid(tiles + 1, all);
   if (dp == 64) { if (o) k_prepare<64, true><<<grid, 256, 0, ctx().stream>>>(d); else k_prepare<64, false><<<grid, 256, 0, ctx().stream>>>(d); }
