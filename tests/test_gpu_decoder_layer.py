@@ -154,3 +154,27 @@ def test_another_current_device_does_not_matter(vb):
         assert np.isfinite(q.segment_attention(q, q, vb.Tensor.from_numpy(np.array([0, 8], np.float32))).numpy()).all()
     finally:
         torch.cuda.set_device(0)
+
+
+def test_one_tensor_in_every_place(vb):
+    """Queries, keys and values the same tensor, one weight for both norms: its gradients add up."""
+    T, h, dk, starts = 90, 2, 32, [0, 33, 90]
+    x, w, r = rnd(400, T, h, dk), 1 + rnd(401, dk, scale=0.1), rnd(402, T, h, dk)
+    vb.zero_gradients(); vb.reset_active_tape()
+    X, W, POS = vb.Tensor.from_numpy(x, True), vb.Tensor.from_numpy(w, True), vb.Tensor.from_numpy(np.arange(T, dtype=np.float32))
+    ST, R = vb.Tensor.from_numpy(np.asarray(starts, np.float32)), vb.Tensor.from_numpy(r)
+    q, k = X.qk_norm_rope(X, W, W, POS)
+    q.segment_attention(k, X, ST).mul(R).reshape([1, T * h * dk]).sum(1).backward()
+    a = q.segment_attention(q, q, ST)      # (and in one call)
+    assert np.isfinite(a.numpy()).all()
+    X64, W64 = (torch.tensor(v, dtype=torch.float64, requires_grad=True) for v in (x, w))
+    y = X64 * torch.rsqrt((X64 * X64).mean(-1, keepdim=True) + 1e-6) * W64
+    ang = torch.arange(T, dtype=torch.float64)[:, None, None] * 10000.0 ** (-2.0 * torch.arange(dk // 2, dtype=torch.float64) / dk)
+    y = torch.cat([y[..., : dk // 2] * ang.cos() - y[..., dk // 2 :] * ang.sin(), y[..., : dk // 2] * ang.sin() + y[..., dk // 2 :] * ang.cos()], -1)
+    seg = np.searchsorted(starts, np.arange(T), side="right")
+    mask = torch.tensor((seg[:, None] == seg[None]) & (np.arange(T)[:, None] >= np.arange(T)[None]))
+    s = (torch.einsum("thd,shd->hts", y, y) * dk ** -0.5).masked_fill(~mask, -1e300)
+    (torch.einsum("hts,shd->thd", torch.softmax(s, -1), X64) * torch.tensor(r, dtype=torch.float64)).sum().backward()
+    for got, want in ((X.grad(), X64.grad), (W.grad(), W64.grad)):
+        # some hundred roundings on the way from a sum of a few hundred terms of order one: 2^-24 * 1000 of the largest
+        assert np.abs(got.contiguous().numpy() - want.numpy()).max() <= 1000 * 2.0 ** -24 * np.abs(want.numpy()).max()
