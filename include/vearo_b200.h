@@ -255,7 +255,7 @@ int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k_or_null, con
  * device error flag.  Scores are scale * q.k; p = exp(score - lse), without the 1e-9 of vb_fused_attention.  lse (may be NULL) is
  * [Hq, T], the natural log of a row's sum of exponentials; the backward call wants it and out.  dk <= 128, Hq <= 1024, T <= 2^24.
  * Components that are not finite: a row that sees one in q, k or v has NaN output and lse, and gradients that it enters are NaN; rows that do
- * not see it are unaffected. */
+ * not see it are unaffected.  The first row of a segment sees itself alone: its score has no gradient, exactly. */
 int vb_segment_attention(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, vb_tensor* out, vb_tensor* lse_or_null);
 int vb_segment_attention_backward(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, const vb_tensor* out,
                                   const vb_tensor* lse, const vb_tensor* grad_out, vb_tensor* dq, vb_tensor* dk, vb_tensor* dv);

@@ -198,3 +198,17 @@ def test_several_heads_of_a_group_in_one_block(vb, hq, hk, dk):
     got = run(vb, q, k, v, starts, scale, g)
     vb.check_errors()
     check(got, *segment_attention(q, k, v, starts, scale, g, err=True))
+
+
+def test_the_first_row_of_a_segment_has_no_gradient_of_its_score(vb):
+    """It sees itself alone: its weight is 1, and queries and keys of texts of one token have gradients of 0, not of rounding."""
+    T, starts = 7, [0, 1, 2, 5, 6]
+    q, k, v, g = rnd(70, T, 8, 96, scale=3.0), rnd(71, T, 4, 96, scale=3.0), rnd(72, T, 4, 96, scale=30.0), rnd(73, T, 8, 96)
+    got = run(vb, q, k, v, starts, 0.1, g)
+    check(got, *segment_attention(q, k, v, starts, 0.1, g, err=True))
+    assert (got[2][[0, 1, 2, 5, 6]] == 0).all() and (got[3][[0, 1, 5, 6]] == 0).all()
+    assert (got[2][[3, 4]] != 0).any() and (got[4][:6] != 0).any()
+    k[5, 1, 3] = np.nan                                        # (a text of one token that is not finite: NaN, as in longer ones)
+    got = run(vb, q, k, v, starts, 0.1, g)
+    assert np.isnan(got[0][5, 2:4]).all() and np.isnan(got[2][5, 2:4]).any(-1).all() and np.isnan(got[3][5, 1]).any() and np.isnan(got[4][5, 1]).any()
+    assert all(np.isfinite(x[r]).all() for x in (got[0], *got[2:]) for r in (0, 1, 2, 3, 4))

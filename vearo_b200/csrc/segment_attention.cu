@@ -1029,7 +1029,16 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     }
   } else {
     const int t = xt * 128 + at.row;
-    const int mine = DK ? (t < p.T ? p.end[t] : 0) : (t < p.T ? p.begin[t] : p.T);
+    // The columns that the row sees, without itself where it is the first of its segment: such a query sees one key, whose weight is 1 whatever the
+    // score, so its dS is 0, where do . v - delta would be the difference of two roundings of one sum.  (NaN stays NaN.)
+    int from = p.T, to = 0;
+    bool lone = false;
+    if (t < p.T) {
+      const int first = p.begin[t];
+      lone = first == t;
+      if (DK) { from = lone ? t + 1 : t; to = p.end[t] - 1; }
+      else { from = first; to = t; }
+    }
     if constexpr (DP == 64) tmem_st16(t_x2 + at.group * 16 + at.lane_off, reinterpret_cast<const uint32_t*>(x2));
     else tmem_st32(t_x2 + at.group * 32 + at.lane_off, reinterpret_cast<const uint32_t*>(x2));
     operand_written(b_x2, at.lane);
@@ -1038,7 +1047,7 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     DsScale ds{};
     if (!DK) ds = ds_scale(p.g.len[x_at], vmax);
     float lift_row = 0.0f, delta_row = 0.0f;
-    if (!DK) { const i64 r = ((i64)hx * p.tiles + xt) * 128 + at.row; lift_row = p.lift[r]; delta_row = p.delta[r]; }
+    if (!DK) { const i64 r = ((i64)hx * p.tiles + xt) * 128 + at.row; lift_row = p.lift[r]; delta_row = p.delta[r]; if (lone && lift_row == lift_row) to = t - 1; }
     float acc[W], f_last = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
@@ -1075,7 +1084,11 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
           v[i] = a.x; v[i + 1] = a.y; v[i + 2] = b.x; v[i + 3] = b.y;
         }
       }
-      if (crossed) keep_columns<H>(v, (DK ? t : mine) - c0, (DK ? mine - 1 : t) - c0, 0.0f);
+      if (crossed) {
+        int lo = from - c0;
+        if (DK && lone && t >= c0 && t < c0 + H && note.v[0][at.group * H + t - c0] != note.v[0][at.group * H + t - c0]) --lo;
+        keep_columns<H>(v, lo, to - c0, 0.0f);
+      }
       uint32_t r[H];
       split_operand<H>(v, r);
       // (a quarter's dS lies within its own quarter of S)
