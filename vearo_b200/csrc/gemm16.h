@@ -44,7 +44,7 @@ struct Product16 {
   const float* lse;                              // [M]
   Split16 grad;                                  // [M, N]
 };
-// n <= 2 (Store), independent of one another, one launch; counter: an int on the device that is 0 when the launch begins.  The RowStats
+// n <= 2 (Store), independent of one another, one launch (and one for each whose long sums are formed in parts); counter: an int on the device that is 0 when the launch begins.  The RowStats
 // kernel may start while the kernel ahead of it runs and waits for it by itself.
 int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter);
 

@@ -136,7 +136,7 @@ __device__ void plan_tiles(const PrepareDev& p, const float* starts, int which, 
 }
 
 // A CTA turns 128 rows of a head into planes.  The first head's CTAs find their rows' segments as well, and one or two CTAs more plan the
-// order of the tiles.  All that a CTA wants of global memory is asked for before the first of it is used, and the offsets are searched
+// order of the tiles.  All that a CTA wants of global memory, but the two ends of the offsets, is asked for before the first of it is used, and the offsets are searched
 // in shared memory where they fit: with few tiles the kernel is as long as its longest chain of waits (1531 tokens, 6 + 2 heads of 80, for the
 // gradient: 23.6 us with the offsets searched and delta formed a load at a time, 12.6 so).  HBM-bound with many: 8192 rows of 36 heads of 64 in
 // 25 us, 6 TB/s read and written.
