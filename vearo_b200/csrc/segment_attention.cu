@@ -665,11 +665,7 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
       if (j > 0 && NB == 2) add_part<W>(t_o + ((j - 1) & 1) * o_step + at.group * W + at.lane_off, acc, keep, v_last);
       keep = shrink; v_last = v_this;
     }
-    if (n > 0) {
-      ok = mbar_wait(b_o, (n - 1) & 1, abort_flag) && ok;
-      tc_fence_after();
-      add_part<W>(t_o + ((n - 1) & 1) * o_step + at.group * W + at.lane_off, acc, keep, v_last);
-    }
+    // the row's sum, while the last product is formed
     float* x = xchg + (n & (NB - 1)) * G * 128 + at.row;
     if (NB == 1) asm volatile("bar.sync %0, 128;" ::"r"(1 + at.quarter) : "memory");
     x[at.group * 128] = l;
@@ -677,6 +673,11 @@ k_forward(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUt
     l = (x[0] + x[128]) + (x[256] + x[384]);
     if (q_inv < 0.0f && begin <= t && ((p.q.bad[((i64)h * p.tiles + qt) * 4 + at.quarter] >> at.lane) & 1)) l = __int_as_float(0x7fffffff);
     const bool dead = l == 0.0f;
+    if (n > 0) {
+      ok = mbar_wait(b_o, (n - 1) & 1, abort_flag) && ok;
+      tc_fence_after();
+      add_part<W>(t_o + ((n - 1) & 1) * o_step + at.group * W + at.lane_off, acc, keep, v_last);
+    }
     const int row0 = qt * 128 + at.quarter * 32;
     if (ok) {
       store_rows<W>((float4*)sq + (at.quarter * G + at.group) * 8 * W, acc, dead ? 0.0f : 1.0f / l, p.out + ((i64)row0 * p.hq + h) * p.dk, (i64)p.hq * p.dk, p.T - row0,
