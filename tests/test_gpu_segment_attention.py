@@ -212,3 +212,19 @@ def test_the_first_row_of_a_segment_has_no_gradient_of_its_score(vb):
     got = run(vb, q, k, v, starts, 0.1, g)
     assert np.isnan(got[0][5, 2:4]).all() and np.isnan(got[2][5, 2:4]).any(-1).all() and np.isnan(got[3][5, 1]).any() and np.isnan(got[4][5, 1]).any()
     assert all(np.isfinite(x[r]).all() for x in (got[0], *got[2:]) for r in (0, 1, 2, 3, 4))
+
+
+def test_keys_broadcast_over_heads_and_rows_in_reverse(vb):
+    """A view with a stride of 0 or a negative one is read in place: the same bits as its copy."""
+    T, dk, starts = 200, 64, [0, 90, 200]
+    q, k, g = rnd(80, T, 4, dk), rnd(81, T, 1, dk), rnd(82, T, 4, dk)
+    many = np.repeat(k, 2, 1)
+    want = run(vb, q, many, many, starts, 0.125, g)
+    Q, K, G = Dev(vb, q[::-1]), Dev(vb, k), Dev(vb, g)
+    K.desc.dims[1], K.desc.strides[1] = 2, 0
+    Q.desc.offset, Q.desc.strides[0] = (T - 1) * 4 * dk, -4 * dk
+    S, O, LSE = Dev(vb, np.asarray(starts, np.float32)), Dev(vb, want[0]), Dev(vb, want[1])
+    got = outputs(vb, vb.lib().vb_segment_attention, Q, K, K, S, 0.125, n=2)
+    got += outputs(vb, vb.lib().vb_segment_attention_backward, Q, K, K, S, 0.125, O, LSE, G, n=3)
+    for a, b in zip(got, want):
+        assert (a == b).all()
