@@ -235,7 +235,7 @@ int vb_layernorm_backward_accum(const vb_tensor* x, const vb_tensor* w, const vb
  * Output descriptors are written last, so they may be those of inputs.  Matrix products run on pairs of half-precision planes that share a power
  * of two per block: 22 significant bits for magnitudes down to 2^-17 of the block's largest, an absolute error of 2^-40 of that largest below.  A
  * block is 128 rows of a head in vb_segment_attention (rows of no segment count as 0), 128 x 128 of the weight and 128 columns of a row of x in
- * vb_linear_cross_entropy (up to 16 rows: plain f32).
+ * vb_linear_cross_entropy (up to 16 rows, or few rows times few columns: plain f32).
  *
  * RMS norm of every head and the rotary position turn, one pass for queries and keys (k, wk, k_out all NULL: queries alone):
  *   y = w * x / sqrt(mean(x^2) + eps);   pair j of a head turned by positions[t] * theta^(-2j / rot_dim).

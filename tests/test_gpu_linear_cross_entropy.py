@@ -277,3 +277,22 @@ def test_few_rows(vb, n, d, v):
         vb.vb_check(L.vb_read(o.slot, 0, a.ctypes.data_as(vb.c_f32p), a.size))
         L.vb_release(o.slot, None)
         assert (a == want).all()
+
+
+@pytest.mark.parametrize("n,d,v", [(17, 64, 700), (33, 128, 512), (100, 1024, 300), (500, 260, 200), (600, 36, 60), (18, 2048, 1), (150, 68, 64)])
+def test_gradients_of_few_blocks(vb, n, d, v):
+    """Several groups of rows and so few columns that one wave of blocks has them all; rows left out hold NaN."""
+    x, w = rnd(60, n, d), rnd(61, v, d, scale=2.0 / np.sqrt(d))
+    t = np.random.default_rng(62).integers(0, v, n).astype(np.float32)
+    t[1::5] = -1
+    (lse, loss, gx, gw), (e_lse, e_loss, egx, egw) = truth(x, w, t, -1, 2.0)
+    x[1::5] = np.nan
+    D = [Dev(vb, a) for a in (x, w, t)]
+    got_loss, got_lse = outputs(vb, vb.lib().vb_linear_cross_entropy, *D, -1, n=2)
+    assert (np.abs(got_lse - lse) <= e_lse)[t != -1].all() and abs(got_loss[0] - loss) <= e_loss
+    rest = (*D, -1, Dev(vb, got_lse), Dev(vb, np.array([2.0], np.float32)))
+    got = outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *rest, n=2)
+    vb.check_errors()
+    assert (np.abs(got[0] - gx) <= egx).all() and (np.abs(got[1] - gw) <= egw).all()
+    for a, b in zip(got, outputs(vb, vb.lib().vb_linear_cross_entropy_backward, *rest, n=2)):
+        assert (a == b).all()

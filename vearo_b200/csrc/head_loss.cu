@@ -8,7 +8,7 @@
 // again and leave the tensor core as dz in half-precision planes (the operand of the two products that follow), and one launch
 // adds the piece to dx and writes its rows of dW.  Tensor-bound: 2 N V D and 6 N V D operations, three instructions each (gemm16.cu):
 // 8192 rows, 768 x 50304: 1.39 to 1.56 ms forward, as the power limit has it; 4097 rows, 1024 x 50304, with the gradients 4.6 to 4.9 ms.
-// Up to 16 rows it is bound by the bytes of W and takes them in 32 bits (below).
+// Up to 16 rows it is bound by the bytes of W and takes them in 32 bits, and so do small products of more rows (below).
 #include "gemm16.h"
 #include "head_loss.h"
 #include "split16.cuh"
@@ -131,7 +131,7 @@ struct FewParams {
   i64 ignore;
   int n, d, v;
   float2* stats; float* target_value; int* target; int* ticket;             // forward
-  const float *lse, *g; float *gw, *gx_part;                                // backward; gx_part: [CTAs][n][d]
+  const float *lse, *g; float *gw, *gx_part;                                // backward; gw: [groups of NR rows][v][d], gx_part: [CTAs][n][d]
   int* err;
 };
 template <int NR, bool GRAD>
@@ -159,10 +159,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) k_few_rows(FewParams p) {
   }
   if (!GRAD && tid == 0 && blockIdx.x == 0 && blockIdx.y == 0) *p.ticket = 0;
   __syncthreads();
-  if (GRAD && tid == 0) {
+  if (GRAD) {
     int live = 0;
-    for (int i = 0; i < NR; ++i) live += target[i] != kNoTarget;
-    coef = *p.g / (float)(live > 0 ? live : 1);
+    for (int i0 = 0; i0 < p.n; i0 += kFewThreads) {
+      const int i = i0 + tid;
+      live += __syncthreads_count(i < p.n && read_target(p.targets[i], p.ignore, p.v, p.err) != kNoTarget);
+    }
+    if (tid == 0) coef = *p.g / (float)(live > 0 ? live : 1);
   }
   for (int i = tid * 4; i < NR * d; i += kFewThreads * 4) {      // (backward, a row that is left out may hold anything)
     const int n = i / d;
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) k_few_rows(FewParams p) {
           }
           if (p.gw) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) if (v0 + r0 + r < p.v) __stcs(reinterpret_cast<float4*>(p.gw + (i64)(v0 + r0 + r) * d + col), dw[r]);
+            for (int r = 0; r < 4; ++r) if (v0 + r0 + r < p.v) __stcs(reinterpret_cast<float4*>(p.gw + ((i64)blockIdx.y * p.v + v0 + r0 + r) * d + col), dw[r]);
           }
         }
       }
@@ -280,14 +283,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) k_few_rows(FewParams p) {
       }
     }
     __syncthreads();
-    float* to = p.gx_part + (i64)blockIdx.x * p.n * d;
-    for (int i = tid * 4; i < p.n * d; i += kFewThreads * 4) *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(xs + i);
+    float* to = p.gx_part + ((i64)blockIdx.x * p.n + row0) * d;
+    for (int i = tid * 4; i < rows * d; i += kFewThreads * 4) *reinterpret_cast<float4*>(to + i) = *reinterpret_cast<const float4*>(xs + i);
   }
 }
 // the CTAs' parts added in a fixed order: 32 numbers x 32 lanes of parts a CTA
 __global__ void __launch_bounds__(1024) k_sum_few(const float* __restrict__ part, float* __restrict__ out, int numbers, int parts) {
   __shared__ float sm[32][33];
-  wait_for_last_kernel();
   const int at = blockIdx.x * 32 + threadIdx.x;
   float s = 0.0f;
   if (at < numbers) {
@@ -302,6 +304,19 @@ __global__ void __launch_bounds__(1024) k_sum_few(const float* __restrict__ part
     for (int i = 0; i < 32; ++i) t += sm[i][threadIdx.x];
     out[at] = t;
   }
+}
+// the groups' parts of dW added in order
+__global__ void __launch_bounds__(256) k_sum_groups(const float4* __restrict__ part, float4* __restrict__ out, int numbers, int groups) {
+  wait_for_last_kernel();
+  const int at = blockIdx.x * 256 + threadIdx.x;
+  if (at >= numbers) return;
+  float4 s = part[at];
+#pragma unroll 4
+  for (int i = 1; i < groups; ++i) {
+    const float4 a = part[(i64)i * numbers + at];
+    s = make_float4(s.x + a.x, s.y + a.y, s.z + a.z, s.w + a.w);
+  }
+  out[at] = s;
 }
 bool few_fit(i64 d) { return d % 4 == 0 && d <= kFewWidth; }
 // the matrix where it is, or a copy that begins on 16 bytes (the same kernel for either: the same bits)
@@ -371,9 +386,13 @@ int launch_head_loss(const float* x, const float* w, const float* targets, i64 i
 int launch_head_loss_backward(const float* x, const float* w, const float* targets, i64 ignore, const float* lse, const float* g, float* gx, float* gw,
                               i64 n, i64 d, i64 v) {
   Temp hx, hk, hw, hz, ht;
-  if (n <= kFewRows && few_fit(d)) {
+  const i64 few_blocks = (v + kFewCols - 1) / kFewCols, few_groups = (n + kFewRows - 1) / kFewRows;
+  // Up to 16 rows, or one wave of blocks that are not wide (a block's three products take 16 x 64 x d each on the ordinary cores) and not of many groups (whose
+  // parts of dW are added).  With gradients, this way / by way of planes, us: 17 rows of 64, 700 columns 38 / 52; 100 of 512, 1000: 54 / 72; 500 of 128, 256: 49 / 57;
+  // and left to the planes 64 of 1024, 300: 74 / 70; 1000 of 512, 128: 96 / 78; 2000 of 256, 64: 89 / 76.
+  if (few_fit(d) && (n <= kFewRows || (few_blocks * few_groups <= ctx().sm_count && d <= 512 && d * few_groups <= 8192))) {
     VB_TRY(on_16_bytes(&x, n * d, hk)); VB_TRY(on_16_bytes(&w, v * d, hw));
-    const i64 blocks = (v + kFewCols - 1) / kFewCols, ctas = blocks < ctx().sm_count ? blocks : ctx().sm_count;
+    const i64 ctas = few_blocks < ctx().sm_count ? few_blocks : ctx().sm_count;
     FewParams p{};
     p.x = x; p.w = w; p.targets = targets; p.ignore = ignore; p.n = (int)n; p.d = (int)d; p.v = (int)v;
     p.lse = lse; p.g = g; p.gw = gw; p.err = ctx().d_err;
@@ -381,8 +400,18 @@ int launch_head_loss_backward(const float* x, const float* w, const float* targe
       VB_TRY(scratch_alloc((size_t)(ctas * n * d) * sizeof(float), &hx.p));
       p.gx_part = (float*)hx.p;
     }
-    VB_TRY(few_rows<true>(p, (unsigned)ctas, 1));
-    if (gx) return launch_early(k_sum_few, dim3((unsigned)((n * d + 31) / 32)), dim3(32, 32), 0, (const float*)hx.p, gx, (int)(n * d), (int)ctas);
+    if (gw && few_groups > 1) {
+      VB_TRY(scratch_alloc((size_t)(few_groups * v * d) * sizeof(float), &hz.p));
+      p.gw = (float*)hz.p;
+    }
+    VB_TRY(few_rows<true>(p, (unsigned)ctas, (unsigned)few_groups));
+    if (gw && few_groups > 1)
+      VB_TRY(launch_early(k_sum_groups, dim3((unsigned)((v * d / 4 + 255) / 256)), dim3(256), 0, (const float4*)hz.p, (float4*)gw, (int)(v * d / 4), (int)few_groups));
+    if (gx) {
+      const dim3 grid((unsigned)((n * d + 31) / 32));
+      k_sum_few<<<grid, dim3(32, 32), 0, ctx().stream>>>((const float*)hx.p, gx, (int)(n * d), (int)ctas);
+      VB_LAUNCH_CHECK();
+    }
     return VB_OK;
   }
   i64 piece = kPieceBytes / (4 * n) / 256 * 256;
