@@ -20,7 +20,7 @@ def sources():
 
 
 def _deps(src):
-    d = [src] + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "host", "*.h")) + \
+    d = [src] + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(CSRC, "host", "*.h")) + \
         glob.glob(os.path.join(os.path.dirname(HERE), "include", "*.h"))
     return d
 
