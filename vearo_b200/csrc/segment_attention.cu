@@ -235,7 +235,9 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   if (with_delta && threadIdx.x < 128) {      // and 14 minus their lse in base 2 (a row of no segment: -infinity, so that every p is 0)
     const float d = row_delta[threadIdx.x];
     const bool dead = lse == -INFINITY;
-    if (d != d) lse = d;                      // (a gradient that is not finite: dv sees it through p)
+    // A row of do with a component that is not finite, which the planes hold as 0: every gradient that the row enters sees it through p.  (One
+    // infinity leaves delta infinite and not NaN.)
+    if (!is_finite(d) || ((bad[threadIdx.x >> 5] >> (threadIdx.x & 31)) & 1)) lse = __int_as_float(0x7fffffff);
     const i64 at = ((i64)h * p.tiles + tile) * 128 + threadIdx.x;
     p.lift[at] = dead ? -INFINITY : 14.0f - lse * kL2e;
     p.delta[at] = dead ? 0.0f : d;
