@@ -234,7 +234,8 @@ int vb_layernorm_backward_accum(const vb_tensor* x, const vb_tensor* w, const vb
  * on the library's device whatever device is current, and are refused (VB_ERR_UNSUPPORTED) while the compute stream is being captured.
  * Output descriptors are written last, so they may be those of inputs.  Matrix products run on pairs of half-precision planes that share a power
  * of two per block: 22 significant bits for magnitudes down to 2^-17 of the block's largest, an absolute error of 2^-40 of that largest below.  A
- * block is 128 rows of a head in vb_segment_attention (rows of no segment count as 0), 128 x 128 of the weight and 128 columns of a row of x in
+ * block is 128 rows of a head in vb_segment_attention (rows of no segment count as 0; the gradient of a row's scores is held to 2^-37 of the longest
+ * gradient row of 128 times twice the longest value row of the row's own segment), 128 x 128 of the weight and 128 columns of a row of x in
  * vb_linear_cross_entropy (up to 16 rows, or few rows times few columns: plain f32).
  *
  * RMS norm of every head and the rotary position turn, one pass for queries and keys (k, wk, k_out all NULL: queries alone):
@@ -253,7 +254,9 @@ int vb_qk_norm_rope_backward(const vb_tensor* q, const vb_tensor* k_or_null, con
  * [starts[i], starts[i + 1]), and a row sees the rows of its segment up to itself.  Segments may be empty; rows before the first or
  * behind the last belong to none: they may hold anything, their output and gradients are 0, their lse is -infinity.  Offsets that decrease or leave [0, T] set the
  * device error flag.  Scores are scale * q.k; p = exp(score - lse), without the 1e-9 of vb_fused_attention.  lse (may be NULL) is
- * [Hq, T], the natural log of a row's sum of exponentials; the backward call wants it and out.  dk <= 128, Hq <= 1024, T <= 2^24.
+ * [Hq, T], the natural log of a row's sum of exponentials; the backward call wants it and out, as the forward call gave them for the same q, k, v,
+ * starts and scale (another out may be longer than the values, and then leaves the range in which the gradients of scores are held).  scale > 0,
+ * dk <= 128, Hq <= 1024, T <= 2^24.
  * Components that are not finite: a row that sees one in q, k or v has NaN output and lse, and gradients that it enters are NaN; rows that do
  * not see it are unaffected.  The first row of a segment sees itself alone: its score has no gradient, exactly. */
 int vb_segment_attention(const vb_tensor* q, const vb_tensor* k, const vb_tensor* v, const vb_tensor* starts, float scale, vb_tensor* out, vb_tensor* lse_or_null);

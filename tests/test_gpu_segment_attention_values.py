@@ -4,7 +4,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from tests.decoder_ops_util import Dev, outputs, rnd
+from tests.decoder_ops_util import Dev, outputs, rnd, segment_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,48 @@ def test_a_gradient_that_is_not_finite_is_not_lost(vb, dk, row, value):
     # what the row does not enter is what it was
     for got, want, entered in ((dq, clean[0], mine), (dk_, clean[1], seen), (dv, clean[2], seen)):
         assert (got[~entered] == want[~entered]).all()
+
+
+def bounded_by_text(q, k, v, starts, scale, g):
+    """Gradients in 64 bits and bounds, every text by itself: what one text holds has no place in another's bound, but for the exponent that the
+    planes of a tile of 128 rows share: a value of a tile is good to 2^-40 of the tile's largest."""
+    T = len(q)
+    vals, errs = [np.zeros(a.shape) for a in (q, k, v)], [np.zeros(a.shape) for a in (q, k, v)]
+    a = np.abs
+    group = q.shape[1] // k.shape[1]
+    for b, e in zip(starts[:-1].astype(int), starts[1:].astype(int)):
+        (_, _, *got), (_, _, *err) = segment_attention(q[b:e], k[b:e], v[b:e], [0, e - b], scale, g[b:e], err=True)
+        tiles = slice(b // 128 * 128, min(T, -(-e // 128) * 128))
+        shared = {name: 2.0 ** -40 * a(x[tiles]).max() for name, x in (("q", q), ("k", k), ("v", v), ("g", g))}
+        n, dk = e - b, q.shape[2]
+        # dS = p (do . v - do . o): v and, through o, its average each off by the shared step, do too; p is off by the scores' error
+        g1, v1 = a(g[b:e]).sum(-1).max(), a(v[b:e]).sum(-1).max()
+        off = scale * (a(q[b:e]).sum(-1).max() * shared["k"] + a(k[b:e]).sum(-1).max() * shared["q"])
+        ds = scale * (2 * g1 * shared["v"] + 2 * v1 * shared["g"] + 4 * off * g1 * a(v[b:e]).max())      # over p, which sums to 1 over keys, to n at most over queries
+        ds_size = scale * 2 * g1 * a(v[b:e]).max()
+        errs[0][b:e] = err[0] + ds * a(k[b:e]).max() + ds_size * shared["k"]
+        errs[1][b:e] = err[1] + group * n * (ds * a(q[b:e]).max() + ds_size * shared["q"])
+        errs[2][b:e] = err[2] + group * n * (2 * off * a(g[b:e]).max() + shared["g"])
+        for to, x in zip(vals, got):
+            to[b:e] = x
+    return vals, errs
+
+
+@pytest.mark.parametrize("starts,power", [([0, 256, 600], 30), ([0, 384, 512, 900], 30), ([0, 300, 600], 20), ([0, 40, 90, 400], 20)])
+@pytest.mark.parametrize("hq,hk,dk", [(4, 2, 64), (2, 1, 96)])
+@pytest.mark.parametrize("large", [0, 1])
+def test_values_of_one_text_do_not_take_bits_from_another(vb, starts, power, hq, hk, dk, large):
+    """The values of one text 2^power times as large as the others' (by more than 2^20 where no tile of 128 rows holds rows of both)."""
+    starts = np.array(starts, np.float32)
+    T = int(starts[-1])
+    q, k, v = rnd(11, T, hq, dk), rnd(12, T, hk, dk), rnd(13, T, hk, dk)
+    g = rnd(14, T, hq, dk)
+    g = (g / np.sqrt((g * g).sum(-1, keepdims=True))).astype(np.float32)
+    b, e = int(starts[large]), int(starts[large + 1])
+    v[b:e] *= np.float32(2.0 ** power)
+    out, lse = forward(vb, q, k, v, starts, dk ** -0.5)
+    got = gradients(vb, q, k, v, starts, dk ** -0.5, out, lse, g)
+    vb.check_errors()
+    vals, errs = bounded_by_text(q, k, v, starts, dk ** -0.5, g)
+    for x, want, err, name in zip(got, vals, errs, ("dq", "dk", "dv")):
+        assert (np.abs(x - want) <= err).all(), (name, (np.abs(x - want) / np.maximum(err, 1e-300)).max())

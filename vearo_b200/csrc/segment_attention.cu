@@ -52,6 +52,7 @@ struct PrepareDev {
   const float* starts; int n_seg; int* begin; int* end; int4* plan; int* err;      // where the segment of each row begins and ends, and the tiles' order with their rows' ranges
   const float* o; i64 o_st, o_sh; bool o_vec; const float* lse;                     // for do: delta and 14 - lse in base 2, padded to whole tiles
   float* delta; float* lift;
+  float* text_len;                                                                  // [key heads][T], for v: longest of the rows of t's text in t's tile
 };
 
 // The offset of the segment that row t is in (-1: none), as an index into the offsets.
@@ -143,7 +144,8 @@ __device__ void plan_tiles(const PrepareDev& p, const float* starts, int which, 
 template <int DP, bool GRAD>
 __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p) {
   constexpr int kLanes = DP / 4, kRows = 256 / kLanes, kPasses = 128 / kRows;      // lanes of a row, rows of a pass
-  __shared__ float red[8], row_delta[128], offsets[1024];
+  __shared__ float red[8], of_row[128], offsets[1024];      // of_row: delta (do), lengths (v)
+  __shared__ int text_top[128], first_row[128];             // (v) first_row: of the tile's rows, the first of the row's text; -1: no text
   __shared__ uint32_t bad[4];
   __shared__ __align__(16) int classes[kClasses];
   const int tile = blockIdx.x;
@@ -172,7 +174,8 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   float lse = -INFINITY;
   if (with_delta && threadIdx.x < 128 && tile * 128 + (int)threadIdx.x < p.T) lse = p.lse[(i64)h * p.T + tile * 128 + threadIdx.x];
   if (threadIdx.x < 4) bad[threadIdx.x] = 0;
-  if (plans || blockIdx.y == 0) {
+  const bool with_lengths = GRAD && which == 2;
+  if (plans || blockIdx.y == 0 || with_lengths) {
     const float* starts = p.starts;
     if (p.n_seg < 1024) {
       for (int i = threadIdx.x; i <= p.n_seg; i += 256) offsets[i] = p.starts[i];
@@ -180,7 +183,12 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
     }
     __syncthreads();
     if (plans) { plan_tiles(p, starts, blockIdx.y, classes, (int*)red); return; }
-    if (threadIdx.x < 128) find_segment(p, starts, tile * 128 + threadIdx.x);
+    if (threadIdx.x < 128 && blockIdx.y == 0) find_segment(p, starts, tile * 128 + threadIdx.x);
+    if (threadIdx.x < 128 && with_lengths) {
+      const int t = tile * 128 + threadIdx.x, begin = t < p.T ? segment_at(p, starts, t).x : p.T;
+      first_row[threadIdx.x] = begin <= t ? max(begin - tile * 128, 0) : -1;
+      text_top[threadIdx.x] = 0;
+    }
   } else __syncthreads();
   if (with_delta) {      // delta of the rows
     const float* o = p.o + t0 * p.o_st + h * p.o_sh + c;
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
         d = fmaf(g.y, y[i].y, d); d = fmaf(g.z, y[i].z, d); d = fmaf(g.w, y[i].w, d);
 #pragma unroll
         for (int k = kLanes / 2; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
-        if (c == 0) row_delta[(i0 + i) * kRows + r0] = d;
+        if (c == 0) of_row[(i0 + i) * kRows + r0] = d;
       }
     }
   }
@@ -233,7 +241,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   if (lane == 0) red[wid] = m;
   __syncthreads();
   if (with_delta && threadIdx.x < 128) {      // and 14 minus their lse in base 2 (a row of no segment: -infinity, so that every p is 0)
-    const float d = row_delta[threadIdx.x];
+    const float d = of_row[threadIdx.x];
     const bool dead = lse == -INFINITY;
     // A row of do with a component that is not finite, which the planes hold as 0: every gradient that the row enters sees it through p.  (One
     // infinity leaves delta infinite and not NaN.)
@@ -257,6 +265,7 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     top = fmaxf(top, ss);
+    if (with_lengths && c == 0) of_row[i * kRows + r0] = sqrtf(ss) * inv;
     if (t < p.T) {
       uint2 hi, lo;
       split2_finite(y.x, y.y, &hi.x, &lo.x);
@@ -270,7 +279,11 @@ __global__ void __launch_bounds__(256, DP == 64 ? 4 : 2) k_prepare(PrepareDev p)
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   __syncthreads();
   if (lane == 0) red[wid] = top;
+  const int first = with_lengths && threadIdx.x < 128 ? first_row[threadIdx.x] : -1;
+  if (first >= 0) atomicMax(&text_top[first], __float_as_int(of_row[threadIdx.x]));      // (lengths are not negative: ordered as integers)
   __syncthreads();
+  if (with_lengths && threadIdx.x < 128 && tile * 128 + (int)threadIdx.x < p.T)
+    p.text_len[(i64)h * p.T + tile * 128 + threadIdx.x] = first >= 0 ? __int_as_float(text_top[first]) : 0.0f;
   const i64 at = (i64)h * p.tiles + tile;
   if (threadIdx.x == 0) {
 #pragma unroll
@@ -484,6 +497,7 @@ struct AttnParams {
   const int4* plan;                           // [2][tiles] (plan_tiles)
   Side q, k, v, g;
   const float* lift; const float* delta;      // [hq][tiles * 128]: 14 - lse in base 2 (a weight comes with a factor of 2^14), delta
+  const float* text_len;                      // (PrepareDev)
   float* out; float* lse;                     // forward
   float *dq, *dk_, *dv;                       // backward; with parts > 1 dk_ and dv are [parts][T, hk, dk], summed afterwards
   int parts;                                  // a key head's group of query heads is dealt to this many CTAs
@@ -946,7 +960,11 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
   };
   const Seat at;
   uint4 x2[DP / 16];                       // row warps: half a row of X2, hi from groups 0 and 1, lo from 2 and 3
-  float vmax = 0.0f;                       // longest value row of the head: the scale of dS has to hold |do| |v| twice
+  // The scale of a row of dS has to hold |do| |v| twice, delta being an average of do . v: the longest value row that the row's text has (DK), or has
+  // up to the row's tile (dQ).  Texts differ in size, so no other's values count: its own rows of the tiles where it begins and ends, and the
+  // whole tiles between them.
+  float vmax = 0.0f;
+  int begin = p.T, end = 0;                // of the row's text
   if (threadIdx.x == 0 && n > 0) {
     load_tile<128, DP>(x1, map_x1, b_x, xt * 128, hx);
     copy_y1(); copy_y2();
@@ -957,9 +975,23 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     const uint4* src = reinterpret_cast<const uint4*>(side.planes + ((i64)(at.group >> 1) * x_heads * p.T + (i64)hx * p.T + t) * DP) + (at.group & 1) * (DP / 16);
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) x2[i] = t < p.T ? src[i] : make_uint4(0, 0, 0, 0);
-    for (int i = at.lane; i < p.tiles; i += 32) vmax = fmaxf(vmax, p.v.len[(i64)hk * p.tiles + i]);
+    const float *own = p.text_len + (i64)hk * p.T, *whole = p.v.len + (i64)hk * p.tiles;
+    if (t < p.T) { begin = p.begin[t]; end = p.end[t]; vmax = own[t]; }
+    // the text that reaches back out of the tile, if any of the warp's rows is in it, and the one that reaches ahead
+    const int b = (int)__reduce_min_sync(0xffffffffu, (unsigned)begin), e = (int)__reduce_max_sync(0xffffffffu, (unsigned)end);
+    float back = 0.0f, ahead = 0.0f;
+    if (b < xt * 128) {
+      if (at.lane == 0) back = own[b];
+      for (int i = b / 128 + 1 + at.lane; i < xt; i += 32) back = fmaxf(back, whole[i]);
+    }
+    if (DK && e > xt * 128 + 128) {
+      if (at.lane == 0) ahead = own[e - 1];
+      for (int i = xt + 1 + at.lane; i < (e - 1) / 128; i += 32) ahead = fmaxf(ahead, whole[i]);
+    }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+    for (int o = 16; o > 0; o >>= 1) { back = fmaxf(back, __shfl_xor_sync(0xffffffffu, back, o)); ahead = fmaxf(ahead, __shfl_xor_sync(0xffffffffu, ahead, o)); }
+    if (begin < xt * 128) vmax = fmaxf(vmax, back);
+    if (end > xt * 128 + 128) vmax = fmaxf(vmax, ahead);
   }
   tc_fence_before();
   __syncthreads();
@@ -1037,10 +1069,9 @@ __device__ __forceinline__ void grad_qk(uint8_t* smem, const BwdMaps& maps, cons
     int from = p.T, to = 0;
     bool lone = false;
     if (t < p.T) {
-      const int first = p.begin[t];
-      lone = first == t;
-      if (DK) { from = lone ? t + 1 : t; to = p.end[t] - 1; }
-      else { from = first; to = t; }
+      lone = begin == t;
+      if (DK) { from = lone ? t + 1 : t; to = end - 1; }
+      else { from = begin; to = t; }
     }
     if constexpr (DP == 64) tmem_st16(t_x2 + at.group * 16 + at.lane_off, reinterpret_cast<const uint32_t*>(x2));
     else tmem_st32(t_x2 + at.group * 32 + at.lane_off, reinterpret_cast<const uint32_t*>(x2));
@@ -1191,7 +1222,7 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
     inv[i] = take((size_t)heads[i] * tiles * 4); len[i] = take((size_t)heads[i] * tiles * 4); bad[i] = take((size_t)heads[i] * tiles * 16);
   }
   const size_t begin = take((size_t)s.T * 4), end = take((size_t)s.T * 4), plan = take((size_t)tiles * 2 * sizeof(int4));
-  const size_t delta = o ? take((size_t)s.hq * tiles * 512) : 0, lift = o ? take((size_t)s.hq * tiles * 512) : 0;
+  const size_t delta = o ? take((size_t)s.hq * tiles * 512) : 0, lift = o ? take((size_t)s.hq * tiles * 512) : 0, text_len = o ? take((size_t)s.hk * s.T * 4) : 0;
   VB_TRY(scratch_alloc(at, &w.hold.p));
   uint8_t* base = (uint8_t*)w.hold.p;
   PrepareDev& d = w.prep;
@@ -1206,10 +1237,11 @@ int prepare(const SegShape& s, const SegHeads* in, const int* heads, int n, cons
   }
   d.starts = starts; d.n_seg = (int)n_seg; d.begin = (int*)(base + begin); d.end = (int*)(base + end); d.plan = (int4*)(base + plan); d.err = ctx().d_err;
   if (o) { d.o = o->p; d.o_st = o->st; d.o_sh = o->sh; d.lse = lse;
-           d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lift = (float*)(base + lift); }
+           d.o_vec = s.dk % 4 == 0 && o->st % 4 == 0 && o->sh % 4 == 0 && (reinterpret_cast<uintptr_t>(o->p) & 15) == 0; d.delta = (float*)(base + delta); d.lift = (float*)(base + lift);
+           d.text_len = (float*)(base + text_len); }
   AttnParams& p = w.p;
   p.T = (int)s.T; p.tiles = tiles; p.hq = s.hq; p.hk = s.hk; p.dk = s.dk; p.steps = (s.dk + 15) / 16; p.scale = s.scale;
-  p.begin = d.begin; p.end = d.end; p.plan = d.plan; p.lift = d.lift; p.delta = d.delta; p.err = ctx().d_err;
+  p.begin = d.begin; p.end = d.end; p.plan = d.plan; p.lift = d.lift; p.delta = d.delta; p.text_len = d.text_len; p.err = ctx().d_err;
   ProfScope prof("segment_attn_prepare", 8.0 * (double)s.T * all * s.dk);
   const dim3 grid(tiles + 1, all);
   if (dp == 64) { if (o) k_prepare<64, true><<<grid, 256, 0, ctx().stream>>>(d); else k_prepare<64, false><<<grid, 256, 0, ctx().stream>>>(d); }
