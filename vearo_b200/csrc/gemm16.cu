@@ -22,11 +22,13 @@ constexpr int kThreads = 320, kBM = 128, kBN = 256, kBK = 64, kStages = 2, kEpiW
 constexpr int kAPlane = kBM * kBK * 2, kBPlane = kBN * kBK * 2;               // 16 KB, 32 KB
 constexpr int kStage = 2 * kAPlane + 2 * kBPlane;
 constexpr int kStaging = 4096;                                                // a warp's 32 x 32 block: f32, or both planes of halves
-constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kStaging + 256;
+constexpr int kExponents = kEpiWarps * 128;                                   // a warp's bytes for 128 columns
+constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * kStaging + kExponents + 256;
+static_assert(kSmem <= 227 * 1024, "shared memory");
 constexpr float kGradScale = 16384.0f;
 
 // ---- splitting ------------------------------------------------------------------------------------------------------------------
-struct SplitDev { const float* x; const int* keep; __half* planes; float* inv; i64 rows, cols, ld, plane, inv_ld; int cb, blocks; bool vec, by_row; };
+struct SplitDev { const float* x; const int* keep; __half* planes; float* inv; i64 rows, cols, ld, plane, inv_ld; int cb, blocks; bool vec, by_row; };      // (by_row: a scale for 128 columns of a row)
 struct SplitJobs { SplitDev job[3]; TargetRows rows; int* err; };
 __global__ void __launch_bounds__(256) k_split16(const __grid_constant__ SplitJobs jobs) {
   __shared__ float red[8];
@@ -88,10 +90,10 @@ __global__ void __launch_bounds__(256) k_split16(const __grid_constant__ SplitJo
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------
-struct OperandDev { CUtensorMap map; const float* inv; i64 inv_ld; int mn, by_row; };
+struct OperandDev { CUtensorMap map; const float* inv; i64 inv_ld; int mn, by_m; };      // by_m: inv is [128 k][m]
 struct ProblemDev {
   OperandDev a, b;
-  CUtensorMap out_map;                       // Store: f32, where `by_copy`; LossGrad: the planes
+  CUtensorMap out_map;                       // Store: f32, where `by_copy`; LossGrad: the planes of grad
   int M, N, K, tiles_m, tiles;               // tiles: of all parts
   int parts, part_k;                         // Store: the sum over k in parts of part_k steps, each a tile of its own in plane `part` of the result
   float* out; i64 ldo; int add, by_copy;
@@ -109,10 +111,12 @@ __device__ __forceinline__ TileAt tile_at(const ProblemDev& q, int t) {
 struct Params {
   ProblemDev prob[2];
   const int* target; int col0; float2* stats; float* target_value; const float* lse;
+  CUtensorMap col_map; float* col_inv; i64 col_inv_ld; int with_rows, with_cols;      // LossGrad: the planes of grad_by_column and their scales
   int* counter;                              // 0: tiles handed out beyond the first of every CTA
   int* err;
 };
-enum { B_FULL = 0, B_EMPTY = B_FULL + kStages, B_RUN = B_EMPTY + kStages, B_RUNFREE = B_RUN + 2, B_POST = B_RUNFREE + 2, B_TAKEN = B_POST + 2, B_COUNT = B_TAKEN + 2 };
+enum { B_FULL = 0, B_EMPTY = B_FULL + kStages, B_RUN = B_EMPTY + kStages, B_RUNFREE = B_RUN + 2, B_POST = B_RUNFREE + 2, B_TAKEN = B_POST + 2, B_COLS = B_TAKEN + 2, B_COLSREAD = B_COLS + 2, B_COUNT = B_COLSREAD + 2 };
+static_assert(B_COUNT * 8 + 16 <= 256, "barriers");
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // (as an instruction of its own: the compiler's form of atomicAdd waits for the answer on the spot)
@@ -129,12 +133,65 @@ __device__ __forceinline__ void add_block(const CUtensorMap* map, const void* sr
 }
 __device__ __forceinline__ void commit_blocks() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
+// A warp's 32 rows x 128 columns as half planes, 32 x 32 blocks through its staging: 16-byte pieces of a plane's 64-byte row, in the copy
+// engine's 64-byte swizzle.  (Ordinary stores, from the staging or of 32 bytes a thread, took LossGrad from 648 to 780 and 688 us.)
+__device__ __forceinline__ void store_planes(const CUtensorMap* map, uint8_t* stg, const float (&acc)[128], int n0, int row, int N, int M, int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (lane == 0) tma_store_wait_read();
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      uint4 h, l;
+      split2_finite(acc[c * 32 + 8 * e], acc[c * 32 + 8 * e + 1], &h.x, &l.x);
+      split2_finite(acc[c * 32 + 8 * e + 2], acc[c * 32 + 8 * e + 3], &h.y, &l.y);
+      split2_finite(acc[c * 32 + 8 * e + 4], acc[c * 32 + 8 * e + 5], &h.z, &l.z);
+      split2_finite(acc[c * 32 + 8 * e + 6], acc[c * 32 + 8 * e + 7], &h.w, &l.w);
+      const int at = lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4);
+      *reinterpret_cast<uint4*>(stg + at) = h;
+      *reinterpret_cast<uint4*>(stg + 2048 + at) = l;
+    }
+    fence_async_smem();
+    __syncwarp();
+    const int col = n0 + c * 32;
+    if (lane == 0 && col < N && row < M) {
+      store_block(map, stg, col, row, 0);
+      store_block(map, stg + 2048, col, row, 1);
+      commit_blocks();
+    }
+  }
+}
+// The largest magnitudes of columns 4 lane .. 4 lane + 3 among the warp's rows, as the upper seven bits of their exponents, a byte each (all ones:
+// NaN or infinity).  Through the warp's staging, a row of bytes a lane: a butterfly of shuffles over pairs of columns, which take their turns with the
+// operands' way through shared memory, cost 6200 cycles a tile, as did 128 reductions by redux.sync; so 1600.
+__device__ __forceinline__ uint32_t largest_of_columns(const float (&acc)[128], uint8_t* stg, int lane) {
+  if (lane == 0) tma_store_wait_read();
+  __syncwarp();
+  auto tops = [](const float* x) -> uint32_t {
+    const uint32_t a = __byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x73), b = __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x73);
+    return __byte_perm(a, b, 0x5410) & 0x7f7f7f7fu;
+  };
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    *reinterpret_cast<uint4*>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(tops(acc + 16 * e), tops(acc + 16 * e + 4), tops(acc + 16 * e + 8), tops(acc + 16 * e + 12));
+  __syncwarp();
+  uint32_t even = 0, odd = 0;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) {
+    const uint32_t x = *reinterpret_cast<const uint32_t*>(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+    even = __vmaxu2(even, x & 0x00ff00ffu); odd = __vmaxu2(odd, x & 0xff00ff00u);
+  }
+  __syncwarp();
+  return even | odd;
+}
+
 template <Tile16 WHAT>
 __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t* staging = smem + kStages * kStage;
-  uint64_t* bars = (uint64_t*)(staging + kEpiWarps * kStaging);
+  uint32_t* exponents = (uint32_t*)(staging + kEpiWarps * kStaging);      // [halves][quarters][32]: a byte for every column
+  uint64_t* bars = (uint64_t*)(exponents + kExponents / 4);
   uint32_t* tmem_slot = (uint32_t*)(bars + B_COUNT);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile int* posted = abort_flag + 1;       // [2] tiles handed to the other roles
@@ -142,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) { mbar_init(&bars[B_FULL + i], 1); mbar_init(&bars[B_EMPTY + i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&bars[B_RUN + i], 1); mbar_init(&bars[B_RUNFREE + i], kEpiWarps); mbar_init(&bars[B_POST + i], 1); mbar_init(&bars[B_TAKEN + i], 1 + kEpiWarps); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&bars[B_RUN + i], 1); mbar_init(&bars[B_RUNFREE + i], kEpiWarps); mbar_init(&bars[B_POST + i], 1); mbar_init(&bars[B_TAKEN + i], 1 + kEpiWarps); mbar_init(&bars[B_COLS + i], 4); mbar_init(&bars[B_COLSREAD + i], 4); }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -262,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
       const int nb = n0 < q.N ? tn * 2 + half : tn * 2;          // (a half tile past the last column has no scale of its own)
       auto scale_of = [&](int kb) -> float {
         float s = 1.0f;
-        if (q.a.by_row) s = m < q.M ? q.a.inv[kb * q.a.inv_ld + m] : 0.0f;
+        if (q.a.by_m) s = m < q.M ? q.a.inv[kb * q.a.inv_ld + m] : 0.0f;
         else if (q.a.inv) s = q.a.mn ? q.a.inv[(i64)kb * q.a.inv_ld + tm] : q.a.inv[(i64)tm * q.a.inv_ld + kb];
         if (q.b.inv) s *= q.b.mn ? q.b.inv[(i64)kb * q.b.inv_ld + nb] : q.b.inv[(i64)nb * q.b.inv_ld + kb];
         return s;
@@ -369,30 +426,36 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
 #pragma unroll
           for (int c = 0; c < 128; ++c) if (n0 + c >= q.N) acc[c] = 0.0f;
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          // 16-byte pieces of a plane's 64-byte row, in the copy engine's 64-byte swizzle
-          if (lane == 0) tma_store_wait_read();
+        // the exponent of the largest of each column among these 32 rows, for the other quarters of the tile's rows
+        if (p.with_cols) {
+          if (i > 0 && !warp_wait(&bars[B_COLSREAD + half], (i - 1) & 1, abort_flag)) break;      // (the last tile's have been read)
+          exponents[(half * 4 + quarter) * 32 + lane] = largest_of_columns(acc, stg, lane);
           __syncwarp();
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint4 h, l;
-            split2_finite(acc[c * 32 + 8 * e], acc[c * 32 + 8 * e + 1], &h.x, &l.x);
-            split2_finite(acc[c * 32 + 8 * e + 2], acc[c * 32 + 8 * e + 3], &h.y, &l.y);
-            split2_finite(acc[c * 32 + 8 * e + 4], acc[c * 32 + 8 * e + 5], &h.z, &l.z);
-            split2_finite(acc[c * 32 + 8 * e + 6], acc[c * 32 + 8 * e + 7], &h.w, &l.w);
-            const int at = lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4);
-            *reinterpret_cast<uint4*>(stg + at) = h;
-            *reinterpret_cast<uint4*>(stg + 2048 + at) = l;
-          }
-          fence_async_smem();
+          if (lane == 0) mbar_arrive(&bars[B_COLS + half]);
+        }
+        if (p.with_rows) store_planes(&q.out_map, stg, acc, n0, mrow, q.N, q.M, lane);
+        if (p.with_cols) {
+          if (!warp_wait(&bars[B_COLS + half], i & 1, abort_flag)) break;
+          const uint32_t* e = exponents + half * 128 + lane;
+          const uint32_t top = __vmaxu4(__vmaxu4(e[0], e[32]), __vmaxu4(e[64], e[96]));
           __syncwarp();
-          const int col = n0 + c * 32;
-          if (lane == 0 && col < q.N && mrow < q.M) {
-            store_block(&q.out_map, stg, col, mrow, 0);
-            store_block(&q.out_map, stg + 2048, col, mrow, 1);
-            commit_blocks();
+          if (lane == 0) mbar_arrive(&bars[B_COLSREAD + half]);
+          uint32_t scale = 0;                // 2^e of the four columns as exponent bytes: the largest comes to lie in [2^13, 2^15); e is not below 0 (NaN), nor above 100
+          float inv[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int up = min(max(14 + 127 - (int)((top >> (8 * j) & 127) * 2 + 1), 0), 100);
+            scale |= (uint32_t)(127 + up) << (8 * j);
+            inv[j] = __uint_as_float((uint32_t)(127 - up) << 23);
           }
+          if (quarter == 0 && n0 + 4 * lane < q.N) *reinterpret_cast<float4*>(p.col_inv + tm * p.col_inv_ld + n0 + 4 * lane) = make_float4(inv[0], inv[1], inv[2], inv[3]);
+#pragma unroll
+          for (int c = 0; c < 128; c += 4) {
+            const uint32_t f = __shfl_sync(0xffffffffu, scale, c >> 2);
+            acc[c] *= __uint_as_float(f << 23 & 0x7f800000u); acc[c + 1] *= __uint_as_float(f << 15 & 0x7f800000u);
+            acc[c + 2] *= __uint_as_float(f << 7 & 0x7f800000u); acc[c + 3] *= __uint_as_float(f >> 1 & 0x7f800000u);
+          }
+          store_planes(&p.col_map, stg, acc, n0, mrow, q.N, q.M, lane);
         }
       }
     }
@@ -429,7 +492,7 @@ int make_operand(const Op16& o, int box_mn, OperandDev* d) {
   CUresult r = encode_fn()(&d->map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, o.s.planes, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(VB_ERR_CUDA, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
-  d->inv = o.s.inv; d->inv_ld = o.s.inv_ld; d->mn = o.mn; d->by_row = o.s.by_row;
+  d->inv = o.s.inv; d->inv_ld = o.s.inv_ld; d->mn = o.mn; d->by_m = o.s.scale != Scale16::Block;
   return VB_OK;
 }
 
@@ -477,9 +540,10 @@ int launch(const Params& p, int ctas) {
 
 }  // namespace
 
-Split16 split16_at(void* mem, i64 rows, i64 cols, bool by_row) {
+Split16 split16_at(void* mem, i64 rows, i64 cols, Scale16 scale) {
   Split16 s{};
-  s.rows = rows; s.cols = cols; s.ld = (cols + 7) / 8 * 8; s.plane = rows * s.ld; s.by_row = by_row; s.inv_ld = by_row ? rows : (cols + 127) / 128;
+  s.rows = rows; s.cols = cols; s.ld = (cols + 7) / 8 * 8; s.plane = rows * s.ld; s.scale = scale;
+  s.inv_ld = scale == Scale16::Row ? rows : scale == Scale16::Column ? s.ld : (cols + 127) / 128;
   s.planes = mem;
   s.inv = reinterpret_cast<float*>(static_cast<uint8_t*>(mem) + ((size_t)(2 * s.plane) * 2 + 15) / 16 * 16);
   return s;
@@ -495,7 +559,7 @@ int launch_split16(const SplitJob* jobs, int n, const TargetRows* rows) {
     const Split16& s = jobs[i].to;
     const i64 cb = (s.cols + 127) / 128, blocks = ((s.rows + 127) / 128) * cb;
     d.job[i] = SplitDev{jobs[i].x, jobs[i].keep, (__half*)s.planes, s.inv, s.rows, s.cols, s.ld, s.plane, s.inv_ld, (int)cb, (int)blocks,
-                        s.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(jobs[i].x) & 15) == 0, s.by_row};
+                        s.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(jobs[i].x) & 15) == 0, s.scale == Scale16::Row};
     all += blocks;
     bytes += 8.0 * (double)s.rows * (double)s.cols;
   }
@@ -548,7 +612,12 @@ int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter) {
       q.by_copy = 1; q.add = 0;
       VB_TRY(make_result(&q.out_map, hold[i].p, g.N, g.M, ld, g.M * ld, q.parts, false));
     } else if (q.by_copy) VB_TRY(make_result(&q.out_map, g.out, g.N, g.M, g.ldo, g.ldo * g.M, 1, false));
-    if (what == Tile16::LossGrad) VB_TRY(make_result(&q.out_map, g.grad.planes, g.N, g.M, g.grad.ld, g.grad.plane, 2, true));
+    if (what == Tile16::LossGrad) {
+      const Split16 &y = g.grad, &z = g.grad_by_column;
+      p.with_rows = y.planes != nullptr; p.with_cols = z.planes != nullptr; p.col_inv = z.inv; p.col_inv_ld = z.inv_ld;
+      if (p.with_rows) VB_TRY(make_result(&q.out_map, y.planes, g.N, g.M, y.ld, y.plane, 2, true));
+      if (p.with_cols) VB_TRY(make_result(&p.col_map, z.planes, g.N, g.M, z.ld, z.plane, 2, true));
+    }
     flops += 2.0 * (double)g.M * (double)g.N * (double)g.K;
   }
   p.target = products[0].target; p.col0 = (int)products[0].col0; p.stats = products[0].stats; p.target_value = products[0].target_value; p.lse = products[0].lse;

@@ -5,9 +5,10 @@
 //
 // Forward: one product whose tiles leave (max, sum of exp) for each row and 128 columns, 8 bytes where the logits would be 512, and
 // the target's logit; a second kernel joins the pairs of a row.  Backward: pieces of the vocabulary; a piece's logits are formed
-// again and leave the tensor core as dz in half-precision planes (the operand of the two products that follow), and one launch
+// again and leave the tensor core as dz in half-precision planes, on one scale for dx and with a scale for 128 rows of a class for dW, and one launch
 // adds the piece to dx and writes its rows of dW.  Tensor-bound: 2 N V D and 6 N V D operations, three instructions each (gemm16.cu):
-// 8192 rows, 768 x 50304: 1.39 to 1.56 ms forward, as the power limit has it; 4097 rows, 1024 x 50304, with the gradients 4.6 to 4.9 ms.
+// 8192 rows, 768 x 50304: 1.39 to 1.56 ms forward, as the power limit has it; 4097 rows, 1024 x 50304, with the gradients 4.9 to 5.0 ms (4.7 with the one
+// scale for both).
 // Up to 16 rows it is bound by the bytes of W and takes them in 32 bits, and so do small products of more rows (below).
 #include "gemm16.h"
 #include "head_loss.h"
@@ -345,7 +346,7 @@ int few_rows(const FewParams& p, unsigned ctas, unsigned groups) {
   return p.n <= 8 ? few_rows<8, GRAD>(p, ctas, groups) : few_rows<kFewRows, GRAD>(p, ctas, groups);
 }
 
-// Half-precision planes of a piece of dz: at most half a gigabyte of them at a time.
+// Half-precision planes of a piece of dz: at most half a gigabyte at a time for dx, and as much for dW.
 constexpr i64 kPieceBytes = (i64)512 << 20;
 
 }  // namespace
@@ -367,12 +368,12 @@ int launch_head_loss(const float* x, const float* w, const float* targets, i64 i
     VB_TRY(few_rows<false>(p, (unsigned)(few_blocks < ctx().sm_count ? few_blocks : ctx().sm_count), (unsigned)few_groups));
     return launch_join_stats((const float2*)hs.p, tv, tgt, lse, nll, loss, tgt + n, n, pairs);
   }
-  VB_TRY(scratch_alloc(split16_bytes(n, d, true), &hx.p));
+  VB_TRY(scratch_alloc(split16_bytes(n, d, Scale16::Row), &hx.p));
   VB_TRY(scratch_alloc(split16_bytes(v, d), &hw.p));
   VB_TRY(scratch_alloc((size_t)(pairs * n) * sizeof(float2), &hs.p));
   VB_TRY(scratch_alloc((size_t)n * 12 + 8, &hr.p));
   float* nll = (float*)hr.p; float* tv = nll + n; int* tgt = (int*)(tv + n); int* counters = tgt + n;
-  const Split16 sx = split16_at(hx.p, n, d, true), sw = split16_at(hw.p, v, d);
+  const Split16 sx = split16_at(hx.p, n, d, Scale16::Row), sw = split16_at(hw.p, v, d);
   const SplitJob jobs[2] = {{x, sx}, {w, sw}};
   const TargetRows rows{targets, ignore, v, tgt, counters, 2};
   VB_TRY(launch_split16(jobs, 2, &rows));
@@ -385,7 +386,7 @@ int launch_head_loss(const float* x, const float* w, const float* targets, i64 i
 
 int launch_head_loss_backward(const float* x, const float* w, const float* targets, i64 ignore, const float* lse, const float* g, float* gx, float* gw,
                               i64 n, i64 d, i64 v) {
-  Temp hx, hk, hw, hz, ht;
+  Temp hx, hk, hw, hz, hc, ht;
   const i64 few_blocks = (v + kFewCols - 1) / kFewCols, few_groups = (n + kFewRows - 1) / kFewRows;
   // Up to 16 rows, or one wave of blocks that are not wide (a block's three products take 16 x 64 x d each on the ordinary cores) and not of many groups (whose
   // parts of dW are added).  With gradients, this way / by way of planes, us: 17 rows of 64, 700 columns 38 / 52; 100 of 512, 1000: 54 / 72; 500 of 128, 256: 49 / 57;
@@ -419,13 +420,14 @@ int launch_head_loss_backward(const float* x, const float* w, const float* targe
   const i64 pieces = (v + piece - 1) / piece;
   piece = ((v + pieces - 1) / pieces + 255) / 256 * 256;
   if (piece > v) piece = v;
-  VB_TRY(scratch_alloc(split16_bytes(n, d, true), &hx.p));
+  VB_TRY(scratch_alloc(split16_bytes(n, d, Scale16::Row), &hx.p));
   if (gw) VB_TRY(scratch_alloc(split16_bytes(n, d), &hk.p));
   VB_TRY(scratch_alloc(split16_bytes(v, d), &hw.p));
-  VB_TRY(scratch_alloc(split16_bytes(n, piece), &hz.p));
+  if (gx) VB_TRY(scratch_alloc(split16_bytes(n, piece), &hz.p));
+  if (gw) VB_TRY(scratch_alloc(split16_bytes(n, piece, Scale16::Column), &hc.p));
   VB_TRY(scratch_alloc((size_t)(n + 2 * pieces) * 4 + 16, &ht.p));
   float* coef = (float*)ht.p; int* tgt = (int*)(coef + 4); int* counters = tgt + n;
-  const Split16 sx = split16_at(hx.p, n, d, true), sw = split16_at(hw.p, v, d);      // x for the logits, where its rows are the product's,
+  const Split16 sx = split16_at(hx.p, n, d, Scale16::Row), sw = split16_at(hw.p, v, d);      // x for the logits, where its rows are the product's,
   const Split16 sk = gw ? split16_at(hk.p, n, d) : sx;                                  // and for dW, which sums over them
   k_targets<<<1, 1024, 0, ctx().stream>>>(targets, n, ignore, v, tgt, g, coef, counters, (int)(2 * pieces), ctx().d_err);
   VB_LAUNCH_CHECK();
@@ -435,12 +437,16 @@ int launch_head_loss_backward(const float* x, const float* w, const float* targe
     const i64 vc = v - v0 < piece ? v - v0 : piece;
     Split16 wc = sw;                                     // this piece's rows of W
     wc.planes = (uint16_t*)sw.planes + v0 * sw.ld; wc.inv = sw.inv + v0 / 128 * sw.inv_ld; wc.rows = vc;
-    Split16 z = split16_at(hz.p, n, vc);
+    // A row of dx sums over classes whose probabilities add up to 1, so one scale does for all of them.  A row of dW belongs to one class, however
+    // improbable: its dz are held on the scale of the largest among 128 rows (with the one scale, a class at e^-30 kept a bit or two).
+    Split16 z{}, zc{};
+    if (gx) z = split16_at(hz.p, n, vc);
+    if (gw) zc = split16_at(hc.p, n, vc, Scale16::Column);
+    z.inv = nullptr;
     Product16 f{};
     f.a = Op16{sx, false}; f.b = Op16{wc, false}; f.M = n; f.N = vc; f.K = d;
-    f.target = tgt; f.col0 = v0; f.lse = lse; f.grad = z;
+    f.target = tgt; f.col0 = v0; f.lse = lse; f.grad = z; f.grad_by_column = zc;
     VB_TRY(launch_gemm16(Tile16::LossGrad, &f, 1, counters));
-    z.inv = nullptr;
     Product16 b[2] = {};
     int nb = 0;
     if (gx) {
@@ -450,7 +456,7 @@ int launch_head_loss_backward(const float* x, const float* w, const float* targe
     }
     if (gw) {
       Product16& q = b[nb++];
-      q.a = Op16{z, true}; q.b = Op16{sk, true}; q.M = vc; q.N = d; q.K = n;
+      q.a = Op16{zc, true}; q.b = Op16{sk, true}; q.M = vc; q.N = d; q.K = n;
       q.out = gw + v0 * d; q.ldo = d; q.alpha = coef; q.alpha_host = 1.0f / 16384.0f;
     }
     if (nb) VB_TRY(launch_gemm16(Tile16::Store, b, nb, counters + 1));
