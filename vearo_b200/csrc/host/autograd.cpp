@@ -286,7 +286,7 @@ std::pair<Tensor, Tensor> Tensor::qk_norm_rope(const Tensor& q, const Tensor& k,
 }
 // saved behind the inputs: the output; extra: the rows' log-sum-exp
 Tensor Tensor::segment_attention(const Tensor& k, const Tensor& v, const Tensor& starts, float scale) const {
-  const bool rec = t_enabled && (requires_grad() || k.requires_grad() || v.requires_grad());
+  const bool rec = t_enabled && (requires_grad() || k.requires_grad() || v.requires_grad() || starts.requires_grad());      // (whether record() makes a node)
   vb_tensor o_, l_;
   check(vb_segment_attention(&d_, &k.d_, &v.d_, &starts.d_, scale, &o_, rec ? &l_ : nullptr), "segment_attention");
   Tensor out = Tensor::adopt(o_), lse;
@@ -295,7 +295,7 @@ Tensor Tensor::segment_attention(const Tensor& k, const Tensor& v, const Tensor&
   return out;
 }
 Tensor Tensor::linear_cross_entropy(const Tensor& weight, const Tensor& targets, i64 ignore_index) const {
-  const bool rec = t_enabled && (requires_grad() || weight.requires_grad());
+  const bool rec = t_enabled && (requires_grad() || weight.requires_grad() || targets.requires_grad());
   vb_tensor o_, l_;
   check(vb_linear_cross_entropy(&d_, &weight.d_, &targets.d_, ignore_index, &o_, rec ? &l_ : nullptr), "linear_cross_entropy");
   Tensor out = Tensor::adopt(o_), lse;
