@@ -91,3 +91,36 @@ def test_values_of_one_text_do_not_take_bits_from_another(vb, starts, power, hq,
     vals, errs = bounded_by_text(q, k, v, starts, dk ** -0.5, g)
     for x, want, err, name in zip(got, vals, errs, ("dq", "dk", "dv")):
         assert (np.abs(x - want) <= err).all(), (name, (np.abs(x - want) / np.maximum(err, 1e-300)).max())
+
+
+@pytest.mark.parametrize("T", [2 ** 23 + 2, 2 ** 24])
+def test_the_last_offset_of_a_long_pack(vb, T):
+    """Offsets of which neighbours are one step of f32 apart: T is a whole number of them, T + 1 rounds to one as well."""
+    a = rnd(21, 300)
+    slots = []
+
+    def far(tail):      # [T, 1, 1], zeros with `tail` in its last rows
+        slot = C.c_uint32()
+        vb.vb_check(vb.lib().vb_alloc(T, 1, C.byref(slot)))
+        vb.vb_check(vb.lib().vb_write(slot.value, T - tail.size, tail.ctypes.data_as(vb.c_f32p), tail.size))
+        vb.sync()
+        slots.append(slot.value)
+        return vb.VbTensor.contiguous(slot.value, (T, 1, 1))
+    x = far(a)
+    out = vb.VbTensor()
+    starts = Dev(vb, np.array([T - 300, T - 100, T], np.float32))
+    vb.vb_check(vb.lib().vb_segment_attention(C.byref(x), C.byref(x), C.byref(x), starts.ref, 1.0, C.byref(out), None))
+    vb.check_errors()
+    got = np.empty(300, np.float32)
+    vb.vb_check(vb.lib().vb_read(out.slot, T - 300, got.ctypes.data_as(vb.c_f32p), 300))
+    vb.lib().vb_release(out.slot, None)
+    want = np.concatenate([segment_attention(a[s, None, None], a[s, None, None], a[s, None, None], [0, n], 1.0, err=False)[0][:, 0, 0]
+                           for s, n in ((slice(0, 200), 200), (slice(200, 300), 100))])
+    assert np.abs(got - want).max() <= 200 * 2.0 ** -24 * np.abs(a).max() * (1 + np.abs(a).max() ** 2)      # (57 U of a score of at most max^2, 80 U of the sum)
+    bad = Dev(vb, np.array([T - 300, T - 100, T + 2], np.float32))
+    vb.vb_check(vb.lib().vb_segment_attention(C.byref(x), C.byref(x), C.byref(x), bad.ref, 1.0, C.byref(out), None))
+    vb.lib().vb_release(out.slot, None)
+    with pytest.raises(vb.VearoError):
+        vb.check_errors()
+    for s in slots:
+        vb.lib().vb_release(s, None)

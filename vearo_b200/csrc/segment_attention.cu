@@ -77,7 +77,7 @@ __device__ __forceinline__ void find_segment(const PrepareDev& p, const float* s
   for (int i = t; i <= p.n_seg; i += p.tiles * 128) {
     const float s = starts[i];
     if (!(s > -0.5f)) atomicOr(p.err, ERRBIT_NEG_ID);
-    else if (!(s < (float)p.T + 0.5f) || (i > 0 && !(starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
+    else if (!(roundf(s) <= (float)p.T) || (i > 0 && !(starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
   }
   if (t >= p.T) return;
   const int2 r = segment_at(p, starts, t);
