@@ -124,3 +124,22 @@ def test_the_last_offset_of_a_long_pack(vb, T):
         vb.check_errors()
     for s in slots:
         vb.lib().vb_release(s, None)
+
+
+@pytest.mark.parametrize("starts,fine", [([0], True), ([0, 0, 0], True), ([0, 5], False), ([-3, 0], False), ([0, np.nan], False)])
+def test_offsets_of_no_rows(vb, starts, fine):
+    x = np.zeros((0, 2, 16), np.float32)
+    out, lse = forward(vb, x, x, x, np.array(starts, np.float32), 0.5)
+    assert out.shape == (0, 2, 16) and lse.shape == (2, 0)
+    if fine:
+        vb.check_errors()
+    else:
+        with pytest.raises(vb.VearoError):
+            vb.check_errors()
+    grads = gradients(vb, x, x, x, np.array(starts, np.float32), 0.5, out, lse, x)
+    assert all(g.shape == x.shape for g in grads)
+    if fine:
+        vb.check_errors()
+    else:
+        with pytest.raises(vb.VearoError):
+            vb.check_errors()

@@ -183,7 +183,8 @@ int vb_segment_attention(const vb_tensor* q, const vb_tensor* k, const vb_tensor
   const i64 ld[2] = {s.hq, s.T};
   VB_TRY(outs.add(out, 3, q->dims, &po));
   if (lse) VB_TRY(outs.add(lse, 2, ld, &pl));
-  if (s.T > 0) VB_TRY(launch_segment_attention(s, vq, vk, vv, ps, starts->dims[0] - 1, po, pl));
+  if (s.T == 0) VB_TRY(launch_check_offsets(ps, starts->dims[0] - 1));
+  else VB_TRY(launch_segment_attention(s, vq, vk, vv, ps, starts->dims[0] - 1, po, pl));
   outs.done();
   return VB_OK;
 }
@@ -205,7 +206,8 @@ int vb_segment_attention_backward(const vb_tensor* q, const vb_tensor* k, const 
   Outputs outs;
   float *pdq, *pdk, *pdv;
   VB_TRY(outs.add(dq, 3, q->dims, &pdq)); VB_TRY(outs.add(dk, 3, k->dims, &pdk)); VB_TRY(outs.add(dv, 3, v->dims, &pdv));
-  if (s.T > 0) VB_TRY(launch_segment_attention_backward(s, vq, vk, vv, ps, starts->dims[0] - 1, vo, pl, vg, pdq, pdk, pdv));
+  if (s.T == 0) VB_TRY(launch_check_offsets(ps, starts->dims[0] - 1));
+  else VB_TRY(launch_segment_attention_backward(s, vq, vk, vv, ps, starts->dims[0] - 1, vo, pl, vg, pdq, pdk, pdv));
   outs.done();
   return VB_OK;
 }

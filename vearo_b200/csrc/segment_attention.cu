@@ -72,13 +72,19 @@ __device__ __forceinline__ int2 segment_at(const PrepareDev& p, const float* sta
   const int b = fb > 0.0f ? (int)fb : 0, e = fe < (float)p.T ? (int)fe : p.T;
   return b <= t && t < e ? make_int2(b, e) : make_int2(p.T, 0);
 }
-// A row's segment.  Offsets that decrease or leave [0, T] are reported.
+// Offsets that decrease or leave [0, T] are reported.
+__device__ __forceinline__ void check_offset(const float* starts, int i, int T, int* err) {
+  const float s = starts[i];
+  if (!(s > -0.5f)) atomicOr(err, ERRBIT_NEG_ID);
+  else if (!(roundf(s) <= (float)T) || (i > 0 && !(starts[i - 1] <= s))) atomicOr(err, ERRBIT_OOB_ID);
+}
+// of a pack without rows, which has no other work
+__global__ void __launch_bounds__(256) k_check_offsets(const float* __restrict__ starts, int n, int* err) {
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) check_offset(starts, i, 0, err);
+}
+// A row's segment.
 __device__ __forceinline__ void find_segment(const PrepareDev& p, const float* starts, int t) {
-  for (int i = t; i <= p.n_seg; i += p.tiles * 128) {
-    const float s = starts[i];
-    if (!(s > -0.5f)) atomicOr(p.err, ERRBIT_NEG_ID);
-    else if (!(roundf(s) <= (float)p.T) || (i > 0 && !(starts[i - 1] <= s))) atomicOr(p.err, ERRBIT_OOB_ID);
-  }
+  for (int i = t; i <= p.n_seg; i += p.tiles * 128) check_offset(starts, i, p.T, p.err);
   if (t >= p.T) return;
   const int2 r = segment_at(p, starts, t);
   p.begin[t] = r.x; p.end[t] = r.y;
@@ -1302,6 +1308,12 @@ int backward(Work& w, float* dq, float* dk, float* dv) {
 
 }  // namespace
 
+int launch_check_offsets(const float* starts, i64 n) {
+  const i64 ctas = (n + 256) / 256, cap = ctx().sm_count;
+  k_check_offsets<<<(unsigned)(ctas < cap ? ctas : cap), 256, 0, ctx().stream>>>(starts, (int)n + 1, ctx().d_err);
+  VB_LAUNCH_CHECK();
+  return VB_OK;
+}
 int launch_segment_attention(const SegShape& s, const SegHeads& q, const SegHeads& k, const SegHeads& v, const float* starts, i64 n, float* out, float* lse) {
   Work w;
   const SegHeads in[3] = {q, k, v};
