@@ -233,11 +233,11 @@ int vb_layernorm_backward_accum(const vb_tensor* x, const vb_tensor* w, const vb
  * read in place while the components of a head are contiguous, else copied), outputs fresh and contiguous.  The calls run
  * on the library's device whatever device is current, and are refused (VB_ERR_UNSUPPORTED) while the compute stream is being captured.
  * Output descriptors are written last, so they may be those of inputs.  Matrix products run on pairs of half-precision planes that share a power
- * of two per block: 22 significant bits for magnitudes down to 2^-17 of the block's largest, an absolute error of 2^-40 of that largest below.  A
- * block is 128 rows of a head in vb_segment_attention (rows of no segment count as 0; the gradient of a row's scores is held to 2^-37 of the longest
- * gradient row of 128 times twice the longest value row of the row's own segment), in vb_linear_cross_entropy 128 x 128 of the weight, 128 columns
- * of a row of x (in dW 128 x 128 of x), and of the logits' gradients 128 rows of a class in dW and the whole matrix, its largest being 1, in dx (up
- * to 16 rows, or few rows times few columns: plain f32).
+ * of two per block: 22 significant bits for magnitudes down to 2^-17 of the block's largest, an absolute error of 2^-40 of that largest below.
+ * Blocks of vb_segment_attention: 128 rows of a head (rows of no segment count as 0).  Its weights are held to 2^-38 of the row's largest in out and
+ * of 1 in dv, the gradient of a row's scores to 2^-37 of the longest gradient row of 128 times twice the longest value row of the row's own segment.
+ * Blocks of vb_linear_cross_entropy: 128 x 128 of the weight, 128 columns of a row of x (in dW 128 x 128 of x), and of the logits' gradients 128
+ * rows of a class in dW and all of them, their largest being 1, in dx (up to 16 rows, or few rows times few columns: plain f32).
  *
  * RMS norm of every head and the rotary position turn, one pass for queries and keys (k, wk, k_out all NULL: queries alone):
  *   y = w * x / sqrt(mean(x^2) + eps);   pair j of a head turned by positions[t] * theta^(-2j / rot_dim).
@@ -265,8 +265,9 @@ int vb_segment_attention_backward(const vb_tensor* q, const vb_tensor* k, const 
                                   const vb_tensor* lse, const vb_tensor* grad_out, vb_tensor* dq, vb_tensor* dk, vb_tensor* dv);
 /* The vocabulary projection and its softmax cross entropy without the logits in memory: vb_linear (no bias) followed by
  * vb_cross_entropy.  x: [.., D] (rows = all leading dims), weight: [V, D], targets: as many classes as rows.  loss (shape [1]) is the
- * mean over the rows whose target is not ignore_index; 0 when there are none.  A negative or too large target that is not
- * ignore_index sets the device error flag, and its row is left out.  lse (may be NULL; [rows]): log of the sum of exponentials of every
+ * mean over the rows whose target is not ignore_index; 0 when there are none.  What a row of x with a component that is not finite enters is not
+ * finite (of a row that is left out, its lse alone); a weight that is not finite may make NaN of everything.  A negative or too large target that is
+ * not ignore_index sets the device error flag, and its row is left out.  lse (may be NULL; [rows]): log of the sum of exponentials of every
  * row, which the backward call wants.  The backward call forms the logits again, a piece of the vocabulary at a time; gx or gw may be NULL.
  * V <= 2^24.  Workspace: 4 bytes for every number of x and of the weight, 8 for every row and 128 classes; backward, 4 bytes for every number of the
  * weight and of x (twice for x where gw is wanted), half a gigabyte for a piece of the logits' gradients for each of gx and gw (more from 2^19 rows

@@ -119,7 +119,7 @@ enum { B_FULL = 0, B_EMPTY = B_FULL + kStages, B_RUN = B_EMPTY + kStages, B_RUNF
 static_assert(B_COUNT * 8 + 16 <= 256, "barriers");
 
 __device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// (as an instruction of its own: the compiler's form of atomicAdd waits for the answer on the spot)
+// (asked for here, looked at when the copies of the tile in hand have been issued)
 __device__ __forceinline__ int next_tile(int* counter) {
   int r;
   asm volatile("atom.global.add.s32 %0, [%1], 1;" : "=r"(r) : "l"(counter) : "memory");

@@ -46,7 +46,7 @@ struct Product16 {
   Split16 grad, grad_by_column;                  // [M, N]; planes null: not wanted.  grad holds 2^14 times the values and has no scales
 };
 // n <= 2 (Store), independent of one another, one launch (and one for each whose long sums are formed in parts); counter: an int on the device that is 0 when the launch begins.  The RowStats
-// kernel may start while the kernel ahead of it runs and waits for it by itself.
+// kernel is launched by launch_early and waits for the kernel ahead of it by itself.
 int launch_gemm16(Tile16 what, const Product16* products, int n, int* counter);
 
 }  // namespace vb

@@ -1283,7 +1283,8 @@ int backward(Work& w, float* dq, float* dk, float* dv) {
   // A CTA that walks the query heads of a whole group is the longest of the launch, and dealing the group to several costs their parts' sums and
   // more CTAs.  So it is dealt out until a CTA's heads are no more than an SM's share of the launch: 3 tiles' worth for every query head.
   // Gradient, group in one CTA / dealt to as many as make four for every SM / by this rule: 4096 tokens in 9 texts, 16 + 4 heads of 64 131 / 176 / 131 us;
-  // 1531 in 3, 6 + 2 of 80 113 / 63 / 63; 1024 in one, 16 + 2 of 64 122 / 53 / 45; 8192 in 4, 16 + 4 of 128 884 / 1000 / 889.
+  // 1531 in 3, 6 + 2 of 80 113 / 63 / 63; 1024 in one, 16 + 2 of 64 122 / 53 / 45; 8192 in 4, 16 + 4 of 128 884 / 1000 / 889.  It counts tiles and not the
+  // lengths of texts, which the host does not know; by the rule / in two parts: 4096 in one text, 8 + 2 of 64 234 / 186; 600 in two, 4 + 1 of 96 37 / 33.
   const int group = p.hq / p.hk;
   p.parts = 1;
   for (int d = 2; d <= group && (i64)group * ctx().sm_count > 3 * (i64)p.tiles * p.hq * p.parts; ++d) if (group % d == 0) p.parts = d;

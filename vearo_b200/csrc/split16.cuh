@@ -65,9 +65,8 @@ __device__ __forceinline__ uint64_t desc16(uint32_t smem_addr, uint32_t block_by
 __device__ __forceinline__ uint32_t idesc16(int m, int n, int a_mn, int b_mn) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// The issuing warp runs converged and one lane of it, the leader, executes the instruction: addresses and descriptors then stay in
-// uniform registers.  (One lane of a diverged warp costs its instruction six moves into them, 65-75 cycles an MMA: more than a
-// 128 x 128 x 16 product takes.)
+// The issuing warp runs converged and one lane of it, the leader, executes the instruction.  (Issued by one lane of a diverged warp, MMAs came 65-75
+// cycles apart by the clock, more than a 128 x 128 x 16 product takes: attention of 16384 tokens, 8 + 2 heads of 128, 1359 us instead of 1063.)
 __device__ __forceinline__ uint32_t elect_leader() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
@@ -126,7 +125,8 @@ __device__ __forceinline__ int read_target(float v, i64 ignore, i64 vocab, int* 
 }
 // of a kernel launched by launch_early: nothing that the kernel ahead of it in the stream writes is touched before this
 __device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// a launch that may begin while the kernel ahead of it in the stream still runs
+// A launch that is made ready while the kernel ahead of it in the stream still runs.  No kernel here lets its successor go before its own end, so what is
+// saved is the launch's latency, not time of the kernel ahead.
 template <class... P, class... A>
 int launch_early(void (*kernel)(P...), dim3 ctas, dim3 threads, int smem, A... args) {
   cudaLaunchAttribute at{};
