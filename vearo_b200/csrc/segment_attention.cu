@@ -24,7 +24,7 @@
 //
 // Bound by the tensor cores where texts are long (16384 tokens, 8 + 2 heads of 128: k_forward 1067 us, 517 TFLOP/s useful, 1550 issued, at the
 // 1.53 GHz that the power limit leaves), by what a CTA does before its first tile and after its last where they are short: about 10 of 23
-// thousand cycles for four tiles (4096 tokens in 9 texts, 16 + 4 heads of 64: k_forward 55 us, k_backward 172; 8 texts of 1024, 12 heads: 73), and by
+// thousand cycles for four tiles (4096 tokens in 9 texts, 16 + 4 heads of 64: k_forward 53 us, k_backward 130 to 146; 8 texts of 1024, 12 heads: 71), and by
 // the chain of tiles of the longest text where there are fewer CTAs than SMs (1357 of 1531 tokens, 6 + 2 heads of 80: 35 and 66 us).
 // 128 x 128 tiles and one CTA an SM: two streamed operands, four planes each, fill shared memory, and scores in two buffers with what
 // follows from them tensor memory; two smaller CTAs an SM, and one that takes tiles from a counter, measured no better.
