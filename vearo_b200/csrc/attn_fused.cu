@@ -674,21 +674,6 @@ k_attn_bwd_dq(const __grid_constant__ CUtensorMap map_v, const __grid_constant__
 }
 
 // ---- host side --------------------------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeTiledFn)p;
-    else cudaGetLastError();
-  }
-  return fn;
-}
 // [B,H,S,64] view with element strides {sb, sh, ss, 1}: dims {64, S, H, B}; boxes of 32 columns x `rows` rows
 int head_map(CUtensorMap* map, const float* base, i64 S, i64 H, i64 B, i64 ss, i64 sh, i64 sb, int rows, CUtensorMapSwizzle sw) {
   cuuint64_t dims[4] = {64, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};

@@ -118,7 +118,6 @@ struct Params {
 enum { B_FULL = 0, B_EMPTY = B_FULL + kStages, B_RUN = B_EMPTY + kStages, B_RUNFREE = B_RUN + 2, B_POST = B_RUNFREE + 2, B_TAKEN = B_POST + 2, B_COLS = B_TAKEN + 2, B_COLSREAD = B_COLS + 2, B_COUNT = B_COLSREAD + 2 };
 static_assert(B_COUNT * 8 + 16 <= 256, "barriers");
 
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 // (asked for here, looked at when the copies of the tile in hand have been issued)
 __device__ __forceinline__ int next_tile(int* counter) {
   int r;
@@ -252,13 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
           }
         }
       }
-      if (*abort_flag) {      // give copies already issued a bounded time to land before the CTA exits
-        for (int i = 0; i < kStages; ++i) {
-          uint32_t addr = smem_u32(&bars[B_FULL + i]), done = 0;
-          for (uint32_t n = 0; n < (1u << 14) && !done; ++n)
-            asm volatile("{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(done) : "r"(addr), "r"(0u) : "memory");
-        }
-      }
+      if (*abort_flag) let_land(&bars[B_FULL], kStages);
     }
   } else if (warp == 1) {
     const uint32_t leader = elect_leader();
@@ -469,20 +462,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_gemm16(const __grid_constant__ 
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
   if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, ERRBIT_WAIT_TIMEOUT);
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) return (EncodeTiledFn)p;
-    cudaGetLastError();
-    return (EncodeTiledFn) nullptr;
-  }();
-  return fn;
 }
 
 int make_operand(const Op16& o, int box_mn, OperandDev* d) {

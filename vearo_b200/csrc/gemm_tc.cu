@@ -637,22 +637,6 @@ __global__ void __launch_bounds__(256) k_tf32_lo(const float* __restrict__ x, fl
 }
 
 // ---- host side --------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (!tried) {
-    tried = true;
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) fn = (EncodeTiledFn)p;
-    else cudaGetLastError();
-  }
-  return fn;
-}
-
 struct Operand { const float* p; i64 rows, rs, b1, b2; bool bc1, bc2; bool mn; };   // [rows, K]; rs = row stride (K-major) or k stride (MN-major)
 
 bool tma_ok(const Operand& o, i64 nb1, i64 nb2) {

@@ -40,7 +40,6 @@ constexpr float kL2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float2 lo2(const float4& v) { return make_float2(v.x, v.y); }
 __device__ __forceinline__ float2 hi2(const float4& v) { return make_float2(v.z, v.w); }
-__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
 // ---- planes ------------------------------------------------------------------------------------------------------------------------
 // One of q, k, v, do: planes [2][heads][T][DP], and per head and tile the inverse scale (negative where a component is not finite), the
@@ -468,14 +467,6 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
 }
 __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
-}
-// copies already issued get a bounded time to land before a CTA that gave up exits
-__device__ __forceinline__ void let_land(uint64_t* bars, int n) {
-  for (int i = 0; i < n; ++i) {
-    uint32_t addr = smem_u32(&bars[i]), done = 0;
-    for (uint32_t k = 0; k < (1u << 14) && !done; ++k)
-      asm volatile("{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(done) : "r"(addr), "r"(0u) : "memory");
-  }
 }
 // a row warp has written its operand (and read the last accumulator)
 __device__ __forceinline__ void operand_written(uint64_t* bar, int lane) {
@@ -1186,19 +1177,6 @@ __global__ void __launch_bounds__(256) k_add_parts(const V* __restrict__ a, cons
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) return (EncodeTiledFn)p;
-    cudaGetLastError();
-    return (EncodeTiledFn) nullptr;
-  }();
-  return fn;
-}
 int make_map(CUtensorMap* map, const PlanesDev& x, int T, int dp, int rows) {
   if (!encode_fn()) return set_error(VB_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const cuuint64_t row = (cuuint64_t)dp * 2;

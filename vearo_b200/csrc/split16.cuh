@@ -29,6 +29,7 @@ __device__ __forceinline__ float block_scale(float amax, float* inverse) {
   *inverse = __uint_as_float((uint32_t)(127 - e) << 23);
   return __uint_as_float((uint32_t)(127 + e) << 23);
 }
+__device__ __forceinline__ float exp2_fast(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 __device__ __forceinline__ float finite_abs(float x) { const float a = fabsf(x); return a <= 3.402823466e38f ? a : 0.0f; }
 

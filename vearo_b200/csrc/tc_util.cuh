@@ -3,9 +3,26 @@
 // the MMA / commit / tensor-memory load and store wrappers, and the TF32 remainder ("lo") of an f32 value.
 #pragma once
 #include <cuda.h>
+#include <cuda_runtime.h>
 #include <cstdint>
 
 namespace vb {
+
+// host: the driver's encoder of tensor maps; null where there is none
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess) return (EncodeTiledFn)p;
+    cudaGetLastError();
+    return (EncodeTiledFn) nullptr;
+  }();
+  return fn;
+}
+
 namespace tc {
 
 constexpr uint32_t kSpinLimit = 1u << 20; // polls of try_wait (each waits a bounded time) before giving up
@@ -61,6 +78,15 @@ __device__ __forceinline__ void tma_store_block(const CUtensorMap* map, const vo
 }
 // The issuing thread's earlier block stores have finished reading shared memory.
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// Copies already issued get a bounded time to land before a CTA that gave up exits: the first phase of each of their barriers.
+__device__ __forceinline__ void let_land(uint64_t* bars, int n) {
+  for (int i = 0; i < n; ++i) {
+    uint32_t addr = smem_u32(&bars[i]), done = 0;
+    for (uint32_t k = 0; k < (1u << 14) && !done; ++k)
+      asm volatile("{\n\t.reg .pred q;\n\tmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(done) : "r"(addr), "r"(0u) : "memory");
+  }
+}
 
 // Shared-memory matrix descriptor, K-major: rows of bk floats -- 64 bytes with SWIZZLE_64B (bk = 16) or 128 bytes with
 // SWIZZLE_128B (bk = 32) -- and 8-row groups 512 / 1024 bytes apart.
