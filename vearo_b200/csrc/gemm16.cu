@@ -133,7 +133,8 @@ __device__ __forceinline__ void add_block(const CUtensorMap* map, const void* sr
 __device__ __forceinline__ void commit_blocks() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 
 // A warp's 32 rows x 128 columns as half planes, 32 x 32 blocks through its staging: 16-byte pieces of a plane's 64-byte row, in the copy
-// engine's 64-byte swizzle.  (Ordinary stores, from the staging or of 32 bytes a thread, took LossGrad from 648 to 780 and 688 us.)
+// engine's 64-byte swizzle.  (Ordinary stores, of 64 bytes of a row from the staging or 32 a thread, took LossGrad of
+// 4097 rows, 1024 x 25152 columns, then at 648 us with the butterfly below, to 780 and 688; it takes 609.)
 __device__ __forceinline__ void store_planes(const CUtensorMap* map, uint8_t* stg, const float (&acc)[128], int n0, int row, int N, int M, int lane) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {

@@ -438,7 +438,7 @@ int launch_head_loss_backward(const float* x, const float* w, const float* targe
     Split16 wc = sw;                                     // this piece's rows of W
     wc.planes = (uint16_t*)sw.planes + v0 * sw.ld; wc.inv = sw.inv + v0 / 128 * sw.inv_ld; wc.rows = vc;
     // A row of dx sums over classes whose probabilities add up to 1, so one scale does for all of them.  A row of dW belongs to one class, however
-    // improbable: its dz are held on the scale of the largest among 128 rows (with the one scale, a class at e^-30 kept a bit or two).
+    // improbable: its dz are held on the scale of the largest among 128 rows (with the one scale, a class at e^-20 kept some twelve bits, one at e^-30 none).
     Split16 z{}, zc{};
     if (gx) z = split16_at(hz.p, n, vc);
     if (gw) zc = split16_at(hc.p, n, vc, Scale16::Column);
